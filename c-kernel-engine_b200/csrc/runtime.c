@@ -134,6 +134,12 @@ int ckb200_init(int device)
 }
 
 int ckb_ensure_init(void) { return g.inited ? 0 : ckb200_init(-1); }
+int ckb_check_device(const char *what)
+{
+    int now = -1;
+    if (ckb_check_cuda((int)cudaGetDevice(&now), what)) return CKB_ERR_CUDA;
+    return now == g.device ? 0 : ckb_fail(CKB_ERR_STATE, "%s: the current device is %d, the library runs on device %d", what, now, g.device);
+}
 int ckb_sm_count(void) { return g.sm_count > 0 ? g.sm_count : 148; }
 int *ckb_device_error_word(void) { return g.dev_err; }
 void *ckb200_stream(void) { return ckb_ensure_init() ? NULL : (void *)g.stream; }

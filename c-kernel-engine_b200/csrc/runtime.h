@@ -13,6 +13,7 @@ enum { CKB_SLOT_W = 0, CKB_SLOT_X = 1, CKB_SLOT_Y = 2, CKB_SLOT_A = 3, CKB_SLOT_
 
 int ckb_ensure_init(void);                 /* 0 or CKB_ERR_NO_DEVICE; initialises on first use */
 int ckb_sm_count(void);
+int ckb_check_device(const char *what);     /* 0, or CKB_ERR_STATE when the caller's current device is not the library's */
 int *ckb_device_error_word(void);
 cudaStream_t ckb_stream(void *user);       /* user stream, or the library stream when NULL */
 int ckb_on_own_stream(void *user);         /* that is the library stream, and no capture is running on it */
