@@ -1,7 +1,27 @@
-// Causal attention over a paged 4-bit KV cache (include/ckb200_cache.h).
+// Causal attention over a paged 4-bit KV cache (include/ckb200_cache.h), one or several new tokens of each sequence, on the tensor cores at fp32
+// accuracy.
 //
-// One CTA per (query token, head): its warps take every fourth visible key, a lane the codes of head_dim / 32 values, with a running
-// maximum and sum each; the four are merged at the end.
+// Mathematics.  A key block of 32 channels is k = d c + m with 4-bit codes c, so a score is sum over blocks of d (q . c) + m (sum q), and
+// the output of a block's channels is sum over keys of (p d) c + sum p m.  Both inner products have a 4-bit integer on one side, which as an
+// fp16 operand is exact; the other side, fp32, goes in as two fp16 pieces (x = hi + lo, 22 bits), whose products add up in the same fp32
+// accumulators.  The codes are never converted: a nibble in bits 4..7 of a half IS the subnormal 16 c * 2^-24, so masks and shifts of a
+// 32-bit word of codes make A operands, and the power of two is taken out of the result.  (Not in bits 0..3: the tensor cores line products
+// up without normalising them, and what a subnormal has in leading zeros is lost below: 2e-5 of the result at 500 keys.)  Queries are scaled so
+// that the largest of a row is in [2^14, 2^15); weights p d by 2^e, e from the largest d so far, kept with the running maximum as one reference
+// (accumulators hold values relative to 2^ref, ref = max - e): neither piece falls out of fp16's range whatever the cache's magnitude.
+//
+//   scores  S^T = K Q^T   mma.m16n8k16: 16 keys x 8 query rows; a thread's A words are 4 bytes of codes of keys g and g + 8 (lane = 4 g + t), which
+//                         settles which channel sits at which k: the query's fragments are laid out to match
+//   output  O^T = V^T P^T 16 channels x 8 query rows; A words are the same two bytes (four channels) of two keys, joined by one byte permute
+//
+// A query row is a (token, head) of the kv head's group: up to 8 NB rows share every code that is unpacked (NB = 1 for decoding, more for
+// drafts and portions of prompts).
+//
+// Work.  A unit is 128 keys of one (sequence, kv head, 8 NB rows); the units of all sequences form one line that is cut evenly among the CTAs that
+// the GPU holds at once, so long and short sequences load it alike and nothing but the lengths on the device decides.  Each of the four warps takes
+// 32 keys of a unit through a ring of its own (untiled bulk copies of 16-key pieces, the largest that never leave a page), without meeting the
+// others until a sequence's stretch ends.  Stretches that lie within one CTA are written out at once, the others as partial results that
+// a second kernel joins (log-sum-exp).
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -9,77 +29,673 @@
 #include "device_common.cuh"
 #include "kv_q4.cuh"
 #include "launch.h"
+#include "pdl.cuh"
 #include "runtime.h"
 
 namespace ckb {
 
-constexpr int AQ_WARPS = 4, AQ_THREADS = 32 * AQ_WARPS;
+constexpr int AQ_WARPS = 4, AQ_THREADS = 32 * AQ_WARPS, AQ_CHUNK = 32, AQ_UNIT = AQ_WARPS * AQ_CHUNK;
+constexpr int AQ_SP = 40;                      // floats between rows of the score exchange: 8 lanes' float2 loads touch every bank once
+constexpr int AQ_MERGE_WARPS = 8;
 
-template <int NB>
-__global__ void __launch_bounds__(AQ_THREADS) attn_q4_kernel(const float *__restrict__ q, long long q_stride, const uint8_t *__restrict__ kp, const uint8_t *__restrict__ vp,
-                                                             float *__restrict__ out, long long out_stride, KvQ4 c, int H, int window, float scale)
+template <int HD, int NB>
+struct AqShape {
+    static constexpr int G4 = HD / 32, KS = HD / 16, ROW = G4 * KQ4_BLOCK, ROWS = 8 * NB;
+    static constexpr int STAGE = 2 * AQ_CHUNK * ROW;                              // K rows, then V rows
+    static constexpr int STAGES = HD <= 64 ? 4 : (HD <= 128 ? 3 : 2);
+    static constexpr int OREG = NB * G4 * 8, DUMP = (OREG + 2 * NB) * 32 * 4;      // a warp's accumulators, maxima and sums, register by register
+    static constexpr int RING = AQ_WARPS * STAGES * STAGE, QF = NB * KS * 32 * 16, QS = NB * G4 * 8 * 4, EX = AQ_WARPS * NB * 8 * AQ_SP * 4;
+    static constexpr int SMEM = RING + QF + QS + EX + 2 * DUMP;
+    static constexpr int CTAS = SMEM <= 74 * 1024 && NB == 1 && HD <= 128 ? 3 : (SMEM <= 112 * 1024 ? 2 : 1);
+};
+
+struct AqParams {
+    const float *q;
+    const uint8_t *k, *v;
+    float *out;
+    long long q_stride, out_stride;
+    KvQ4 c;
+    int H, G, R, RC, window, *err;             // G heads a kv head, R = tokens * G query rows a kv head, RC blocks of them
+    float scale;
+    int4 *desc;                                // for each CTA: the stretch that begins in it and ends in a later one {last CTA, b, h, rc}, last CTA < 0: none
+    float *part;                               // [2 CTAs][8 NB][HD + 2]: the stretch that began before the CTA, the one that goes on after it
+};
+
+// where a CTA is on the line of units
+struct AqWalk {
+    int b, h, rc, u, n, begin, end, len;       // unit u of n; keys [begin, end), begin a multiple of 32
+};
+// tokens r0 / G .. of block rc: the keys that any of them sees
+__device__ __forceinline__ void aq_range(const AqParams &p, int nrows, AqWalk &w)
 {
-    __shared__ float acc_s[AQ_WARPS][32 * NB], m_s[AQ_WARPS], l_s[AQ_WARPS];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.x % H;
-    const long long row = blockIdx.x / H;
-    const int b = (int)(row / c.tokens), t = (int)(row - (long long)b * c.tokens), kvh = h / (H / c.Hkv);
-    const int pos = kv_len(c.lens[b], c.stride, c.page_tokens) - c.tokens + t, first = window > 0 ? max(0, pos - window + 1) : 0;
-    float qv[NB], acc[NB], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        qv[i] = q[row * q_stride + (long long)h * 32 * NB + 32 * i + lane] * scale;
-        acc[i] = 0.0f;
-    }
-    const int byte = 4 + (lane & 15), shift = lane < 16 ? 0 : 4;
-    for (int key = first + warp; key <= pos; key += AQ_WARPS) {
-        const int page = kv_page(c.table + (size_t)b * c.stride, c.stride, c.pages, c.page_tokens, key);
-        if (page < 0) continue;
-        const size_t at = kv_row(page, kvh, key % c.page_tokens, c.Hkv, c.page_tokens, NB);
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const uint8_t *p = kp + at + i * KQ4_BLOCK;
-            const uint32_t dm = *reinterpret_cast<const uint32_t *>(p);
-            s = fmaf(qv[i], fmaf(half_bits_to_float(dm & 0xffffu), (float)(p[byte] >> shift & 15), half_bits_to_float(dm >> 16)), s);
+    const int t0 = w.rc * nrows / p.G, t1 = (min(p.R, (w.rc + 1) * nrows) - 1) / p.G, at = w.len - p.c.tokens;
+    w.end = max(0, at + t1 + 1);
+    w.begin = p.window > 0 ? max(0, at + t0 - p.window + 1) & ~(AQ_CHUNK - 1) : 0;
+    w.n = w.end > w.begin ? (w.end - w.begin + AQ_UNIT - 1) / AQ_UNIT : 0;
+}
+__device__ __forceinline__ int aq_length(const AqParams &p, int b) { return kv_len(__ldg(p.c.lens + b), p.c.stride, p.c.page_tokens); }
+// the next stretch that has units; its first one.  False: there is none
+__device__ __forceinline__ bool aq_next_stretch(const AqParams &p, int nrows, AqWalk &w)
+{
+    w.u = 0;
+    for (;;) {
+        if (++w.rc == p.RC) {
+            w.rc = 0;
+            if (++w.h == p.c.Hkv) {
+                w.h = 0;
+                if (++w.b >= p.c.batch) return false;
+                w.len = aq_length(p, w.b);
+            }
         }
-        s = group_sum<32>(s);
-        const float m_new = fmaxf(m, s), m_ref = m_new == -INFINITY ? 0.0f : m_new;
-        const float alpha = m == -INFINITY ? 0.0f : expf(m - m_ref), p = expf(s - m_ref);
-        m = m_new;
-        l = l * alpha + p;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const uint8_t *pv = vp + at + i * KQ4_BLOCK;
-            const uint32_t dm = *reinterpret_cast<const uint32_t *>(pv);
-            acc[i] = fmaf(p, fmaf(half_bits_to_float(dm & 0xffffu), (float)(pv[byte] >> shift & 15), half_bits_to_float(dm >> 16)), acc[i] * alpha);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < NB; ++i) acc_s[warp][32 * i + lane] = acc[i];
-    if (lane == 0) { m_s[warp] = m; l_s[warp] = l; }
-    __syncthreads();
-    float mm = -INFINITY;
-    for (int w = 0; w < AQ_WARPS; ++w) mm = fmaxf(mm, m_s[w]);
-    const float m_ref = mm == -INFINITY ? 0.0f : mm;
-    for (int x = threadIdx.x; x < 32 * NB; x += AQ_THREADS) {
-        float a = 0.0f, ll = 0.0f;
-        for (int w = 0; w < AQ_WARPS; ++w) {
-            const float f = m_s[w] == -INFINITY ? (l_s[w] == 0.0f ? 0.0f : 1.0f) : expf(m_s[w] - m_ref);      // a sum without a maximum: NaN scores
-            a = fmaf(acc_s[w][x], f, a);
-            ll = fmaf(l_s[w], f, ll);
-        }
-        out[row * out_stride + (long long)h * 32 * NB + x] = ll == 0.0f ? 0.0f : a / ll;
+        aq_range(p, nrows, w);
+        if (w.n) return true;
     }
 }
+
+__device__ __forceinline__ void aq_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void aq_mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void aq_split(float a, float b, uint32_t &hi, uint32_t &lo)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+__device__ __forceinline__ float aq_exp2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));       // two units in the last place
+    return y;
+}
+__device__ __forceinline__ uint32_t aq_lds32(uint32_t a)
+{
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t aq_lds16(uint32_t a)
+{
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+    return v;
+}
+// nibble P of each half of the word, as 16 c * 2^-24
+template <int P>
+__device__ __forceinline__ uint32_t aq_codes(uint32_t w) { return (P == 0 ? w << 4 : w >> (P ? 4 * (P - 1) : 0)) & 0x00f000f0u; }
+constexpr float AQ_UNSCALE = 1048576.0f;       // 2^20
+__device__ __forceinline__ float aq_lo(uint32_t dm) { return __low2float(*reinterpret_cast<const __half2 *>(&dm)); }
+__device__ __forceinline__ float aq_hi(uint32_t dm) { return __high2float(*reinterpret_cast<const __half2 *>(&dm)); }
+__device__ __forceinline__ bool aq_no_number(uint32_t dm) { return (dm & 0x7c00u) == 0x7c00u || (dm & 0x7c000000u) == 0x7c000000u; }
+
+template <int HD, int NB>
+__global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_kernel(const AqParams p)
+{
+    using S = AqShape<HD, NB>;
+    constexpr int G4 = S::G4, KS = S::KS, ROW = S::ROW, ROWS = S::ROWS, STAGES = S::STAGES;
+    extern __shared__ __align__(128) uint8_t aq_smem[];
+    __shared__ __align__(8) uint64_t full[AQ_WARPS][STAGES];
+    __shared__ int pieces[AQ_WARPS][STAGES];
+    __shared__ long long s_sum[AQ_WARPS], s_rest;
+    __shared__ int s_b;
+    uint4 *qf = reinterpret_cast<uint4 *>(aq_smem + S::RING);                     // [NB][KS][lane] {hi b0, hi b1, lo b0, lo b1}
+    float *qs = reinterpret_cast<float *>(aq_smem + S::RING + S::QF);             // [NB][G4][8] sums of the scaled query over a block
+    __shared__ float q_factor[ROWS];
+    float *dump = reinterpret_cast<float *>(aq_smem + S::RING + S::QF + S::QS + S::EX);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    float *ex = reinterpret_cast<float *>(aq_smem + S::RING + S::QF + S::QS) + warp * NB * 8 * AQ_SP;
+    const int N = gridDim.x, me = blockIdx.x;
+
+    if (lane == 0) {
+        for (int i = 0; i < STAGES; ++i) mbar_init(smem_u32(&full[warp][i]), 1);
+        mbar_fence_init();
+    }
+    pdl_trigger();
+
+    // ---- this CTA's part of the line: units of all sequences are counted, each thread some consecutive ones
+    const int each = (p.c.batch + AQ_THREADS - 1) / AQ_THREADS, b0 = min(p.c.batch, tid * each), b1 = min(p.c.batch, b0 + each);
+    auto units_of = [&](int b) {
+        AqWalk w;
+        w.b = b;
+        w.len = aq_length(p, b);
+        long long n = 0;
+        for (w.rc = 0; w.rc < p.RC; ++w.rc) {
+            aq_range(p, ROWS, w);
+            n += w.n;
+        }
+        return n * p.c.Hkv;
+    };
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += units_of(b);
+    long long before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += y;
+    }
+    if (lane == 31) s_sum[warp] = before;
+    before -= mine;
+    __syncthreads();
+    long long total = 0;
+    for (int w = 0; w < AQ_WARPS; ++w) {
+        if (w < warp) before += s_sum[w];
+        total += s_sum[w];
+    }
+    const int parts = (int)min((long long)N, total);                              // every CTA below has at least one unit
+    const long long first = me < parts ? total * me / parts : 0, last = me < parts ? total * (me + 1) / parts : 0;         // its units [first, last)
+    if (first < last && mine && before <= first && first < before + mine) {
+        long long rest = first - before;
+        int b = b0;
+        for (;; ++b) {
+            const long long n = units_of(b);
+            if (rest < n) break;
+            rest -= n;
+        }
+        s_b = b;
+        s_rest = rest;
+    }
+    __syncthreads();
+    if (tid == 0 && p.desc) p.desc[me] = make_int4(-1, 0, 0, 0);
+
+    bool ok = true;
+    if (first < last) {
+        AqWalk w;                                              // the unit being computed
+        w.b = s_b;
+        w.len = aq_length(p, w.b);
+        {
+            long long rest = s_rest, per_head = 0;
+            for (w.rc = 0; w.rc < p.RC; ++w.rc) {
+                aq_range(p, ROWS, w);
+                per_head += w.n;
+            }
+            w.h = (int)(rest / per_head);
+            rest -= per_head * w.h;
+            for (w.rc = 0;; ++w.rc) {
+                aq_range(p, ROWS, w);
+                if (rest < w.n) break;
+                rest -= w.n;
+            }
+            w.u = (int)rest;
+        }
+        AqWalk f = w;                                          // the unit being fetched, up to STAGES - 1 further on
+        long long f_at = first;
+        int entry = -1;                                        // lanes 0 and 1: the table entry of their piece of the next unit to fetch
+        auto look = [&]() {
+            const int pos = f.begin + f.u * AQ_UNIT + warp * AQ_CHUNK + 16 * lane;
+            entry = f_at < last && lane < 2 && pos < f.end ? kv_entry(__ldg(p.c.table + (size_t)f.b * p.c.stride + pos / p.c.page_tokens), p.c.pages) : -1;
+        };
+        const uint32_t ring = smem_u32(aq_smem) + warp * STAGES * S::STAGE;
+        auto fetch = [&](int i) {                              // the i-th unit of this CTA into stage i % STAGES
+            if (f_at >= last) return;
+            __syncwarp();
+            const int stage = i % STAGES;
+            const uint32_t bar = smem_u32(&full[warp][stage]), to = ring + stage * S::STAGE + lane * 16 * ROW;
+            const uint32_t there = __ballot_sync(0xffffffffu, entry >= 0) & 3u;
+            if (lane == 0) {
+                pieces[warp][stage] = there;
+                mbar_arrive_expect_tx(bar, __popc(there) * 2 * 16 * ROW);
+            }
+            __syncwarp();
+            if (entry >= 0) {
+                const int pos = f.begin + f.u * AQ_UNIT + warp * AQ_CHUNK + 16 * lane;
+                const size_t at = kv_row(entry, f.h, pos % p.c.page_tokens, p.c.Hkv, p.c.page_tokens, G4);
+                bulk_g2s(to, p.k + at, 16 * ROW, bar);
+                bulk_g2s(to + AQ_CHUNK * ROW, p.v + at, 16 * ROW, bar);
+            }
+            ++f_at;
+            if (++f.u >= f.n && f_at < last) aq_next_stretch(p, ROWS, f);
+            look();
+        };
+        look();
+        for (int i = 0; i < STAGES - 1; ++i) fetch(i);
+
+        int i = 0;
+        for (long long at = first; at < last;) {
+            // ---- a stretch: query fragments of its rows
+            const int r0 = w.rc * ROWS, u_first = w.u;
+            __syncthreads();                                   // the stretch before is done with them
+            for (int r = warp; r < ROWS; r += AQ_WARPS) {      // a warp per row, a lane the channels 4 (lane % 4 ..) of its blocks
+                float x[G4], top = 0.0f;
+                const int row = r0 + r, tok = row / p.G;
+                const float *src = p.q + ((long long)w.b * p.c.tokens + tok) * p.q_stride + (long long)(w.h * p.G + row - tok * p.G) * HD;
+#pragma unroll
+                for (int j = 0; j < G4; ++j) {
+                    x[j] = row < p.R ? __ldg(src + 32 * j + lane) : 0.0f;
+                    top = fmaxf(top, fabsf(x[j]));
+                }
+                const int ex_top = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23);      // biased exponent of the row's largest
+                const int sh = max(-126, min(126, 141 - ex_top));                                           // largest into [2^14, 2^15)
+                const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
+                if (lane == 0) q_factor[r] = __uint_as_float((uint32_t)(127 - sh) << 23) * p.scale * (1.44269504088896340736f * AQ_UNSCALE);
+#pragma unroll
+                for (int j = 0; j < G4; ++j) {
+                    const float y = x[j] * up;
+                    const float sum = group_sum<32>(y);
+                    if (lane == 0) qs[((r >> 3) * G4 + j) * 8 + (r & 7)] = sum * (1.0f / AQ_UNSCALE);
+                    // channel c of the block: k-step c / 16, thread t = (c % 16) / 4, place c % 4: b0 holds places 0 and 2, b1 places 1 and 3
+                    const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
+                    const int place = lane & 3, to = ((((r >> 3) * KS + 2 * j + (lane >> 4)) * 32 + 4 * (r & 7) + ((lane & 15) >> 2)) * 8) + (place & 1) * 2 + (place >> 1);
+                    reinterpret_cast<__half *>(qf)[to] = hi;
+                    reinterpret_cast<__half *>(qf)[to + 4] = lo;
+                }
+            }
+            __syncthreads();
+            uint4 qr[NB == 1 ? KS : 1];
+            float2 qsr[NB == 1 ? G4 : 1];
+            if constexpr (NB == 1) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) qr[ks] = qf[ks * 32 + lane];
+#pragma unroll
+                for (int j = 0; j < G4; ++j) qsr[j] = make_float2(qs[j * 8 + 2 * t], qs[j * 8 + 2 * t + 1]);
+            }
+            float o[NB][G4][2][4], om[NB][G4], m_run[NB], l_run[NB], fac[NB];
+            int pos_row[NB], e_run = 60;                       // pos_row: the position of row g of each block, -1 where there is none
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const int row = r0 + 8 * nb + g;
+                pos_row[nb] = row < p.R ? w.len - p.c.tokens + row / p.G : -1;
+                fac[nb] = q_factor[8 * nb + g];
+                m_run[nb] = -INFINITY;
+                l_run[nb] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < G4; ++j) {
+                    om[nb][j] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] = 0.0f;
+                }
+            }
+            // chunks in [all_from, all_to) are seen by every row
+            const int pos_first = w.len - p.c.tokens + r0 / p.G, pos_last = w.len - p.c.tokens + (min(p.R, r0 + ROWS) - 1) / p.G;
+            const int all_to = pos_first + 1, all_from = p.window > 0 ? pos_last - p.window + 1 : 0;
+
+            for (;;) {
+                fetch(i + STAGES - 1);
+                const int stage = i % STAGES;
+                if (ok && !mbar_wait_spin(smem_u32(&full[warp][stage]), (uint32_t)(i / STAGES) & 1u)) {
+                    ok = false;
+                    if (lane == 0) atomicExch(p.err, DEV_ERR_FULL_WAIT);
+                }
+                const uint32_t there = pieces[warp][stage];
+                const int key0 = w.begin + w.u * AQ_UNIT + warp * AQ_CHUNK;
+                if (there) {
+                    const uint32_t kb = ring + stage * S::STAGE, vb = kb + AQ_CHUNK * ROW;
+                    const bool mixed = there != 3u || key0 < all_from || key0 + AQ_CHUNK > all_to;
+                    if (mixed) {
+                        // What no row sees must not reach the products even with weight zero (0 x NaN), what some rows see only those: scales that are no
+                        // numbers are taken out, and the rows that see them marked.
+                        const int key = key0 + lane;
+                        const bool in = (there >> (lane >> 4) & 1u) && key < w.end;
+                        const uint32_t row = vb + lane * ROW;
+#pragma unroll 1
+                        for (int j = 0; j < G4; ++j) {
+                            const uint32_t dm = aq_lds32(row + j * KQ4_BLOCK);
+                            const bool nan = in && aq_no_number(dm);
+                            if (!in || nan) asm volatile("st.shared.u32 [%0], %1;" ::"r"(row + j * KQ4_BLOCK), "r"(0u) : "memory");
+                            for (uint32_t bad = __ballot_sync(0xffffffffu, nan); bad; bad &= bad - 1) {
+                                const int at_key = key0 + __ffs(bad) - 1;
+#pragma unroll
+                                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) {
+                                        const int pos = __shfl_sync(0xffffffffu, pos_row[nb], 4 * (2 * t + e));
+                                        if (at_key <= pos && (p.window == 0 || at_key > pos - p.window))
+#pragma unroll
+                                            for (int jj = 0; jj < G4; ++jj)
+                                                if (jj == j)
+#pragma unroll
+                                                    for (int x = 0; x < 2; ++x) o[nb][jj][x][e] = o[nb][jj][x][e + 2] = __int_as_float(0x7fffffff);
+                                    }
+                            }
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the next copy into this stage comes after these stores
+                        __syncwarp();
+                    }
+                    // ---- scores of 2 x 16 keys
+                    float s[NB][2][4];
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) s[nb][e >> 2][e & 3] = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < G4; ++j) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t at0 = kb + (16 * x + g) * ROW + j * KQ4_BLOCK, at1 = at0 + 8 * ROW;
+                            const uint32_t c0 = aq_lds32(at0 + 4 + 4 * t), c1 = aq_lds32(at1 + 4 + 4 * t), dm0 = aq_lds32(at0), dm1 = aq_lds32(at1);
+                            const uint32_t a0[4] = {aq_codes<0>(c0), aq_codes<0>(c1), aq_codes<2>(c0), aq_codes<2>(c1)};
+                            const uint32_t a1[4] = {aq_codes<1>(c0), aq_codes<1>(c1), aq_codes<3>(c0), aq_codes<3>(c1)};
+                            const float d0 = aq_lo(dm0), m0 = aq_hi(dm0), d1 = aq_lo(dm1), m1 = aq_hi(dm1);
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) {
+                                const uint4 b0 = NB == 1 ? qr[NB == 1 ? 2 * j : 0] : qf[(nb * KS + 2 * j) * 32 + lane];
+                                const uint4 b1 = NB == 1 ? qr[NB == 1 ? 2 * j + 1 : 0] : qf[(nb * KS + 2 * j + 1) * 32 + lane];
+                                const float2 qq = NB == 1 ? qsr[NB == 1 ? j : 0] : *reinterpret_cast<const float2 *>(qs + (nb * G4 + j) * 8 + 2 * t);
+                                float acc[4];
+                                aq_mma_first(acc, a0, b0.x, b0.y);
+                                aq_mma(acc, a0, b0.z, b0.w);
+                                aq_mma(acc, a1, b1.x, b1.y);
+                                aq_mma(acc, a1, b1.z, b1.w);
+                                s[nb][x][0] = fmaf(d0, acc[0], fmaf(m0, qq.x, s[nb][x][0]));
+                                s[nb][x][1] = fmaf(d0, acc[1], fmaf(m0, qq.y, s[nb][x][1]));
+                                s[nb][x][2] = fmaf(d1, acc[2], fmaf(m1, qq.x, s[nb][x][2]));
+                                s[nb][x][3] = fmaf(d1, acc[3], fmaf(m1, qq.y, s[nb][x][3]));
+                            }
+                        }
+                    }
+                    // the largest step of the values: what the weights are scaled by
+                    uint32_t dtop = 0;
+#pragma unroll
+                    for (int j = 0; j < G4; ++j) dtop = max(dtop, aq_lds16(vb + lane * ROW + j * KQ4_BLOCK) & 0x7fffu);
+                    dtop = __reduce_max_sync(0xffffffffu, dtop) >> 10;
+                    const int e_new = min(e_run, 29 - (int)min(30u, max(1u, dtop)));
+
+                    // ---- from (keys g, rows 2t) to (row g, keys 2t): weights
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) ex[(nb * 8 + 2 * t + (e & 1)) * AQ_SP + 16 * x + 8 * (e >> 1) + g] = s[nb][x][e];
+                    __syncwarp();
+                    float pr[NB][8];                           // keys 16 x + 8 y + 2t + z at [4 x + 2 y + z]
+                    float alpha[NB];
+                    bool moved = e_new != e_run;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            const float2 v = *reinterpret_cast<const float2 *>(ex + (nb * 8 + g) * AQ_SP + 8 * y + 2 * t);
+                            pr[nb][2 * y] = v.x * fac[nb];
+                            pr[nb][2 * y + 1] = v.y * fac[nb];
+                            if (mixed) {
+#pragma unroll
+                                for (int z = 0; z < 2; ++z) {
+                                    const int key = key0 + 8 * y + 2 * t + z;
+                                    const bool seen = key <= pos_row[nb] && (p.window == 0 || key > pos_row[nb] - p.window) && (there >> (y >> 1) & 1u);
+                                    if (!seen) pr[nb][2 * y + z] = -INFINITY;
+                                }
+                            }
+                            top = fmaxf(top, fmaxf(pr[nb][2 * y], pr[nb][2 * y + 1]));
+                        }
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                        const float m_new = fmaxf(m_run[nb], top);
+                        moved |= m_new != m_run[nb];
+                        const float ref = (m_new == -INFINITY ? 0.0f : m_new) - (float)e_new;
+                        alpha[nb] = m_run[nb] == -INFINITY ? 0.0f : aq_exp2(m_run[nb] - (float)e_run - ref);
+                        m_run[nb] = m_new;
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) {
+                            pr[nb][y] = aq_exp2(pr[nb][y] - ref);
+                            sum += pr[nb][y];
+                        }
+                        l_run[nb] = fmaf(l_run[nb], alpha[nb], sum);
+                    }
+                    e_run = e_new;
+                    if (__any_sync(0xffffffffu, moved)) {      // rare once the first keys have been seen
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            const float f0 = __shfl_sync(0xffffffffu, alpha[nb], 8 * t), f1 = __shfl_sync(0xffffffffu, alpha[nb], 8 * t + 4);
+#pragma unroll
+                            for (int j = 0; j < G4; ++j) {
+                                om[nb][j] *= alpha[nb];
+#pragma unroll
+                                for (int x = 0; x < 2; ++x) {
+                                    o[nb][j][x][0] *= f0;
+                                    o[nb][j][x][1] *= f1;
+                                    o[nb][j][x][2] *= f0;
+                                    o[nb][j][x][3] *= f1;
+                                }
+                            }
+                        }
+                    }
+                    // ---- values.  The tensor cores cut what they add to an accumulator instead of rounding it, and all terms here have one sign: sums
+                    // over the chunk start from zero and are added up in fp32 by the rounding adder (300 keys: an error of 2e-5 without, 2e-6 so).
+#pragma unroll
+                    for (int j = 0; j < G4; ++j) {
+                        float acc[NB][2][4];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t at = vb + (16 * x + 2 * t) * ROW + j * KQ4_BLOCK;
+                            const uint32_t dm0 = aq_lds32(at), dm1 = aq_lds32(at + ROW), dm2 = aq_lds32(at + 8 * ROW), dm3 = aq_lds32(at + 9 * ROW);
+                            const uint32_t w0 = __byte_perm(aq_lds16(at + 4 + 2 * g), aq_lds16(at + ROW + 4 + 2 * g), 0x5410);
+                            const uint32_t w1 = __byte_perm(aq_lds16(at + 8 * ROW + 4 + 2 * g), aq_lds16(at + 9 * ROW + 4 + 2 * g), 0x5410);
+                            const uint32_t a0[4] = {aq_codes<0>(w0), aq_codes<1>(w0), aq_codes<0>(w1), aq_codes<1>(w1)};
+                            const uint32_t a1[4] = {aq_codes<2>(w0), aq_codes<3>(w0), aq_codes<2>(w1), aq_codes<3>(w1)};
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) {
+                                const float *q4 = pr[nb] + 4 * x;
+                                om[nb][j] = fmaf(q4[0], aq_hi(dm0), fmaf(q4[1], aq_hi(dm1), fmaf(q4[2], aq_hi(dm2), fmaf(q4[3], aq_hi(dm3), om[nb][j]))));
+                                uint32_t h0, l0, h1, l1;
+                                aq_split(q4[0] * aq_lo(dm0), q4[1] * aq_lo(dm1), h0, l0);
+                                aq_split(q4[2] * aq_lo(dm2), q4[3] * aq_lo(dm3), h1, l1);
+                                if (x == 0) {
+                                    aq_mma_first(acc[nb][0], a0, l0, l1);
+                                    aq_mma_first(acc[nb][1], a1, l0, l1);
+                                } else {
+                                    aq_mma(acc[nb][0], a0, l0, l1);
+                                    aq_mma(acc[nb][1], a1, l0, l1);
+                                }
+                                aq_mma(acc[nb][0], a0, h0, h1);
+                                aq_mma(acc[nb][1], a1, h0, h1);
+                            }
+                        }
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] += acc[nb][e >> 2][e & 3];
+                    }
+                    __syncwarp();                              // the stage and the exchange are free again
+                }
+                ++i;
+                ++at;
+                if (++w.u >= w.n || at >= last) break;
+            }
+
+            // ---- the stretch ends here: the four warps' results, relative to 2^ref, become one
+            float ref[NB];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                ref[nb] = m_run[nb] == -INFINITY ? -INFINITY : m_run[nb] - (float)e_run;
+                l_run[nb] += __shfl_xor_sync(0xffffffffu, l_run[nb], 1);
+                l_run[nb] += __shfl_xor_sync(0xffffffffu, l_run[nb], 2);
+#pragma unroll
+                for (int j = 0; j < G4; ++j) {
+                    float a = om[nb][j];
+                    a += __shfl_xor_sync(0xffffffffu, a, 1);
+                    a += __shfl_xor_sync(0xffffffffu, a, 2);
+                    const float a0 = __shfl_sync(0xffffffffu, a, 8 * t), a1 = __shfl_sync(0xffffffffu, a, 8 * t + 4);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        o[nb][j][x][0] = fmaf(o[nb][j][x][0], AQ_UNSCALE, a0);
+                        o[nb][j][x][1] = fmaf(o[nb][j][x][1], AQ_UNSCALE, a1);
+                        o[nb][j][x][2] = fmaf(o[nb][j][x][2], AQ_UNSCALE, a0);
+                        o[nb][j][x][3] = fmaf(o[nb][j][x][3], AQ_UNSCALE, a1);
+                    }
+                }
+            }
+            auto put = [&](float *to) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int e = 0; e < G4 * 8; ++e) to[(nb * G4 * 8 + e) * 32 + lane] = o[nb][e >> 3][e >> 2 & 1][e & 3];
+                    to[(S::OREG + 2 * nb) * 32 + lane] = ref[nb];
+                    to[(S::OREG + 2 * nb + 1) * 32 + lane] = l_run[nb];
+                }
+            };
+            auto join = [&](const float *from) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const float ref2 = from[(S::OREG + 2 * nb) * 32 + lane], l2 = from[(S::OREG + 2 * nb + 1) * 32 + lane], both = fmaxf(ref[nb], ref2);
+                    const float f = ref[nb] == -INFINITY ? 0.0f : aq_exp2(ref[nb] - both), f2 = ref2 == -INFINITY ? 0.0f : aq_exp2(ref2 - both);
+                    l_run[nb] = l_run[nb] * f + l2 * f2;
+                    ref[nb] = both;
+                    const float fa = __shfl_sync(0xffffffffu, f, 8 * t), fb = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+                    const float f2a = __shfl_sync(0xffffffffu, f2, 8 * t), f2b = __shfl_sync(0xffffffffu, f2, 8 * t + 4);
+#pragma unroll
+                    for (int e = 0; e < G4 * 8; ++e) {
+                        float &x = o[nb][e >> 3][e >> 2 & 1][e & 3];
+                        x = x * (e & 1 ? fb : fa) + from[(nb * G4 * 8 + e) * 32 + lane] * (e & 1 ? f2b : f2a);
+                    }
+                }
+            };
+            float *half = dump + (warp & 1) * (S::DUMP / 4);
+            if (warp >= 2) put(half);
+            __syncthreads();
+            if (warp < 2) join(half);
+            __syncthreads();
+            if (warp == 1) put(dump);
+            __syncthreads();
+            if (warp == 0) {
+                join(dump);
+                const bool whole = u_first == 0 && w.u >= w.n;
+                float *part = whole ? nullptr : p.part + (size_t)(2 * me + (u_first == 0)) * ROWS * (HD + 2);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    if (part && t == 0) {
+                        part[(8 * nb + g) * (HD + 2) + HD] = ref[nb];
+                        part[(8 * nb + g) * (HD + 2) + HD + 1] = l_run[nb];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int r = 8 * nb + 2 * t + e, row = r0 + r, tok = row / p.G;
+                        const float l = __shfl_sync(0xffffffffu, l_run[nb], 8 * t + 4 * e);
+                        if (row >= p.R) continue;
+                        float *to = part ? part + r * (HD + 2) : p.out + ((long long)w.b * p.c.tokens + tok) * p.out_stride + (long long)(w.h * p.G + row - tok * p.G) * HD;
+#pragma unroll
+                        for (int j = 0; j < G4; ++j)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                                for (int y = 0; y < 2; ++y) {
+                                    const float v = o[nb][j][x][2 * y + e];
+                                    to[32 * j + 2 * g + x + 16 * y] = part ? v : (l == 0.0f ? 0.0f : v / l);
+                                }
+                    }
+                }
+                if (!whole && u_first == 0 && lane == 0)        // its last unit is n - u units behind the end of this CTA's part
+                    p.desc[me] = make_int4((int)(((last + w.n - w.u) * parts - 1) / total), w.b, w.h, w.rc);
+            }
+            if (at < last) aq_next_stretch(p, ROWS, w);
+        }
+        if (!ok)                                               // a wait ran out: the copies still on their way end before the CTA does
+            for (int s = max(0, i - STAGES); s < i; ++s) mbar_wait_spin(smem_u32(&full[warp][s % STAGES]), (uint32_t)(s / STAGES) & 1u);
+    }
+    // blocks of query rows that see no key
+    for (int x = me; x < p.c.batch * p.RC; x += N) {
+        AqWalk w;
+        w.b = x / p.RC;
+        w.rc = x - w.b * p.RC;
+        w.len = aq_length(p, w.b);
+        aq_range(p, ROWS, w);
+        if (w.n) continue;
+        const int r0 = w.rc * ROWS, rows = min(p.R, r0 + ROWS) - r0;
+        for (int y = tid; y < rows * p.c.Hkv * HD; y += AQ_THREADS) {
+            const int c = y % HD, hr = y / HD, h = hr / rows, row = r0 + hr - h * rows, tok = row / p.G;
+            p.out[((long long)w.b * p.c.tokens + tok) * p.out_stride + (long long)(h * p.G + row - tok * p.G) * HD + c] = 0.0f;
+        }
+    }
+}
+
+// One CTA per (stretch that spans CTAs, query row): its warps take every eighth partial result.
+template <int HD>
+__global__ void __launch_bounds__(32 * AQ_MERGE_WARPS) attn_q4_merge_kernel(const AqParams p, int nrows)
+{
+    constexpr int PER = HD / 32;
+    __shared__ float acc_s[AQ_MERGE_WARPS][HD], ref_s[AQ_MERGE_WARPS], l_s[AQ_MERGE_WARPS];
+    pdl_wait();
+    const int a = blockIdx.x, r = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int4 d = __ldcg(p.desc + a);
+    const int row = d.w * nrows + r;
+    if (d.x < 0 || row >= p.R) return;
+    const int count = d.x - a + 1;
+    auto slot = [&](int i) { return p.part + ((size_t)(2 * (a + i) + (i == 0)) * nrows + r) * (HD + 2); };
+    float ref = -INFINITY, l = 0.0f, acc[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) acc[j] = 0.0f;
+    for (int i = warp; i < count; i += AQ_MERGE_WARPS) {
+        const float *s = slot(i);
+        const float ref2 = __ldcg(s + HD), l2 = __ldcg(s + HD + 1), both = fmaxf(ref, ref2);
+        const float f = ref == -INFINITY ? 0.0f : aq_exp2(ref - both), f2 = ref2 == -INFINITY ? 0.0f : aq_exp2(ref2 - both);
+        ref = both;
+        l = l * f + l2 * f2;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) acc[j] = acc[j] * f + __ldcg(s + 32 * j + lane) * f2;
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) acc_s[warp][32 * j + lane] = acc[j];
+    if (lane == 0) { ref_s[warp] = ref; l_s[warp] = l; }
+    __syncthreads();
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < AQ_MERGE_WARPS; ++w) top = fmaxf(top, ref_s[w]);
+    const int tok = row / p.G;
+    float *to = p.out + ((long long)d.y * p.c.tokens + tok) * p.out_stride + (long long)(d.z * p.G + row - tok * p.G) * HD;
+    for (int c = threadIdx.x; c < HD; c += 32 * AQ_MERGE_WARPS) {
+        float sum = 0.0f, v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < AQ_MERGE_WARPS; ++w) {
+            const float f = ref_s[w] == -INFINITY ? 0.0f : aq_exp2(ref_s[w] - top);
+            sum += l_s[w] * f;
+            v += acc_s[w][c] * f;
+        }
+        to[c] = sum == 0.0f ? 0.0f : v / sum;
+    }
+}
+
+template <int HD, int NB>
+static int aq_launch(AqParams p, void *ws, bool joins, cudaStream_t st)
+{
+    using S = AqShape<HD, NB>;
+    static_assert(S::SMEM <= 227 * 1024, "shared memory");
+    const int N = ckb_sm_count() * S::CTAS;
+    p.RC = (p.R + S::ROWS - 1) / S::ROWS;
+    p.desc = (int4 *)ws;
+    p.part = (float *)((uint8_t *)ws + sizeof(int4) * N);
+    if (ckb_check_cuda((int)cudaFuncSetAttribute(attn_q4_kernel<HD, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "attention_q4cache")) return CKB_ERR_CUDA;
+    attn_q4_kernel<HD, NB><<<N, AQ_THREADS, S::SMEM, st>>>(p);
+    const int rc = ckb_check_launch("attention_q4cache");
+    if (rc || !joins) return rc;
+    return launch_pdl("attention_q4cache", attn_q4_merge_kernel<HD>, dim3(N, S::ROWS < p.R ? S::ROWS : p.R), dim3(32 * AQ_MERGE_WARPS), 0, st, p, S::ROWS);
+}
+
+template <int HD, int NB>
+static size_t aq_bytes()
+{
+    using S = AqShape<HD, NB>;
+    const size_t N = (size_t)ckb_sm_count() * S::CTAS;
+    return N * (sizeof(int4) + 2 * sizeof(float) * S::ROWS * (HD + 2));
+}
+
+// Blocks of 8 query rows that share the codes a CTA unpacks.
+static int aq_blocks(long long rows, int hd) { return rows <= 8 ? 1 : (rows <= 16 || hd > 128 ? 2 : 4); }
 
 }  // namespace ckb
 
 using namespace ckb;
 
+#define AQ_EACH(hd, nb, F)                                                          \
+    (hd == 64 ? (nb == 1 ? F<64, 1> : nb == 2 ? F<64, 2> : F<64, 4>)                \
+     : hd == 96 ? (nb == 1 ? F<96, 1> : nb == 2 ? F<96, 2> : F<96, 4>)              \
+     : hd == 128 ? (nb == 1 ? F<128, 1> : nb == 2 ? F<128, 2> : F<128, 4>)          \
+     : hd == 192 ? (nb == 1 ? F<192, 1> : F<192, 2>)                                \
+                 : (nb == 1 ? F<256, 1> : F<256, 2>))
+
 extern "C" size_t ckb200_attention_q4cache_workspace_bytes(int batch, int num_tokens, int num_heads, int num_kv_heads, int head_dim)
 {
-    (void)batch; (void)num_tokens; (void)num_heads; (void)num_kv_heads; (void)head_dim;
-    return 0;
+    if (batch <= 0 || num_tokens <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads || !ckb200_kv_q4_page_bytes(1, 16, head_dim)) return 0;
+    const int nb = aq_blocks((long long)num_tokens * (num_heads / num_kv_heads), head_dim);
+    return AQ_EACH(head_dim, nb, aq_bytes)();
 }
 
 extern "C" int ckb200_dev_attention_q4cache(const float *q, long long q_stride, const void *k_pages, const void *v_pages, float *out, long long out_stride, const int *page_table,
@@ -96,25 +712,28 @@ extern "C" int ckb200_dev_attention_q4cache(const float *q, long long q_stride, 
     if (rows > 1 && (q_stride < (long long)num_heads * head_dim || out_stride < (long long)num_heads * head_dim))
         return ckb_fail(CKB_ERR_SHAPE, "%s: rows of %lld values lie %lld and %lld apart", what, (long long)num_heads * head_dim, q_stride, out_stride);
     if (((uintptr_t)q | (uintptr_t)out) & 3) return ckb_fail(CKB_ERR_ALIGN, "%s: rows must be aligned to 4 bytes", what);
-    if (workspace_bytes < ckb200_attention_q4cache_workspace_bytes(batch, num_tokens, num_heads, num_kv_heads, head_dim))
-        return ckb_fail(CKB_ERR_STATE, "%s: the workspace is too small", what);
-    if (rows * num_heads > 0x7fffffffLL) return ckb_fail(CKB_ERR_LIMIT, "%s: %lld query rows in one call", what, rows * num_heads);
+    if (rows * num_heads > 1 << 30 || num_heads > 1 << 20) return ckb_fail(CKB_ERR_LIMIT, "%s: %lld query rows in one call", what, rows * num_heads);
     if (!rows) return 0;
     if (ckb_ensure_init()) return CKB_ERR_NO_DEVICE;
     if ((rc = ckb_check_device(what))) return rc;
-    (void)workspace;
-    const KvQ4 c = {page_table, kv_lens, table_stride, batch, num_tokens, num_pages, page_tokens, num_kv_heads, head_dim / 32};
-    const float scale = 1.0f / sqrtf((float)head_dim);
-    const unsigned grid = (unsigned)(rows * num_heads);
-    cudaStream_t st = ckb_stream(stream);
-#define AQ_RUN(NB) attn_q4_kernel<NB><<<grid, AQ_THREADS, 0, st>>>(q, q_stride, (const uint8_t *)k_pages, (const uint8_t *)v_pages, out, out_stride, c, num_heads, sliding_window, scale)
-    switch (head_dim) {
-    case 64: AQ_RUN(2); break;
-    case 96: AQ_RUN(3); break;
-    case 128: AQ_RUN(4); break;
-    case 192: AQ_RUN(6); break;
-    default: AQ_RUN(8); break;
-    }
-#undef AQ_RUN
-    return ckb_check_launch(what);
+    if (!workspace || workspace_bytes < ckb200_attention_q4cache_workspace_bytes(batch, num_tokens, num_heads, num_kv_heads, head_dim))
+        return ckb_fail(CKB_ERR_STATE, "%s: the workspace is too small", what);
+    if ((uintptr_t)workspace & 15) return ckb_fail(CKB_ERR_ALIGN, "%s: the workspace must be aligned to 16 bytes", what);
+    AqParams p = {};
+    p.q = q;
+    p.k = (const uint8_t *)k_pages;
+    p.v = (const uint8_t *)v_pages;
+    p.out = out;
+    p.q_stride = q_stride;
+    p.out_stride = out_stride;
+    p.c = {page_table, kv_lens, table_stride, batch, num_tokens, num_pages, page_tokens, num_kv_heads, head_dim / 32};
+    p.H = num_heads;
+    p.G = num_heads / num_kv_heads;
+    p.R = num_tokens * p.G;
+    p.window = sliding_window;
+    p.scale = 1.0f / sqrtf((float)head_dim);
+    p.err = ckb_device_error_word();
+    const bool joins = (long long)table_stride * page_tokens > AQ_UNIT;           // else no stretch has two units
+    const int nb = aq_blocks(p.R, head_dim);
+    return AQ_EACH(head_dim, nb, aq_launch)(p, workspace, joins, ckb_stream(stream));
 }
