@@ -42,11 +42,12 @@ template <int HD, int NB>
 struct AqShape {
     static constexpr int G4 = HD / 32, KS = HD / 16, ROW = G4 * KQ4_BLOCK, ROWS = 8 * NB;
     static constexpr int STAGE = 2 * AQ_CHUNK * ROW;                              // K rows, then V rows
-    static constexpr int STAGES = HD <= 64 ? 4 : (HD <= 128 ? 3 : 2);
+    static constexpr int CTAS = NB > 1 && HD > 192 ? 1 : (NB > 1 || HD > 128 ? 2 : 4);                       // resident on an SM, for which registers and shared memory are kept
+    static constexpr int STAGES = HD <= 64 ? 4 : 2;
     static constexpr int OREG = NB * G4 * 8, DUMP = (OREG + 2 * NB) * 32 * 4;      // a warp's accumulators, maxima and sums, register by register
-    static constexpr int RING = AQ_WARPS * STAGES * STAGE, QF = NB * KS * 32 * 16, QS = NB * G4 * 8 * 4, EX = AQ_WARPS * NB * 8 * AQ_SP * 4;
-    static constexpr int SMEM = RING + QF + QS + EX + 2 * DUMP;
-    static constexpr int CTAS = SMEM <= 74 * 1024 && NB == 1 && HD <= 128 ? 3 : (SMEM <= 112 * 1024 ? 2 : 1);
+    static constexpr int RING = AQ_WARPS * STAGES * STAGE, QF = NB * KS * 32 * 16, QS = NB * 32 * 8, EX = AQ_WARPS * NB * 8 * AQ_SP * 4, TAB = AQ_WARPS * 3 * G4 * 64;
+    static constexpr int SMEM = RING + (QF + QS + EX + TAB > 2 * DUMP ? QF + QS + EX + TAB : 2 * DUMP);      // the exchange between warps lies over the queries
+    static_assert(CTAS * (SMEM + 2048) <= 227 * 1024, "shared memory");
 };
 
 struct AqParams {
@@ -57,6 +58,7 @@ struct AqParams {
     KvQ4 c;
     int H, G, R, RC, window, *err;             // G heads a kv head, R = tokens * G query rows a kv head, RC blocks of them
     float scale;
+    uint32_t page_mul, page_shift;             // position / page_tokens = (position * page_mul >> 32) >> page_shift
     int4 *desc;                                // for each CTA: the stretch that begins in it and ends in a later one {last CTA, b, h, rc}, last CTA < 0: none
     float *part;                               // [2 CTAs][8 NB][HD + 2]: the stretch that began before the CTA, the one that goes on after it
 };
@@ -97,16 +99,34 @@ __device__ __forceinline__ void aq_mma(float (&c)[4], const uint32_t (&a)[4], ui
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void aq_mma_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b)
+{
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};" : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(b));
+}
 __device__ __forceinline__ void aq_mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
-__device__ __forceinline__ void aq_split(float a, float b, uint32_t &hi, uint32_t &lo)
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 aq_sub2(float2 a, float2 b)
 {
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    unsigned long long d;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long *>(&a)), "l"(*reinterpret_cast<unsigned long long *>(&b)));
+    return *reinterpret_cast<float2 *>(&d);
+}
+__device__ __forceinline__ float2 aq_add2(float2 a, float2 b)
+{
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long *>(&a)), "l"(*reinterpret_cast<unsigned long long *>(&b)));
+    return *reinterpret_cast<float2 *>(&d);
+}
+// p = hi + lo, both fp16
+__device__ __forceinline__ void aq_split(float2 p, uint32_t &hi, uint32_t &lo)
+{
+    const __half2 h = __floats2half2_rn(p.x, p.y);
+    const float2 r = aq_sub2(p, __half22float2(h));
+    const __half2 l = __floats2half2_rn(r.x, r.y);
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
@@ -131,6 +151,25 @@ __device__ __forceinline__ uint32_t aq_lds16(uint32_t a)
 // nibble P of each half of the word, as 16 c * 2^-24
 template <int P>
 __device__ __forceinline__ uint32_t aq_codes(uint32_t w) { return (P == 0 ? w << 4 : w >> (P ? 4 * (P - 1) : 0)) & 0x00f000f0u; }
+// nibble P of each half of the word, as the number c - 8
+template <int P>
+__device__ __forceinline__ uint32_t aq_centred(uint32_t w)
+{
+    const uint32_t x = ((P & 2 ? w >> 8 : w) & (P & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;      // 1024 + c, or 1024 + 16 c
+    uint32_t y;
+    if constexpr (P & 1) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(0x2c002c00u), "r"(0xd480d480u));      // x / 16 - 72
+    else asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0xe408e408u));                                              // x - 1032
+    return y;
+}
+__device__ __forceinline__ __half2 aq_h2(uint32_t x) { return *reinterpret_cast<const __half2 *>(&x); }
+__device__ __forceinline__ uint32_t aq_u32(__half2 x) { return *reinterpret_cast<const uint32_t *>(&x); }
+// (hi + lo) d of two keys = h + l: h the rounded product, l what it lacks, exact, and lo d
+__device__ __forceinline__ void aq_weigh(uint32_t hi, uint32_t lo, uint32_t d, uint32_t &h, uint32_t &l)
+{
+    const __half2 p = __hmul2_rn(aq_h2(hi), aq_h2(d));
+    l = aq_u32(__hfma2(aq_h2(lo), aq_h2(d), __hfma2(aq_h2(hi), aq_h2(d), __hneg2(p))));
+    h = aq_u32(p);
+}
 constexpr float AQ_UNSCALE = 1048576.0f;       // 2^20
 __device__ __forceinline__ float aq_lo(uint32_t dm) { return __low2float(*reinterpret_cast<const __half2 *>(&dm)); }
 __device__ __forceinline__ float aq_hi(uint32_t dm) { return __high2float(*reinterpret_cast<const __half2 *>(&dm)); }
@@ -147,11 +186,14 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
     __shared__ long long s_sum[AQ_WARPS], s_rest;
     __shared__ int s_b;
     uint4 *qf = reinterpret_cast<uint4 *>(aq_smem + S::RING);                     // [NB][KS][lane] {hi b0, hi b1, lo b0, lo b1}
-    float *qs = reinterpret_cast<float *>(aq_smem + S::RING + S::QF);             // [NB][G4][8] sums of the scaled query over a block
+    uint2 *qsum = reinterpret_cast<uint2 *>(aq_smem + S::RING + S::QF);           // [NB][lane] {hi, lo} sums of the scaled query over blocks 2t and 2t + 1, times 2^-6
     __shared__ float q_factor[ROWS];
-    float *dump = reinterpret_cast<float *>(aq_smem + S::RING + S::QF + S::QS + S::EX);
+    float *dump = reinterpret_cast<float *>(aq_smem + S::RING);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     float *ex = reinterpret_cast<float *>(aq_smem + S::RING + S::QF + S::QS) + warp * NB * 8 * AQ_SP;
+    // for each key of the warp's chunk: d times 2^b, and the middle m + 8 d of the values that a block can say, as two pieces; [G4][32] halves each
+    __half *tab = reinterpret_cast<__half *>(aq_smem + S::RING + S::QF + S::QS + S::EX) + warp * 3 * G4 * 32;
+    const uint32_t tab_d = smem_u32(tab);
     const int N = gridDim.x, me = blockIdx.x;
 
     if (lane == 0) {
@@ -227,10 +269,11 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
         }
         AqWalk f = w;                                          // the unit being fetched, up to STAGES - 1 further on
         long long f_at = first;
+        auto page_of = [&](int pos) { return (int)(__umulhi((uint32_t)pos, p.page_mul) >> p.page_shift); };
         int entry = -1;                                        // lanes 0 and 1: the table entry of their piece of the next unit to fetch
         auto look = [&]() {
             const int pos = f.begin + f.u * AQ_UNIT + warp * AQ_CHUNK + 16 * lane;
-            entry = f_at < last && lane < 2 && pos < f.end ? kv_entry(__ldg(p.c.table + (size_t)f.b * p.c.stride + pos / p.c.page_tokens), p.c.pages) : -1;
+            entry = f_at < last && lane < 2 && pos < f.end ? kv_entry(__ldg(p.c.table + (size_t)f.b * p.c.stride + page_of(pos)), p.c.pages) : -1;
         };
         const uint32_t ring = smem_u32(aq_smem) + warp * STAGES * S::STAGE;
         auto fetch = [&](int i) {                              // the i-th unit of this CTA into stage i % STAGES
@@ -246,7 +289,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
             __syncwarp();
             if (entry >= 0) {
                 const int pos = f.begin + f.u * AQ_UNIT + warp * AQ_CHUNK + 16 * lane;
-                const size_t at = kv_row(entry, f.h, pos % p.c.page_tokens, p.c.Hkv, p.c.page_tokens, G4);
+                const size_t at = kv_row(entry, f.h, pos - page_of(pos) * p.c.page_tokens, p.c.Hkv, p.c.page_tokens, G4);
                 bulk_g2s(to, p.k + at, 16 * ROW, bar);
                 bulk_g2s(to + AQ_CHUNK * ROW, p.v + at, 16 * ROW, bar);
             }
@@ -275,29 +318,28 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                 const int sh = max(-126, min(126, 141 - ex_top));                                           // largest into [2^14, 2^15)
                 const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
                 if (lane == 0) q_factor[r] = __uint_as_float((uint32_t)(127 - sh) << 23) * p.scale * (1.44269504088896340736f * AQ_UNSCALE);
+                float sum0 = 0.0f, sum1 = 0.0f;                // lane t: of blocks 2t and 2t + 1
 #pragma unroll
                 for (int j = 0; j < G4; ++j) {
                     const float y = x[j] * up;
-                    const float sum = group_sum<32>(y);
-                    if (lane == 0) qs[((r >> 3) * G4 + j) * 8 + (r & 7)] = sum * (1.0f / AQ_UNSCALE);
+                    const float sum = group_sum<32>(y) * 0.015625f;
+                    if (lane == j / 2) (j & 1 ? sum1 : sum0) = sum;
                     // channel c of the block: k-step c / 16, thread t = (c % 16) / 4, place c % 4: b0 holds places 0 and 2, b1 places 1 and 3
                     const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
                     const int place = lane & 3, to = ((((r >> 3) * KS + 2 * j + (lane >> 4)) * 32 + 4 * (r & 7) + ((lane & 15) >> 2)) * 8) + (place & 1) * 2 + (place >> 1);
                     reinterpret_cast<__half *>(qf)[to] = hi;
                     reinterpret_cast<__half *>(qf)[to + 4] = lo;
                 }
+                if (lane < 4) {
+                    uint2 v;
+                    aq_split(make_float2(sum0, sum1), v.x, v.y);
+                    qsum[(r >> 3) * 32 + 4 * (r & 7) + lane] = v;
+                }
             }
             __syncthreads();
-            uint4 qr[NB == 1 ? KS : 1];
-            float2 qsr[NB == 1 ? G4 : 1];
-            if constexpr (NB == 1) {
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) qr[ks] = qf[ks * 32 + lane];
-#pragma unroll
-                for (int j = 0; j < G4; ++j) qsr[j] = make_float2(qs[j * 8 + 2 * t], qs[j * 8 + 2 * t + 1]);
-            }
-            float o[NB][G4][2][4], om[NB][G4], m_run[NB], l_run[NB], fac[NB];
-            int pos_row[NB], e_run = 60;                       // pos_row: the position of row g of each block, -1 where there is none
+            float om[NB][2];                                   // row g: block g's sum of weight times middle
+            float o[NB][G4][2][4], m_run[NB], l_run[NB], fac[NB];
+            int pos_row[NB], b_run = 14;                       // pos_row: the position of row g of each block, -1 where there is none
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 const int row = r0 + 8 * nb + g;
@@ -305,12 +347,9 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                 fac[nb] = q_factor[8 * nb + g];
                 m_run[nb] = -INFINITY;
                 l_run[nb] = 0.0f;
+                om[nb][0] = om[nb][1] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < G4; ++j) {
-                    om[nb][j] = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] = 0.0f;
-                }
+                for (int e = 0; e < G4 * 8; ++e) o[nb][e >> 3][e >> 2 & 1][e & 3] = 0.0f;
             }
             // chunks in [all_from, all_to) are seen by every row
             const int pos_first = w.len - p.c.tokens + r0 / p.G, pos_last = w.len - p.c.tokens + (min(p.R, r0 + ROWS) - 1) / p.G;
@@ -328,17 +367,18 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                 if (there) {
                     const uint32_t kb = ring + stage * S::STAGE, vb = kb + AQ_CHUNK * ROW;
                     const bool mixed = there != 3u || key0 < all_from || key0 + AQ_CHUNK > all_to;
+                    // ---- the values' scales, a lane a key
+                    uint32_t dm[G4], dtop = 0;
+#pragma unroll
+                    for (int j = 0; j < G4; ++j) dm[j] = aq_lds32(vb + lane * ROW + j * KQ4_BLOCK);
                     if (mixed) {
                         // What no row sees must not reach the products even with weight zero (0 x NaN), what some rows see only those: scales that are no
                         // numbers are taken out, and the rows that see them marked.
-                        const int key = key0 + lane;
-                        const bool in = (there >> (lane >> 4) & 1u) && key < w.end;
-                        const uint32_t row = vb + lane * ROW;
-#pragma unroll 1
+                        const bool in = (there >> (lane >> 4) & 1u) && key0 + lane < w.end;
+#pragma unroll
                         for (int j = 0; j < G4; ++j) {
-                            const uint32_t dm = aq_lds32(row + j * KQ4_BLOCK);
-                            const bool nan = in && aq_no_number(dm);
-                            if (!in || nan) asm volatile("st.shared.u32 [%0], %1;" ::"r"(row + j * KQ4_BLOCK), "r"(0u) : "memory");
+                            const bool nan = in && aq_no_number(dm[j]);
+                            if (!in || nan) dm[j] = 0;
                             for (uint32_t bad = __ballot_sync(0xffffffffu, nan); bad; bad &= bad - 1) {
                                 const int at_key = key0 + __ffs(bad) - 1;
 #pragma unroll
@@ -348,154 +388,172 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                                         const int pos = __shfl_sync(0xffffffffu, pos_row[nb], 4 * (2 * t + e));
                                         if (at_key <= pos && (p.window == 0 || at_key > pos - p.window))
 #pragma unroll
-                                            for (int jj = 0; jj < G4; ++jj)
-                                                if (jj == j)
-#pragma unroll
-                                                    for (int x = 0; x < 2; ++x) o[nb][jj][x][e] = o[nb][jj][x][e + 2] = __int_as_float(0x7fffffff);
+                                            for (int x = 0; x < 2; ++x) o[nb][j][x][e] = o[nb][j][x][e + 2] = __int_as_float(0x7fffffff);
                                     }
                             }
                         }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the next copy into this stage comes after these stores
-                        __syncwarp();
+                    }
+#pragma unroll
+                    for (int j = 0; j < G4; ++j) dtop = max(dtop, (dm[j] & 0x7c00u) == 0x7c00u ? 0u : dm[j] & 0x7fffu);
+                    // the largest d so far times 2^b is in [1, 2): its products with weights of up to 2^12 stay in fp16's range, their remainders above its least step
+                    const int b_new = min(b_run, 15 - (int)min(29u, max(1u, __reduce_max_sync(0xffffffffu, dtop) >> 10)));
+                    const __half2 d_scale = aq_h2((uint32_t)(15 + b_new) << 10);
+#pragma unroll
+                    for (int j = 0; j < G4; ++j) {
+                        const float mid = fmaf(8.0f, aq_lo(dm[j]), aq_hi(dm[j]));
+                        const __half hi = __float2half_rn(mid), lo = __float2half_rn(mid - __half2float(hi));
+                        tab[j * 32 + lane] = __low2half(__hmul2_rn(aq_h2(dm[j]), d_scale));
+                        tab[(G4 + j) * 32 + lane] = hi;
+                        tab[(2 * G4 + j) * 32 + lane] = lo;
                     }
                     // ---- scores of 2 x 16 keys
-                    float s[NB][2][4];
+#pragma unroll 1
+                    for (int x = 0; x < 2; ++x) {
+                        float s[NB][4];
+                        const uint32_t key_row = kb + (16 * x + g) * ROW;
+                        {
+                            const uint32_t at0 = key_row + min(2 * t, G4 - 1) * KQ4_BLOCK, at1 = key_row + min(2 * t + 1, G4 - 1) * KQ4_BLOCK;
+                            const uint32_t m0 = __byte_perm(aq_lds32(at0), aq_lds32(at1), 0x7632), m1 = __byte_perm(aq_lds32(at0 + 8 * ROW), aq_lds32(at1 + 8 * ROW), 0x7632);
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
+                            for (int nb = 0; nb < NB; ++nb) {
+                                const uint2 b = qsum[nb * 32 + lane];
+                                s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.0f;
+                                aq_mma_k8(s[nb], m0, m1, b.y);
+                                aq_mma_k8(s[nb], m0, m1, b.x);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) s[nb][e >> 2][e & 3] = 0.0f;
+                                for (int e = 0; e < 4; ++e) s[nb][e] *= 64.0f / AQ_UNSCALE;
+                            }
+                        }
 #pragma unroll
-                    for (int j = 0; j < G4; ++j) {
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint32_t at0 = kb + (16 * x + g) * ROW + j * KQ4_BLOCK, at1 = at0 + 8 * ROW;
-                            const uint32_t c0 = aq_lds32(at0 + 4 + 4 * t), c1 = aq_lds32(at1 + 4 + 4 * t), dm0 = aq_lds32(at0), dm1 = aq_lds32(at1);
+                        for (int j = 0; j < G4; ++j) {
+                            const uint32_t at0 = key_row + j * KQ4_BLOCK, at1 = at0 + 8 * ROW;
+                            const uint32_t c0 = aq_lds32(at0 + 4 + 4 * t), c1 = aq_lds32(at1 + 4 + 4 * t);
+                            const float d0 = aq_lo(aq_lds32(at0)), d1 = aq_lo(aq_lds32(at1));
                             const uint32_t a0[4] = {aq_codes<0>(c0), aq_codes<0>(c1), aq_codes<2>(c0), aq_codes<2>(c1)};
                             const uint32_t a1[4] = {aq_codes<1>(c0), aq_codes<1>(c1), aq_codes<3>(c0), aq_codes<3>(c1)};
-                            const float d0 = aq_lo(dm0), m0 = aq_hi(dm0), d1 = aq_lo(dm1), m1 = aq_hi(dm1);
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
-                                const uint4 b0 = NB == 1 ? qr[NB == 1 ? 2 * j : 0] : qf[(nb * KS + 2 * j) * 32 + lane];
-                                const uint4 b1 = NB == 1 ? qr[NB == 1 ? 2 * j + 1 : 0] : qf[(nb * KS + 2 * j + 1) * 32 + lane];
-                                const float2 qq = NB == 1 ? qsr[NB == 1 ? j : 0] : *reinterpret_cast<const float2 *>(qs + (nb * G4 + j) * 8 + 2 * t);
+                                const uint4 b0 = qf[(nb * KS + 2 * j) * 32 + lane], b1 = qf[(nb * KS + 2 * j + 1) * 32 + lane];
                                 float acc[4];
-                                aq_mma_first(acc, a0, b0.x, b0.y);
-                                aq_mma(acc, a0, b0.z, b0.w);
-                                aq_mma(acc, a1, b1.x, b1.y);
+                                aq_mma_first(acc, a0, b0.z, b0.w);
                                 aq_mma(acc, a1, b1.z, b1.w);
-                                s[nb][x][0] = fmaf(d0, acc[0], fmaf(m0, qq.x, s[nb][x][0]));
-                                s[nb][x][1] = fmaf(d0, acc[1], fmaf(m0, qq.y, s[nb][x][1]));
-                                s[nb][x][2] = fmaf(d1, acc[2], fmaf(m1, qq.x, s[nb][x][2]));
-                                s[nb][x][3] = fmaf(d1, acc[3], fmaf(m1, qq.y, s[nb][x][3]));
-                            }
-                        }
-                    }
-                    // the largest step of the values: what the weights are scaled by
-                    uint32_t dtop = 0;
-#pragma unroll
-                    for (int j = 0; j < G4; ++j) dtop = max(dtop, aq_lds16(vb + lane * ROW + j * KQ4_BLOCK) & 0x7fffu);
-                    dtop = __reduce_max_sync(0xffffffffu, dtop) >> 10;
-                    const int e_new = min(e_run, 29 - (int)min(30u, max(1u, dtop)));
-
-                    // ---- from (keys g, rows 2t) to (row g, keys 2t): weights
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                        for (int x = 0; x < 2; ++x)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) ex[(nb * 8 + 2 * t + (e & 1)) * AQ_SP + 16 * x + 8 * (e >> 1) + g] = s[nb][x][e];
-                    __syncwarp();
-                    float pr[NB][8];                           // keys 16 x + 8 y + 2t + z at [4 x + 2 y + z]
-                    float alpha[NB];
-                    bool moved = e_new != e_run;
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        float top = -INFINITY;
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            const float2 v = *reinterpret_cast<const float2 *>(ex + (nb * 8 + g) * AQ_SP + 8 * y + 2 * t);
-                            pr[nb][2 * y] = v.x * fac[nb];
-                            pr[nb][2 * y + 1] = v.y * fac[nb];
-                            if (mixed) {
-#pragma unroll
-                                for (int z = 0; z < 2; ++z) {
-                                    const int key = key0 + 8 * y + 2 * t + z;
-                                    const bool seen = key <= pos_row[nb] && (p.window == 0 || key > pos_row[nb] - p.window) && (there >> (y >> 1) & 1u);
-                                    if (!seen) pr[nb][2 * y + z] = -INFINITY;
-                                }
-                            }
-                            top = fmaxf(top, fmaxf(pr[nb][2 * y], pr[nb][2 * y + 1]));
-                        }
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                        const float m_new = fmaxf(m_run[nb], top);
-                        moved |= m_new != m_run[nb];
-                        const float ref = (m_new == -INFINITY ? 0.0f : m_new) - (float)e_new;
-                        alpha[nb] = m_run[nb] == -INFINITY ? 0.0f : aq_exp2(m_run[nb] - (float)e_run - ref);
-                        m_run[nb] = m_new;
-                        float sum = 0.0f;
-#pragma unroll
-                        for (int y = 0; y < 8; ++y) {
-                            pr[nb][y] = aq_exp2(pr[nb][y] - ref);
-                            sum += pr[nb][y];
-                        }
-                        l_run[nb] = fmaf(l_run[nb], alpha[nb], sum);
-                    }
-                    e_run = e_new;
-                    if (__any_sync(0xffffffffu, moved)) {      // rare once the first keys have been seen
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) {
-                            const float f0 = __shfl_sync(0xffffffffu, alpha[nb], 8 * t), f1 = __shfl_sync(0xffffffffu, alpha[nb], 8 * t + 4);
-#pragma unroll
-                            for (int j = 0; j < G4; ++j) {
-                                om[nb][j] *= alpha[nb];
-#pragma unroll
-                                for (int x = 0; x < 2; ++x) {
-                                    o[nb][j][x][0] *= f0;
-                                    o[nb][j][x][1] *= f1;
-                                    o[nb][j][x][2] *= f0;
-                                    o[nb][j][x][3] *= f1;
-                                }
-                            }
-                        }
-                    }
-                    // ---- values.  The tensor cores cut what they add to an accumulator instead of rounding it, and all terms here have one sign: sums
-                    // over the chunk start from zero and are added up in fp32 by the rounding adder (300 keys: an error of 2e-5 without, 2e-6 so).
-#pragma unroll
-                    for (int j = 0; j < G4; ++j) {
-                        float acc[NB][2][4];
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const uint32_t at = vb + (16 * x + 2 * t) * ROW + j * KQ4_BLOCK;
-                            const uint32_t dm0 = aq_lds32(at), dm1 = aq_lds32(at + ROW), dm2 = aq_lds32(at + 8 * ROW), dm3 = aq_lds32(at + 9 * ROW);
-                            const uint32_t w0 = __byte_perm(aq_lds16(at + 4 + 2 * g), aq_lds16(at + ROW + 4 + 2 * g), 0x5410);
-                            const uint32_t w1 = __byte_perm(aq_lds16(at + 8 * ROW + 4 + 2 * g), aq_lds16(at + 9 * ROW + 4 + 2 * g), 0x5410);
-                            const uint32_t a0[4] = {aq_codes<0>(w0), aq_codes<1>(w0), aq_codes<0>(w1), aq_codes<1>(w1)};
-                            const uint32_t a1[4] = {aq_codes<2>(w0), aq_codes<3>(w0), aq_codes<2>(w1), aq_codes<3>(w1)};
-#pragma unroll
-                            for (int nb = 0; nb < NB; ++nb) {
-                                const float *q4 = pr[nb] + 4 * x;
-                                om[nb][j] = fmaf(q4[0], aq_hi(dm0), fmaf(q4[1], aq_hi(dm1), fmaf(q4[2], aq_hi(dm2), fmaf(q4[3], aq_hi(dm3), om[nb][j]))));
-                                uint32_t h0, l0, h1, l1;
-                                aq_split(q4[0] * aq_lo(dm0), q4[1] * aq_lo(dm1), h0, l0);
-                                aq_split(q4[2] * aq_lo(dm2), q4[3] * aq_lo(dm3), h1, l1);
-                                if (x == 0) {
-                                    aq_mma_first(acc[nb][0], a0, l0, l1);
-                                    aq_mma_first(acc[nb][1], a1, l0, l1);
-                                } else {
-                                    aq_mma(acc[nb][0], a0, l0, l1);
-                                    aq_mma(acc[nb][1], a1, l0, l1);
-                                }
-                                aq_mma(acc[nb][0], a0, h0, h1);
-                                aq_mma(acc[nb][1], a1, h0, h1);
+                                aq_mma(acc, a0, b0.x, b0.y);
+                                aq_mma(acc, a1, b1.x, b1.y);
+                                s[nb][0] = fmaf(d0, acc[0], s[nb][0]);
+                                s[nb][1] = fmaf(d0, acc[1], s[nb][1]);
+                                s[nb][2] = fmaf(d1, acc[2], s[nb][2]);
+                                s[nb][3] = fmaf(d1, acc[3], s[nb][3]);
                             }
                         }
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] += acc[nb][e >> 2][e & 3];
+                            for (int e = 0; e < 4; ++e) ex[(nb * 8 + 2 * t + (e & 1)) * AQ_SP + 16 * x + 8 * (e >> 1) + g] = s[nb][e];
                     }
-                    __syncwarp();                              // the stage and the exchange are free again
+                    __syncwarp();
+
+                    // ---- from (keys g, rows 2t) to (row g, keys 2t): weights times 2^12, as two pieces
+                    uint32_t ph[NB][4], pl[NB][4];             // keys 8y + 2t and 8y + 2t + 1
+                    float alpha[NB];
+                    bool moved = b_new != b_run;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        float2 v[4];
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            v[y] = *reinterpret_cast<const float2 *>(ex + (nb * 8 + g) * AQ_SP + 8 * y + 2 * t);
+                            if (mixed) {
+                                const int key = key0 + 8 * y + 2 * t, from = p.window > 0 ? pos_row[nb] - p.window : -1;
+                                const bool page = there >> (y >> 1) & 1u;
+                                if (!page || key > pos_row[nb] || key <= from) v[y].x = -INFINITY;
+                                if (!page || key + 1 > pos_row[nb] || key + 1 <= from) v[y].y = -INFINITY;
+                            }
+                            top = fmaxf(top, fmaxf(v[y].x, v[y].y));
+                        }
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                        const float m_new = fmaxf(m_run[nb], top * fac[nb]);
+                        moved |= m_new != m_run[nb];
+                        const float ref = m_new == -INFINITY ? 0.0f : m_new;
+                        alpha[nb] = m_run[nb] == -INFINITY ? 0.0f : aq_exp2(m_run[nb] - ref);
+                        m_run[nb] = m_new;
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            const float2 e = make_float2(aq_exp2(fmaf(v[y].x, fac[nb], 12.0f - ref)), aq_exp2(fmaf(v[y].y, fac[nb], 12.0f - ref)));
+                            sum += e.x + e.y;
+                            aq_split(e, ph[nb][y], pl[nb][y]);
+                        }
+                        l_run[nb] = fmaf(l_run[nb], alpha[nb], sum);
+                    }
+                    if (__any_sync(0xffffffffu, moved)) {      // rare once the first keys have been seen
+                        const float shift = __uint_as_float((uint32_t)(127 + b_new - b_run) << 23);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            const float f0 = __shfl_sync(0xffffffffu, alpha[nb], 8 * t), f1 = __shfl_sync(0xffffffffu, alpha[nb], 8 * t + 4);
+                            om[nb][0] *= f0;
+                            om[nb][1] *= f1;
+#pragma unroll
+                            for (int e = 0; e < G4 * 8; ++e) o[nb][e >> 3][e >> 2 & 1][e & 3] *= (e & 1 ? f1 : f0) * shift;
+                        }
+                        b_run = b_new;
+                    }
+                    // ---- values.  The tensor cores cut what they add to an accumulator instead of rounding it: a tile's sums start from zero and are
+                    // added up by the rounding adder, and codes are taken from their middle, so that the terms do not all have one sign.
+#pragma unroll 1
+                    for (int x = 0; x < 2; ++x) {
+                        uint32_t p0[NB], p1[NB], r0_[NB], r1_[NB];
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            p0[nb] = x ? ph[nb][2] : ph[nb][0];
+                            p1[nb] = x ? ph[nb][3] : ph[nb][1];
+                            r0_[nb] = x ? pl[nb][2] : pl[nb][0];
+                            r1_[nb] = x ? pl[nb][3] : pl[nb][1];
+                        }
+                        const uint32_t at_t = tab_d + (16 * x + 2 * t) * 2;
+                        {
+                            const uint32_t at_m = at_t + (G4 + min(g, G4 - 1)) * 64;
+                            const uint32_t hi[4] = {aq_lds32(at_m), 0, aq_lds32(at_m + 16), 0}, lo[4] = {aq_lds32(at_m + G4 * 64), 0, aq_lds32(at_m + G4 * 64 + 16), 0};
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) {
+                                float acc[4];
+                                aq_mma_first(acc, lo, p0[nb], p1[nb]);
+                                aq_mma(acc, hi, r0_[nb], r1_[nb]);
+                                aq_mma(acc, hi, p0[nb], p1[nb]);
+                                om[nb][0] += acc[0];
+                                om[nb][1] += acc[1];
+                            }
+                        }
+                        const uint32_t key_row = vb + (16 * x + 2 * t) * ROW + 4 + 2 * g;
+#pragma unroll
+                        for (int j = 0; j < G4; ++j) {
+                            const uint32_t at = key_row + j * KQ4_BLOCK, d0 = aq_lds32(at_t + j * 64), d1 = aq_lds32(at_t + j * 64 + 16);
+                            const uint32_t w0 = __byte_perm(aq_lds16(at), aq_lds16(at + ROW), 0x5410), w1 = __byte_perm(aq_lds16(at + 8 * ROW), aq_lds16(at + 9 * ROW), 0x5410);
+                            const uint32_t a0[4] = {aq_centred<0>(w0), aq_centred<1>(w0), aq_centred<0>(w1), aq_centred<1>(w1)};
+                            const uint32_t a1[4] = {aq_centred<2>(w0), aq_centred<3>(w0), aq_centred<2>(w1), aq_centred<3>(w1)};
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) {
+                                uint32_t h0, l0, h1, l1;
+                                aq_weigh(p0[nb], r0_[nb], d0, h0, l0);
+                                aq_weigh(p1[nb], r1_[nb], d1, h1, l1);
+                                float acc[2][4];
+                                aq_mma_first(acc[0], a0, l0, l1);
+                                aq_mma_first(acc[1], a1, l0, l1);
+                                aq_mma(acc[0], a0, h0, h1);
+                                aq_mma(acc[1], a1, h0, h1);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    float *to = &o[nb][j][e >> 1][2 * (e & 1)];
+                                    const float *add = &acc[e >> 1][2 * (e & 1)];
+                                    const float2 sum = aq_add2(make_float2(to[0], to[1]), make_float2(add[0], add[1]));
+                                    to[0] = sum.x;
+                                    to[1] = sum.y;
+                                }
+                            }
+                        }
+                    }
+                    __syncwarp();                              // the stage, the exchange and the table are free again
                 }
                 ++i;
                 ++at;
@@ -503,25 +561,18 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
             }
 
             // ---- the stretch ends here: the four warps' results, relative to 2^ref, become one
+            const float unscale = __uint_as_float((uint32_t)(127 - b_run) << 23);
             float ref[NB];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                ref[nb] = m_run[nb] == -INFINITY ? -INFINITY : m_run[nb] - (float)e_run;
+                ref[nb] = m_run[nb];
                 l_run[nb] += __shfl_xor_sync(0xffffffffu, l_run[nb], 1);
                 l_run[nb] += __shfl_xor_sync(0xffffffffu, l_run[nb], 2);
 #pragma unroll
                 for (int j = 0; j < G4; ++j) {
-                    float a = om[nb][j];
-                    a += __shfl_xor_sync(0xffffffffu, a, 1);
-                    a += __shfl_xor_sync(0xffffffffu, a, 2);
-                    const float a0 = __shfl_sync(0xffffffffu, a, 8 * t), a1 = __shfl_sync(0xffffffffu, a, 8 * t + 4);
+                    const float a0 = __shfl_sync(0xffffffffu, om[nb][0], 4 * j + t), a1 = __shfl_sync(0xffffffffu, om[nb][1], 4 * j + t);
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        o[nb][j][x][0] = fmaf(o[nb][j][x][0], AQ_UNSCALE, a0);
-                        o[nb][j][x][1] = fmaf(o[nb][j][x][1], AQ_UNSCALE, a1);
-                        o[nb][j][x][2] = fmaf(o[nb][j][x][2], AQ_UNSCALE, a0);
-                        o[nb][j][x][3] = fmaf(o[nb][j][x][3], AQ_UNSCALE, a1);
-                    }
+                    for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] = fmaf(o[nb][j][e >> 2][e & 3], unscale, e & 1 ? a1 : a0);
                 }
             }
             auto put = [&](float *to) {
@@ -550,6 +601,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                 }
             };
             float *half = dump + (warp & 1) * (S::DUMP / 4);
+            __syncthreads();                                   // the queries are no longer needed
             if (warp >= 2) put(half);
             __syncthreads();
             if (warp < 2) join(half);
@@ -678,17 +730,17 @@ static size_t aq_bytes()
 }
 
 // Blocks of 8 query rows that share the codes a CTA unpacks.
-static int aq_blocks(long long rows, int hd) { return rows <= 8 ? 1 : (rows <= 16 || hd > 128 ? 2 : 4); }
+static int aq_blocks(long long rows, int hd) { (void)hd; return rows <= 8 ? 1 : 2; }
 
 }  // namespace ckb
 
 using namespace ckb;
 
-#define AQ_EACH(hd, nb, F)                                                          \
-    (hd == 64 ? (nb == 1 ? F<64, 1> : nb == 2 ? F<64, 2> : F<64, 4>)                \
-     : hd == 96 ? (nb == 1 ? F<96, 1> : nb == 2 ? F<96, 2> : F<96, 4>)              \
-     : hd == 128 ? (nb == 1 ? F<128, 1> : nb == 2 ? F<128, 2> : F<128, 4>)          \
-     : hd == 192 ? (nb == 1 ? F<192, 1> : F<192, 2>)                                \
+#define AQ_EACH(hd, nb, F)                                \
+    (hd == 64 ? (nb == 1 ? F<64, 1> : F<64, 2>)           \
+     : hd == 96 ? (nb == 1 ? F<96, 1> : F<96, 2>)         \
+     : hd == 128 ? (nb == 1 ? F<128, 1> : F<128, 2>)      \
+     : hd == 192 ? (nb == 1 ? F<192, 1> : F<192, 2>)      \
                  : (nb == 1 ? F<256, 1> : F<256, 2>))
 
 extern "C" size_t ckb200_attention_q4cache_workspace_bytes(int batch, int num_tokens, int num_heads, int num_kv_heads, int head_dim)
@@ -733,6 +785,9 @@ extern "C" int ckb200_dev_attention_q4cache(const float *q, long long q_stride, 
     p.window = sliding_window;
     p.scale = 1.0f / sqrtf((float)head_dim);
     p.err = ckb_device_error_word();
+    p.page_shift = 3;                                          // 2^(page_shift + 1) >= page_tokens >= 16: exact for positions below 2^31
+    while (2u << p.page_shift < (uint32_t)page_tokens) ++p.page_shift;
+    p.page_mul = (uint32_t)((((uint64_t)1 << (32 + p.page_shift)) + page_tokens - 1) / page_tokens);
     const bool joins = (long long)table_stride * page_tokens > AQ_UNIT;           // else no stretch has two units
     const int nb = aq_blocks(p.R, head_dim);
     return AQ_EACH(head_dim, nb, aq_launch)(p, workspace, joins, ckb_stream(stream));

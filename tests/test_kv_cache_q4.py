@@ -307,6 +307,21 @@ def test_rows_that_are_no_numbers(gpu, which, head_dim):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_a_row_that_is_no_number_spoils_its_block_alone(gpu, head_dim):
+    """A value block of NaN early in a long context, seen by every query: the other blocks' channels are as exact as without it."""
+    rng = np.random.default_rng(13)
+    c = random_cache(rng, 1, head_dim, 16, [400])
+    page, slot = c.place(0, 10)
+    c.v[page, 0, slot, :4] = 255
+    q = rng.standard_normal((1, 4 * head_dim)).astype(np.float32)
+    got = Device(gpu, c).attention(q, 1, 4).reshape(4, head_dim)
+    want, off = (a.reshape(4, head_dim) for a in c.attention(q, 1, 4))
+    assert np.isnan(got[:, :32]).all() and np.isnan(want[:, :32]).all()
+    near(got[:, 32:], want[:, 32:], off[:, 32:])
+
+
+@pytest.mark.gpu
 def test_attention_rows_of_wider_tensors(gpu):
     """q is a part of a fused projection's rows at an odd place, out a part of a wider tensor whose other columns stay as they are."""
     rng = np.random.default_rng(8)
