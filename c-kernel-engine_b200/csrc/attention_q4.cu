@@ -17,9 +17,9 @@
 // A query row is a (token, head) of the kv head's group: up to 8 NB rows share every code that is unpacked (NB = 1 for decoding, more for
 // drafts and portions of prompts).
 //
-// Work.  A unit is 128 keys of one (sequence, kv head, 8 NB rows); the units of all sequences form one line that is cut evenly among the CTAs that
+// Work.  A unit is 128 or 256 keys of one (sequence, kv head, 8 NB rows); the units of all sequences form one line that is cut evenly among the CTAs that
 // the GPU holds at once, so long and short sequences load it alike and nothing but the lengths on the device decides.  Each of the four warps takes
-// 32 keys of a unit through a ring of its own (untiled bulk copies of 16-key pieces, the largest that never leave a page), without meeting the
+// a quarter of a unit through a ring of its own (untiled bulk copies of 16-key pieces, the largest that never leave a page), without meeting the
 // others until a sequence's stretch ends.  Stretches that lie within one CTA are written out at once, the others as partial results that
 // a second kernel joins (log-sum-exp).
 #include <cuda_fp16.h>
@@ -34,18 +34,19 @@
 
 namespace ckb {
 
-constexpr int AQ_WARPS = 4, AQ_THREADS = 32 * AQ_WARPS, AQ_CHUNK = 32, AQ_UNIT = AQ_WARPS * AQ_CHUNK;
-constexpr int AQ_SP = 40;                      // floats between rows of the score exchange: 8 lanes' float2 loads touch every bank once
+constexpr int AQ_WARPS = 4, AQ_THREADS = 32 * AQ_WARPS;
 constexpr int AQ_MERGE_WARPS = 8;
 
 template <int HD, int NB>
 struct AqShape {
     static constexpr int G4 = HD / 32, KS = HD / 16, ROW = G4 * KQ4_BLOCK, ROWS = 8 * NB;
-    static constexpr int STAGE = 2 * AQ_CHUNK * ROW;                              // K rows, then V rows
-    static constexpr int CTAS = NB > 1 && HD > 192 ? 1 : (NB > 1 || HD > 128 ? 2 : 4);                       // resident on an SM, for which registers and shared memory are kept
-    static constexpr int STAGES = HD <= 64 ? 4 : 2;
+    static constexpr int XT = 2, CHUNK = 16 * XT, UNIT = AQ_WARPS * CHUNK;      // a warp takes XT tiles of 16 keys at a time
+    static constexpr int SP = CHUNK + 8;                                          // floats between rows of the score exchange: 8 lanes' float2 loads touch every bank once
+    static constexpr int STAGE = 2 * CHUNK * ROW;                              // K rows, then V rows
+    static constexpr int CTAS = NB > 1 && HD > 192 ? 1 : (NB > 1 || HD > 128 ? 2 : 3);                       // resident on an SM, for which registers and shared memory are kept
+    static constexpr int STAGES = HD <= 64 ? 4 : (HD <= 128 && NB < 3 ? 3 : 2);
     static constexpr int OREG = NB * G4 * 8, DUMP = (OREG + 2 * NB) * 32 * 4;      // a warp's accumulators, maxima and sums, register by register
-    static constexpr int RING = AQ_WARPS * STAGES * STAGE, QF = NB * KS * 32 * 16, QS = NB * 32 * 8, EX = AQ_WARPS * NB * 8 * AQ_SP * 4, TAB = AQ_WARPS * 3 * G4 * 64;
+    static constexpr int RING = AQ_WARPS * STAGES * STAGE, QF = NB * KS * 32 * 16, QS = NB * 32 * 8, EX = AQ_WARPS * NB * 8 * SP * 4, TAB = AQ_WARPS * 3 * G4 * 2 * CHUNK;
     static constexpr int SMEM = RING + (QF + QS + EX + TAB > 2 * DUMP ? QF + QS + EX + TAB : 2 * DUMP);      // the exchange between warps lies over the queries
     static_assert(CTAS * (SMEM + 2048) <= 227 * 1024, "shared memory");
 };
@@ -65,19 +66,19 @@ struct AqParams {
 
 // where a CTA is on the line of units
 struct AqWalk {
-    int b, h, rc, u, n, begin, end, len;       // unit u of n; keys [begin, end), begin a multiple of 32
+    int b, h, rc, u, n, begin, end, len;       // unit u of n; keys [begin, end), begin a multiple of 16
 };
 // tokens r0 / G .. of block rc: the keys that any of them sees
-__device__ __forceinline__ void aq_range(const AqParams &p, int nrows, AqWalk &w)
+__device__ __forceinline__ void aq_range(const AqParams &p, int nrows, int unit, AqWalk &w)
 {
     const int t0 = w.rc * nrows / p.G, t1 = (min(p.R, (w.rc + 1) * nrows) - 1) / p.G, at = w.len - p.c.tokens;
     w.end = max(0, at + t1 + 1);
-    w.begin = p.window > 0 ? max(0, at + t0 - p.window + 1) & ~(AQ_CHUNK - 1) : 0;
-    w.n = w.end > w.begin ? (w.end - w.begin + AQ_UNIT - 1) / AQ_UNIT : 0;
+    w.begin = p.window > 0 ? max(0, at + t0 - p.window + 1) & ~15 : 0;
+    w.n = w.end > w.begin ? (w.end - w.begin + unit - 1) / unit : 0;
 }
 __device__ __forceinline__ int aq_length(const AqParams &p, int b) { return kv_len(__ldg(p.c.lens + b), p.c.stride, p.c.page_tokens); }
 // the next stretch that has units; its first one.  False: there is none
-__device__ __forceinline__ bool aq_next_stretch(const AqParams &p, int nrows, AqWalk &w)
+__device__ __forceinline__ bool aq_next_stretch(const AqParams &p, int nrows, int unit, AqWalk &w)
 {
     w.u = 0;
     for (;;) {
@@ -89,7 +90,7 @@ __device__ __forceinline__ bool aq_next_stretch(const AqParams &p, int nrows, Aq
                 w.len = aq_length(p, w.b);
             }
         }
-        aq_range(p, nrows, w);
+        aq_range(p, nrows, unit, w);
         if (w.n) return true;
     }
 }
@@ -115,12 +116,6 @@ __device__ __forceinline__ float2 aq_sub2(float2 a, float2 b)
     asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long *>(&a)), "l"(*reinterpret_cast<unsigned long long *>(&b)));
     return *reinterpret_cast<float2 *>(&d);
 }
-__device__ __forceinline__ float2 aq_add2(float2 a, float2 b)
-{
-    unsigned long long d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<unsigned long long *>(&a)), "l"(*reinterpret_cast<unsigned long long *>(&b)));
-    return *reinterpret_cast<float2 *>(&d);
-}
 // p = hi + lo, both fp16
 __device__ __forceinline__ void aq_split(float2 p, uint32_t &hi, uint32_t &lo)
 {
@@ -136,18 +131,8 @@ __device__ __forceinline__ float aq_exp2(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));       // two units in the last place
     return y;
 }
-__device__ __forceinline__ uint32_t aq_lds32(uint32_t a)
-{
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint32_t aq_lds16(uint32_t a)
-{
-    uint16_t v;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
-    return v;
-}
+__device__ __forceinline__ uint32_t aq_u32(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
+__device__ __forceinline__ uint32_t aq_u16(const uint8_t *p) { return *reinterpret_cast<const uint16_t *>(p); }
 // nibble P of each half of the word, as 16 c * 2^-24
 template <int P>
 __device__ __forceinline__ uint32_t aq_codes(uint32_t w) { return (P == 0 ? w << 4 : w >> (P ? 4 * (P - 1) : 0)) & 0x00f000f0u; }
@@ -155,20 +140,20 @@ __device__ __forceinline__ uint32_t aq_codes(uint32_t w) { return (P == 0 ? w <<
 template <int P>
 __device__ __forceinline__ uint32_t aq_centred(uint32_t w)
 {
-    const uint32_t x = ((P & 2 ? w >> 8 : w) & (P & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;      // 1024 + c, or 1024 + 16 c
-    uint32_t y;
+    uint32_t x, y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(P & 2 ? w >> 8 : w), "r"(P & 1 ? 0x00f000f0u : 0x000f000fu), "r"(0x64006400u));      // and, or: 1024 + c, or 1024 + 16 c
     if constexpr (P & 1) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(0x2c002c00u), "r"(0xd480d480u));      // x / 16 - 72
     else asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0xe408e408u));                                              // x - 1032
     return y;
 }
 __device__ __forceinline__ __half2 aq_h2(uint32_t x) { return *reinterpret_cast<const __half2 *>(&x); }
-__device__ __forceinline__ uint32_t aq_u32(__half2 x) { return *reinterpret_cast<const uint32_t *>(&x); }
+__device__ __forceinline__ uint32_t aq_bits(__half2 x) { return *reinterpret_cast<const uint32_t *>(&x); }
 // (hi + lo) d of two keys = h + l: h the rounded product, l what it lacks, exact, and lo d
 __device__ __forceinline__ void aq_weigh(uint32_t hi, uint32_t lo, uint32_t d, uint32_t &h, uint32_t &l)
 {
     const __half2 p = __hmul2_rn(aq_h2(hi), aq_h2(d));
-    l = aq_u32(__hfma2(aq_h2(lo), aq_h2(d), __hfma2(aq_h2(hi), aq_h2(d), __hneg2(p))));
-    h = aq_u32(p);
+    l = aq_bits(__hfma2(aq_h2(lo), aq_h2(d), __hfma2(aq_h2(hi), aq_h2(d), __hneg2(p))));
+    h = aq_bits(p);
 }
 constexpr float AQ_UNSCALE = 1048576.0f;       // 2^20
 __device__ __forceinline__ float aq_lo(uint32_t dm) { return __low2float(*reinterpret_cast<const __half2 *>(&dm)); }
@@ -186,14 +171,13 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
     __shared__ long long s_sum[AQ_WARPS], s_rest;
     __shared__ int s_b;
     uint4 *qf = reinterpret_cast<uint4 *>(aq_smem + S::RING);                     // [NB][KS][lane] {hi b0, hi b1, lo b0, lo b1}
-    uint2 *qsum = reinterpret_cast<uint2 *>(aq_smem + S::RING + S::QF);           // [NB][lane] {hi, lo} sums of the scaled query over blocks 2t and 2t + 1, times 2^-6
+    uint2 *qsum = reinterpret_cast<uint2 *>(aq_smem + S::RING + S::QF);           // [NB][lane] {hi, lo} sums of the scaled query over blocks 2t and 2t + 1, times 2^-20
     __shared__ float q_factor[ROWS];
     float *dump = reinterpret_cast<float *>(aq_smem + S::RING);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    float *ex = reinterpret_cast<float *>(aq_smem + S::RING + S::QF + S::QS) + warp * NB * 8 * AQ_SP;
-    // for each key of the warp's chunk: d times 2^b, and the middle m + 8 d of the values that a block can say, as two pieces; [G4][32] halves each
-    __half *tab = reinterpret_cast<__half *>(aq_smem + S::RING + S::QF + S::QS + S::EX) + warp * 3 * G4 * 32;
-    const uint32_t tab_d = smem_u32(tab);
+    float *ex = reinterpret_cast<float *>(aq_smem + S::RING + S::QF + S::QS) + warp * NB * 8 * S::SP;
+    // for each key of the warp's chunk: d times 2^b, and the middle m + 8 d of the values that a block can say, as two pieces; [G4][keys] halves each
+    __half *tab = reinterpret_cast<__half *>(aq_smem + S::RING + S::QF + S::QS + S::EX) + warp * 3 * G4 * S::CHUNK;
     const int N = gridDim.x, me = blockIdx.x;
 
     if (lane == 0) {
@@ -210,7 +194,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
         w.len = aq_length(p, b);
         long long n = 0;
         for (w.rc = 0; w.rc < p.RC; ++w.rc) {
-            aq_range(p, ROWS, w);
+            aq_range(p, ROWS, S::UNIT, w);
             n += w.n;
         }
         return n * p.c.Hkv;
@@ -255,13 +239,13 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
         {
             long long rest = s_rest, per_head = 0;
             for (w.rc = 0; w.rc < p.RC; ++w.rc) {
-                aq_range(p, ROWS, w);
+                aq_range(p, ROWS, S::UNIT, w);
                 per_head += w.n;
             }
             w.h = (int)(rest / per_head);
             rest -= per_head * w.h;
             for (w.rc = 0;; ++w.rc) {
-                aq_range(p, ROWS, w);
+                aq_range(p, ROWS, S::UNIT, w);
                 if (rest < w.n) break;
                 rest -= w.n;
             }
@@ -270,34 +254,51 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
         AqWalk f = w;                                          // the unit being fetched, up to STAGES - 1 further on
         long long f_at = first;
         auto page_of = [&](int pos) { return (int)(__umulhi((uint32_t)pos, p.page_mul) >> p.page_shift); };
-        int entry = -1;                                        // lanes 0 and 1: the table entry of their piece of the next unit to fetch
-        auto look = [&]() {
-            const int pos = f.begin + f.u * AQ_UNIT + warp * AQ_CHUNK + 16 * lane;
-            entry = f_at < last && lane < 2 && pos < f.end ? kv_entry(__ldg(p.c.table + (size_t)f.b * p.c.stride + page_of(pos)), p.c.pages) : -1;
-        };
+        // Lane 0 fetches: the table's entry for the start of the next chunk is read one chunk ahead.  A chunk that cannot span pages is one copy
+        // of K rows and one of V rows, another one as many as it has pieces of 16.
+        const bool one_page = p.c.page_tokens % S::CHUNK == 0 && p.window == 0;
+        const size_t page_bytes = kv_row(1, 0, 0, p.c.Hkv, p.c.page_tokens, G4);
+        int entry = -1;
+        auto look = [&](int pos) { return pos < f.end ? kv_entry(__ldg(p.c.table + (size_t)f.b * p.c.stride + page_of(pos)), p.c.pages) : -1; };
         const uint32_t ring = smem_u32(aq_smem) + warp * STAGES * S::STAGE;
         auto fetch = [&](int i) {                              // the i-th unit of this CTA into stage i % STAGES
             if (f_at >= last) return;
-            __syncwarp();
-            const int stage = i % STAGES;
-            const uint32_t bar = smem_u32(&full[warp][stage]), to = ring + stage * S::STAGE + lane * 16 * ROW;
-            const uint32_t there = __ballot_sync(0xffffffffu, entry >= 0) & 3u;
             if (lane == 0) {
-                pieces[warp][stage] = there;
-                mbar_arrive_expect_tx(bar, __popc(there) * 2 * 16 * ROW);
-            }
-            __syncwarp();
-            if (entry >= 0) {
-                const int pos = f.begin + f.u * AQ_UNIT + warp * AQ_CHUNK + 16 * lane;
-                const size_t at = kv_row(entry, f.h, pos - page_of(pos) * p.c.page_tokens, p.c.Hkv, p.c.page_tokens, G4);
-                bulk_g2s(to, p.k + at, 16 * ROW, bar);
-                bulk_g2s(to + AQ_CHUNK * ROW, p.v + at, 16 * ROW, bar);
+                const int stage = i % STAGES, pos = f.begin + f.u * S::UNIT + warp * S::CHUNK;
+                const uint32_t bar = smem_u32(&full[warp][stage]), to = ring + stage * S::STAGE;
+                if (one_page) {
+                    const int n = entry < 0 ? 0 : min(S::XT, (f.end - pos + 15) >> 4);
+                    pieces[warp][stage] = (1 << n) - 1;
+                    mbar_arrive_expect_tx(bar, n * 2 * 16 * ROW);
+                    if (n) {
+                        const size_t at = (size_t)entry * page_bytes + (uint32_t)((f.h * p.c.page_tokens + pos - page_of(pos) * p.c.page_tokens) * ROW);
+                        bulk_g2s(to, p.k + at, n * 16 * ROW, bar);
+                        bulk_g2s(to + S::CHUNK * ROW, p.v + at, n * 16 * ROW, bar);
+                    }
+                } else {
+                    int e[S::XT], there = 0;
+#pragma unroll
+                    for (int x = 0; x < S::XT; ++x) {
+                        e[x] = x ? look(pos + 16 * x) : entry;
+                        there |= (e[x] >= 0) << x;
+                    }
+                    pieces[warp][stage] = there;
+                    mbar_arrive_expect_tx(bar, __popc(there) * 2 * 16 * ROW);
+#pragma unroll
+                    for (int x = 0; x < S::XT; ++x)
+                        if (e[x] >= 0) {
+                            const int at_pos = pos + 16 * x;
+                            const size_t at = kv_row(e[x], f.h, at_pos - page_of(at_pos) * p.c.page_tokens, p.c.Hkv, p.c.page_tokens, G4);
+                            bulk_g2s(to + 16 * x * ROW, p.k + at, 16 * ROW, bar);
+                            bulk_g2s(to + (S::CHUNK + 16 * x) * ROW, p.v + at, 16 * ROW, bar);
+                        }
+                }
             }
             ++f_at;
-            if (++f.u >= f.n && f_at < last) aq_next_stretch(p, ROWS, f);
-            look();
+            if (++f.u >= f.n && f_at < last) aq_next_stretch(p, ROWS, S::UNIT, f);
+            if (lane == 0 && f_at < last) entry = look(f.begin + f.u * S::UNIT + warp * S::CHUNK);
         };
-        look();
+        if (lane == 0) entry = look(f.begin + f.u * S::UNIT + warp * S::CHUNK);
         for (int i = 0; i < STAGES - 1; ++i) fetch(i);
 
         int i = 0;
@@ -322,7 +323,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
 #pragma unroll
                 for (int j = 0; j < G4; ++j) {
                     const float y = x[j] * up;
-                    const float sum = group_sum<32>(y) * 0.015625f;
+                    const float sum = group_sum<32>(y) * (1.0f / AQ_UNSCALE);
                     if (lane == j / 2) (j & 1 ? sum1 : sum0) = sum;
                     // channel c of the block: k-step c / 16, thread t = (c % 16) / 4, place c % 4: b0 holds places 0 and 2, b1 places 1 and 3
                     const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
@@ -363,106 +364,128 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                     if (lane == 0) atomicExch(p.err, DEV_ERR_FULL_WAIT);
                 }
                 const uint32_t there = pieces[warp][stage];
-                const int key0 = w.begin + w.u * AQ_UNIT + warp * AQ_CHUNK;
+                const int key0 = w.begin + w.u * S::UNIT + warp * S::CHUNK;
                 if (there) {
-                    const uint32_t kb = ring + stage * S::STAGE, vb = kb + AQ_CHUNK * ROW;
-                    const bool mixed = there != 3u || key0 < all_from || key0 + AQ_CHUNK > all_to;
+                    const uint8_t *kb = aq_smem + (warp * STAGES + stage) * S::STAGE, *vb = kb + S::CHUNK * ROW;
+                    const bool mixed = there != (1u << S::XT) - 1u || key0 < all_from || key0 + S::CHUNK > all_to;
                     // ---- the values' scales, a lane a key
-                    uint32_t dm[G4], dtop = 0;
+                    constexpr int KL = S::CHUNK / 32;
+                    uint32_t dm[KL][G4], dtop = 0;
 #pragma unroll
-                    for (int j = 0; j < G4; ++j) dm[j] = aq_lds32(vb + lane * ROW + j * KQ4_BLOCK);
+                    for (int y = 0; y < KL; ++y)
+#pragma unroll
+                        for (int j = 0; j < G4; ++j) dm[y][j] = aq_u32(vb + (32 * y + lane) * ROW + j * KQ4_BLOCK);
                     if (mixed) {
                         // What no row sees must not reach the products even with weight zero (0 x NaN), what some rows see only those: scales that are no
                         // numbers are taken out, and the rows that see them marked.
-                        const bool in = (there >> (lane >> 4) & 1u) && key0 + lane < w.end;
 #pragma unroll
-                        for (int j = 0; j < G4; ++j) {
-                            const bool nan = in && aq_no_number(dm[j]);
-                            if (!in || nan) dm[j] = 0;
-                            for (uint32_t bad = __ballot_sync(0xffffffffu, nan); bad; bad &= bad - 1) {
-                                const int at_key = key0 + __ffs(bad) - 1;
+                        for (int y = 0; y < KL; ++y) {
+                            const bool in = (there >> (2 * y + (lane >> 4)) & 1u) && key0 + 32 * y + lane < w.end;
 #pragma unroll
-                                for (int nb = 0; nb < NB; ++nb)
+                            for (int j = 0; j < G4; ++j) {
+                                const bool nan = in && aq_no_number(dm[y][j]);
+                                if (!in || nan) dm[y][j] = 0;
+                                for (uint32_t bad = __ballot_sync(0xffffffffu, nan); bad; bad &= bad - 1) {
+                                    const int at_key = key0 + 32 * y + __ffs(bad) - 1;
 #pragma unroll
-                                    for (int e = 0; e < 2; ++e) {
-                                        const int pos = __shfl_sync(0xffffffffu, pos_row[nb], 4 * (2 * t + e));
-                                        if (at_key <= pos && (p.window == 0 || at_key > pos - p.window))
+                                    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                                            for (int x = 0; x < 2; ++x) o[nb][j][x][e] = o[nb][j][x][e + 2] = __int_as_float(0x7fffffff);
-                                    }
+                                        for (int e = 0; e < 2; ++e) {
+                                            const int pos = __shfl_sync(0xffffffffu, pos_row[nb], 4 * (2 * t + e));
+                                            if (at_key <= pos && (p.window == 0 || at_key > pos - p.window))
+#pragma unroll
+                                                for (int x = 0; x < 2; ++x) o[nb][j][x][e] = o[nb][j][x][e + 2] = __int_as_float(0x7fffffff);
+                                        }
+                                }
                             }
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < G4; ++j) dtop = max(dtop, (dm[j] & 0x7c00u) == 0x7c00u ? 0u : dm[j] & 0x7fffu);
+                    for (int y = 0; y < KL; ++y)
+#pragma unroll
+                        for (int j = 0; j < G4; ++j) dtop = max(dtop, (dm[y][j] & 0x7c00u) == 0x7c00u ? 0u : dm[y][j] & 0x7fffu);
                     // the largest d so far times 2^b is in [1, 2): its products with weights of up to 2^12 stay in fp16's range, their remainders above its least step
                     const int b_new = min(b_run, 15 - (int)min(29u, max(1u, __reduce_max_sync(0xffffffffu, dtop) >> 10)));
                     const __half2 d_scale = aq_h2((uint32_t)(15 + b_new) << 10);
 #pragma unroll
-                    for (int j = 0; j < G4; ++j) {
-                        const float mid = fmaf(8.0f, aq_lo(dm[j]), aq_hi(dm[j]));
-                        const __half hi = __float2half_rn(mid), lo = __float2half_rn(mid - __half2float(hi));
-                        tab[j * 32 + lane] = __low2half(__hmul2_rn(aq_h2(dm[j]), d_scale));
-                        tab[(G4 + j) * 32 + lane] = hi;
-                        tab[(2 * G4 + j) * 32 + lane] = lo;
-                    }
-                    // ---- scores of 2 x 16 keys
-#pragma unroll 1
-                    for (int x = 0; x < 2; ++x) {
-                        float s[NB][4];
-                        const uint32_t key_row = kb + (16 * x + g) * ROW;
-                        {
-                            const uint32_t at0 = key_row + min(2 * t, G4 - 1) * KQ4_BLOCK, at1 = key_row + min(2 * t + 1, G4 - 1) * KQ4_BLOCK;
-                            const uint32_t m0 = __byte_perm(aq_lds32(at0), aq_lds32(at1), 0x7632), m1 = __byte_perm(aq_lds32(at0 + 8 * ROW), aq_lds32(at1 + 8 * ROW), 0x7632);
+                    for (int y = 0; y < KL; ++y)
+#pragma unroll
+                        for (int j = 0; j < G4; ++j) {
+                            const float mid = fmaf(8.0f, aq_lo(dm[y][j]), aq_hi(dm[y][j]));
+                            const __half hi = __float2half_rn(mid), lo = __float2half_rn(mid - __half2float(hi));
+                            tab[j * S::CHUNK + 32 * y + lane] = __low2half(__hmul2_rn(aq_h2(dm[y][j]), d_scale));
+                            tab[(G4 + j) * S::CHUNK + 32 * y + lane] = hi;
+                            tab[(2 * G4 + j) * S::CHUNK + 32 * y + lane] = lo;
+                        }
+                    // ---- scores of tiles of 16 keys.  A product waits long for the one before it in its sum: those of several tiles and blocks take turns.
+                    {
+                        float s[S::XT][NB][4];
+                        const uint8_t *key_row = kb + g * ROW;
+#pragma unroll
+                        for (int x = 0; x < S::XT; ++x) {
+                            const uint8_t *at0 = key_row + 16 * x * ROW + min(2 * t, G4 - 1) * KQ4_BLOCK, *at1 = key_row + 16 * x * ROW + min(2 * t + 1, G4 - 1) * KQ4_BLOCK;
+                            const uint32_t m0 = __byte_perm(aq_u32(at0), aq_u32(at1), 0x7632), m1 = __byte_perm(aq_u32(at0 + 8 * ROW), aq_u32(at1 + 8 * ROW), 0x7632);
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
                                 const uint2 b = qsum[nb * 32 + lane];
-                                s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.0f;
-                                aq_mma_k8(s[nb], m0, m1, b.y);
-                                aq_mma_k8(s[nb], m0, m1, b.x);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) s[nb][e] *= 64.0f / AQ_UNSCALE;
+                                s[x][nb][0] = s[x][nb][1] = s[x][nb][2] = s[x][nb][3] = 0.0f;
+                                aq_mma_k8(s[x][nb], m0, m1, b.y);
+                                aq_mma_k8(s[x][nb], m0, m1, b.x);
                             }
                         }
 #pragma unroll
                         for (int j = 0; j < G4; ++j) {
-                            const uint32_t at0 = key_row + j * KQ4_BLOCK, at1 = at0 + 8 * ROW;
-                            const uint32_t c0 = aq_lds32(at0 + 4 + 4 * t), c1 = aq_lds32(at1 + 4 + 4 * t);
-                            const float d0 = aq_lo(aq_lds32(at0)), d1 = aq_lo(aq_lds32(at1));
-                            const uint32_t a0[4] = {aq_codes<0>(c0), aq_codes<0>(c1), aq_codes<2>(c0), aq_codes<2>(c1)};
-                            const uint32_t a1[4] = {aq_codes<1>(c0), aq_codes<1>(c1), aq_codes<3>(c0), aq_codes<3>(c1)};
+                            uint32_t c[S::XT][2];
+                            float d[S::XT][2];
+#pragma unroll
+                            for (int x = 0; x < S::XT; ++x)
+#pragma unroll
+                                for (int y = 0; y < 2; ++y) {
+                                    const uint8_t *at = key_row + (16 * x + 8 * y) * ROW + j * KQ4_BLOCK;
+                                    c[x][y] = aq_u32(at + 4 + 4 * t);
+                                    d[x][y] = aq_lo(aq_u32(at));
+                                }
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
-                                const uint4 b0 = qf[(nb * KS + 2 * j) * 32 + lane], b1 = qf[(nb * KS + 2 * j + 1) * 32 + lane];
-                                float acc[4];
-                                aq_mma_first(acc, a0, b0.z, b0.w);
-                                aq_mma(acc, a1, b1.z, b1.w);
-                                aq_mma(acc, a0, b0.x, b0.y);
-                                aq_mma(acc, a1, b1.x, b1.y);
-                                s[nb][0] = fmaf(d0, acc[0], s[nb][0]);
-                                s[nb][1] = fmaf(d0, acc[1], s[nb][1]);
-                                s[nb][2] = fmaf(d1, acc[2], s[nb][2]);
-                                s[nb][3] = fmaf(d1, acc[3], s[nb][3]);
+                                const uint4 q0 = qf[(nb * KS + 2 * j) * 32 + lane], q1 = qf[(nb * KS + 2 * j + 1) * 32 + lane];
+                                float acc[S::XT][4];
+#pragma unroll
+                                for (int half = 0; half < 2; ++half)           // of the block
+#pragma unroll
+                                    for (int x = 0; x < S::XT; ++x) {
+                                        const uint4 &q = half ? q1 : q0;
+                                        const uint32_t a[4] = {half ? aq_codes<1>(c[x][0]) : aq_codes<0>(c[x][0]), half ? aq_codes<1>(c[x][1]) : aq_codes<0>(c[x][1]),
+                                                               half ? aq_codes<3>(c[x][0]) : aq_codes<2>(c[x][0]), half ? aq_codes<3>(c[x][1]) : aq_codes<2>(c[x][1])};
+                                        if (half == 0) aq_mma_first(acc[x], a, q.z, q.w);
+                                        else aq_mma(acc[x], a, q.z, q.w);
+                                        aq_mma(acc[x], a, q.x, q.y);
+                                    }
+#pragma unroll
+                                for (int x = 0; x < S::XT; ++x)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) s[x][nb][e] = fmaf(d[x][e >> 1], acc[x][e], s[x][nb][e]);
                             }
                         }
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb)
+                        for (int x = 0; x < S::XT; ++x)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) ex[(nb * 8 + 2 * t + (e & 1)) * AQ_SP + 16 * x + 8 * (e >> 1) + g] = s[nb][e];
+                            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) ex[(nb * 8 + 2 * t + (e & 1)) * S::SP + 16 * x + 8 * (e >> 1) + g] = s[x][nb][e];
                     }
                     __syncwarp();
 
                     // ---- from (keys g, rows 2t) to (row g, keys 2t): weights times 2^12, as two pieces
-                    uint32_t ph[NB][4], pl[NB][4];             // keys 8y + 2t and 8y + 2t + 1
+                    uint32_t ph[NB][2 * S::XT], pl[NB][2 * S::XT];             // keys 8y + 2t and 8y + 2t + 1
                     float alpha[NB];
                     bool moved = b_new != b_run;
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
-                        float2 v[4];
+                        float2 v[2 * S::XT];
                         float top = -INFINITY;
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            v[y] = *reinterpret_cast<const float2 *>(ex + (nb * 8 + g) * AQ_SP + 8 * y + 2 * t);
+                        for (int y = 0; y < 2 * S::XT; ++y) {
+                            v[y] = *reinterpret_cast<const float2 *>(ex + (nb * 8 + g) * S::SP + 8 * y + 2 * t);
                             if (mixed) {
                                 const int key = key0 + 8 * y + 2 * t, from = p.window > 0 ? pos_row[nb] - p.window : -1;
                                 const bool page = there >> (y >> 1) & 1u;
@@ -480,7 +503,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                         m_run[nb] = m_new;
                         float sum = 0.0f;
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
+                        for (int y = 0; y < 2 * S::XT; ++y) {
                             const float2 e = make_float2(aq_exp2(fmaf(v[y].x, fac[nb], 12.0f - ref)), aq_exp2(fmaf(v[y].y, fac[nb], 12.0f - ref)));
                             sum += e.x + e.y;
                             aq_split(e, ph[nb][y], pl[nb][y]);
@@ -499,59 +522,64 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                         }
                         b_run = b_new;
                     }
-                    // ---- values.  The tensor cores cut what they add to an accumulator instead of rounding it: a tile's sums start from zero and are
+                    // ---- values.  The tensor cores cut what they add to an accumulator instead of rounding it: a chunk's sums start from zero and are
                     // added up by the rounding adder, and codes are taken from their middle, so that the terms do not all have one sign.
-#pragma unroll 1
-                    for (int x = 0; x < 2; ++x) {
-                        uint32_t p0[NB], p1[NB], r0_[NB], r1_[NB];
+                    const uint8_t *at_t = reinterpret_cast<const uint8_t *>(tab) + 4 * t;
+                    {
+                        float acc[NB][4];
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) {
-                            p0[nb] = x ? ph[nb][2] : ph[nb][0];
-                            p1[nb] = x ? ph[nb][3] : ph[nb][1];
-                            r0_[nb] = x ? pl[nb][2] : pl[nb][0];
-                            r1_[nb] = x ? pl[nb][3] : pl[nb][1];
-                        }
-                        const uint32_t at_t = tab_d + (16 * x + 2 * t) * 2;
-                        {
-                            const uint32_t at_m = at_t + (G4 + min(g, G4 - 1)) * 64;
-                            const uint32_t hi[4] = {aq_lds32(at_m), 0, aq_lds32(at_m + 16), 0}, lo[4] = {aq_lds32(at_m + G4 * 64), 0, aq_lds32(at_m + G4 * 64 + 16), 0};
+                        for (int x = 0; x < S::XT; ++x) {
+                            const uint8_t *at_m = at_t + 32 * x + (G4 + min(g, G4 - 1)) * 2 * S::CHUNK;
+                            const uint32_t hi[4] = {aq_u32(at_m), 0, aq_u32(at_m + 16), 0}, lo[4] = {aq_u32(at_m + G4 * 2 * S::CHUNK), 0, aq_u32(at_m + G4 * 2 * S::CHUNK + 16), 0};
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
-                                float acc[4];
-                                aq_mma_first(acc, lo, p0[nb], p1[nb]);
-                                aq_mma(acc, hi, r0_[nb], r1_[nb]);
-                                aq_mma(acc, hi, p0[nb], p1[nb]);
-                                om[nb][0] += acc[0];
-                                om[nb][1] += acc[1];
+                                if (x == 0) aq_mma_first(acc[nb], lo, ph[nb][0], ph[nb][1]);
+                                else aq_mma(acc[nb], lo, ph[nb][2 * x], ph[nb][2 * x + 1]);
+                                aq_mma(acc[nb], hi, pl[nb][2 * x], pl[nb][2 * x + 1]);
+                                aq_mma(acc[nb], hi, ph[nb][2 * x], ph[nb][2 * x + 1]);
                             }
                         }
-                        const uint32_t key_row = vb + (16 * x + 2 * t) * ROW + 4 + 2 * g;
 #pragma unroll
-                        for (int j = 0; j < G4; ++j) {
-                            const uint32_t at = key_row + j * KQ4_BLOCK, d0 = aq_lds32(at_t + j * 64), d1 = aq_lds32(at_t + j * 64 + 16);
-                            const uint32_t w0 = __byte_perm(aq_lds16(at), aq_lds16(at + ROW), 0x5410), w1 = __byte_perm(aq_lds16(at + 8 * ROW), aq_lds16(at + 9 * ROW), 0x5410);
-                            const uint32_t a0[4] = {aq_centred<0>(w0), aq_centred<1>(w0), aq_centred<0>(w1), aq_centred<1>(w1)};
-                            const uint32_t a1[4] = {aq_centred<2>(w0), aq_centred<3>(w0), aq_centred<2>(w1), aq_centred<3>(w1)};
+                        for (int nb = 0; nb < NB; ++nb) {
+                            om[nb][0] += acc[nb][0];
+                            om[nb][1] += acc[nb][1];
+                        }
+                    }
+                    const uint8_t *key_row = vb + 2 * t * ROW + 4 + 2 * g;
+#pragma unroll
+                    for (int j = 0; j < G4; ++j) {
+                        float acc[NB][2][4];
+#pragma unroll
+                        for (int x = 0; x < S::XT; ++x) {
+                            uint32_t w[2], d[2];
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                const uint8_t *at = key_row + (16 * x + 8 * y) * ROW + j * KQ4_BLOCK;
+                                w[y] = __byte_perm(aq_u16(at), aq_u16(at + ROW), 0x5410);
+                                d[y] = aq_u32(at_t + j * 2 * S::CHUNK + 32 * x + 16 * y);
+                            }
+                            const uint32_t a0[4] = {aq_centred<0>(w[0]), aq_centred<1>(w[0]), aq_centred<0>(w[1]), aq_centred<1>(w[1])};
+                            const uint32_t a1[4] = {aq_centred<2>(w[0]), aq_centred<3>(w[0]), aq_centred<2>(w[1]), aq_centred<3>(w[1])};
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
                                 uint32_t h0, l0, h1, l1;
-                                aq_weigh(p0[nb], r0_[nb], d0, h0, l0);
-                                aq_weigh(p1[nb], r1_[nb], d1, h1, l1);
-                                float acc[2][4];
-                                aq_mma_first(acc[0], a0, l0, l1);
-                                aq_mma_first(acc[1], a1, l0, l1);
-                                aq_mma(acc[0], a0, h0, h1);
-                                aq_mma(acc[1], a1, h0, h1);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    float *to = &o[nb][j][e >> 1][2 * (e & 1)];
-                                    const float *add = &acc[e >> 1][2 * (e & 1)];
-                                    const float2 sum = aq_add2(make_float2(to[0], to[1]), make_float2(add[0], add[1]));
-                                    to[0] = sum.x;
-                                    to[1] = sum.y;
+                                aq_weigh(ph[nb][2 * x], pl[nb][2 * x], d[0], h0, l0);
+                                aq_weigh(ph[nb][2 * x + 1], pl[nb][2 * x + 1], d[1], h1, l1);
+                                if (x == 0) {
+                                    aq_mma_first(acc[nb][0], a0, l0, l1);
+                                    aq_mma_first(acc[nb][1], a1, l0, l1);
+                                } else {
+                                    aq_mma(acc[nb][0], a0, l0, l1);
+                                    aq_mma(acc[nb][1], a1, l0, l1);
                                 }
+                                aq_mma(acc[nb][0], a0, h0, h1);
+                                aq_mma(acc[nb][1], a1, h0, h1);
                             }
                         }
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] += acc[nb][e >> 2][e & 3];
                     }
                     __syncwarp();                              // the stage, the exchange and the table are free again
                 }
@@ -622,6 +650,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                     for (int e = 0; e < 2; ++e) {
                         const int r = 8 * nb + 2 * t + e, row = r0 + r, tok = row / p.G;
                         const float l = __shfl_sync(0xffffffffu, l_run[nb], 8 * t + 4 * e);
+                        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                         if (row >= p.R) continue;
                         float *to = part ? part + r * (HD + 2) : p.out + ((long long)w.b * p.c.tokens + tok) * p.out_stride + (long long)(w.h * p.G + row - tok * p.G) * HD;
 #pragma unroll
@@ -631,14 +660,14 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
 #pragma unroll
                                 for (int y = 0; y < 2; ++y) {
                                     const float v = o[nb][j][x][2 * y + e];
-                                    to[32 * j + 2 * g + x + 16 * y] = part ? v : (l == 0.0f ? 0.0f : v / l);
+                                    to[32 * j + 2 * g + x + 16 * y] = part ? v : v * inv;
                                 }
                     }
                 }
                 if (!whole && u_first == 0 && lane == 0)        // its last unit is n - u units behind the end of this CTA's part
                     p.desc[me] = make_int4((int)(((last + w.n - w.u) * parts - 1) / total), w.b, w.h, w.rc);
             }
-            if (at < last) aq_next_stretch(p, ROWS, w);
+            if (at < last) aq_next_stretch(p, ROWS, S::UNIT, w);
         }
         if (!ok)                                               // a wait ran out: the copies still on their way end before the CTA does
             for (int s = max(0, i - STAGES); s < i; ++s) mbar_wait_spin(smem_u32(&full[warp][s % STAGES]), (uint32_t)(s / STAGES) & 1u);
@@ -649,7 +678,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
         w.b = x / p.RC;
         w.rc = x - w.b * p.RC;
         w.len = aq_length(p, w.b);
-        aq_range(p, ROWS, w);
+        aq_range(p, ROWS, S::UNIT, w);
         if (w.n) continue;
         const int r0 = w.rc * ROWS, rows = min(p.R, r0 + ROWS) - r0;
         for (int y = tid; y < rows * p.c.Hkv * HD; y += AQ_THREADS) {
@@ -706,7 +735,7 @@ __global__ void __launch_bounds__(32 * AQ_MERGE_WARPS) attn_q4_merge_kernel(cons
 }
 
 template <int HD, int NB>
-static int aq_launch(AqParams p, void *ws, bool joins, cudaStream_t st)
+static int aq_launch(AqParams p, void *ws, cudaStream_t st)
 {
     using S = AqShape<HD, NB>;
     static_assert(S::SMEM <= 227 * 1024, "shared memory");
@@ -717,7 +746,7 @@ static int aq_launch(AqParams p, void *ws, bool joins, cudaStream_t st)
     if (ckb_check_cuda((int)cudaFuncSetAttribute(attn_q4_kernel<HD, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "attention_q4cache")) return CKB_ERR_CUDA;
     attn_q4_kernel<HD, NB><<<N, AQ_THREADS, S::SMEM, st>>>(p);
     const int rc = ckb_check_launch("attention_q4cache");
-    if (rc || !joins) return rc;
+    if (rc || p.c.stride * p.c.page_tokens <= S::UNIT) return rc;      // no stretch has two units
     return launch_pdl("attention_q4cache", attn_q4_merge_kernel<HD>, dim3(N, S::ROWS < p.R ? S::ROWS : p.R), dim3(32 * AQ_MERGE_WARPS), 0, st, p, S::ROWS);
 }
 
@@ -729,18 +758,20 @@ static size_t aq_bytes()
     return N * (sizeof(int4) + 2 * sizeof(float) * S::ROWS * (HD + 2));
 }
 
-// Blocks of 8 query rows that share the codes a CTA unpacks.
-static int aq_blocks(long long rows, int hd) { (void)hd; return rows <= 8 ? 1 : 2; }
+// Blocks of 8 query rows that share the codes a CTA unpacks.  A unit costs 1 : 1.45 : 2.3 with one, two and three (128 channels), so three are worth it only where
+// they hold all the rows: 20 rows of 16 sequences (five drafts, up to 8190 tokens) 119 us with three, 152 us with two and two; 516 rows 55 us in blocks of two, 61 us
+// in blocks of three.
+static int aq_blocks(long long rows, int hd) { return rows <= 8 ? 1 : (rows > 16 && rows <= 24 && hd <= 128 ? 3 : 2); }
 
 }  // namespace ckb
 
 using namespace ckb;
 
-#define AQ_EACH(hd, nb, F)                                \
-    (hd == 64 ? (nb == 1 ? F<64, 1> : F<64, 2>)           \
-     : hd == 96 ? (nb == 1 ? F<96, 1> : F<96, 2>)         \
-     : hd == 128 ? (nb == 1 ? F<128, 1> : F<128, 2>)      \
-     : hd == 192 ? (nb == 1 ? F<192, 1> : F<192, 2>)      \
+#define AQ_EACH(hd, nb, F)                                                          \
+    (hd == 64 ? (nb == 1 ? F<64, 1> : nb == 2 ? F<64, 2> : F<64, 3>)                \
+     : hd == 96 ? (nb == 1 ? F<96, 1> : nb == 2 ? F<96, 2> : F<96, 3>)              \
+     : hd == 128 ? (nb == 1 ? F<128, 1> : nb == 2 ? F<128, 2> : F<128, 3>)          \
+     : hd == 192 ? (nb == 1 ? F<192, 1> : F<192, 2>)                                \
                  : (nb == 1 ? F<256, 1> : F<256, 2>))
 
 extern "C" size_t ckb200_attention_q4cache_workspace_bytes(int batch, int num_tokens, int num_heads, int num_kv_heads, int head_dim)
@@ -788,7 +819,6 @@ extern "C" int ckb200_dev_attention_q4cache(const float *q, long long q_stride, 
     p.page_shift = 3;                                          // 2^(page_shift + 1) >= page_tokens >= 16: exact for positions below 2^31
     while (2u << p.page_shift < (uint32_t)page_tokens) ++p.page_shift;
     p.page_mul = (uint32_t)((((uint64_t)1 << (32 + p.page_shift)) + page_tokens - 1) / page_tokens);
-    const bool joins = (long long)table_stride * page_tokens > AQ_UNIT;           // else no stretch has two units
     const int nb = aq_blocks(p.R, head_dim);
-    return AQ_EACH(head_dim, nb, aq_launch)(p, workspace, joins, ckb_stream(stream));
+    return AQ_EACH(head_dim, nb, aq_launch)(p, workspace, ckb_stream(stream));
 }

@@ -156,6 +156,7 @@ extern "C" int ckb_check_kv_q4(const char *what, const void *k_pages, const void
     if (!ckb200_kv_q4_page_bytes(num_kv_heads, page_tokens, head_dim))
         return ckb_fail(CKB_ERR_SHAPE, "%s: %d kv heads, pages of %d tokens, head size %d (64, 96, 128, 192 or 256; pages of a multiple of 16 tokens)", what, num_kv_heads, page_tokens, head_dim);
     if (num_kv_heads > 1024) return ckb_fail(CKB_ERR_LIMIT, "%s: %d kv heads, at most 1024", what, num_kv_heads);
+    if (ckb200_kv_q4_page_bytes(num_kv_heads, page_tokens, head_dim) > 0x7fffffffu) return ckb_fail(CKB_ERR_LIMIT, "%s: a page of 2 GB or more", what);
     if ((long long)table_stride * page_tokens > 1 << 30 || num_tokens > 1 << 30) return ckb_fail(CKB_ERR_LIMIT, "%s: a sequence may have up to 2^30 tokens", what);
     if ((long long)batch * num_tokens > 0x7fffffffLL) return ckb_fail(CKB_ERR_LIMIT, "%s: %lld rows in one call", what, (long long)batch * num_tokens);
     if (((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) return ckb_fail(CKB_ERR_ALIGN, "%s: pools must be aligned to 16 bytes", what);
