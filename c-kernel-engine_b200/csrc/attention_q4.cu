@@ -17,7 +17,7 @@
 // A query row is a (token, head) of the kv head's group: up to 8 NB rows share every code that is unpacked (NB = 1 for decoding, more for
 // drafts and portions of prompts).
 //
-// Work.  A unit is 128 or 256 keys of one (sequence, kv head, 8 NB rows); the units of all sequences form one line that is cut evenly among the CTAs that
+// Work.  A unit is 128 keys of one (sequence, kv head, 8 NB rows); the units of all sequences form one line that is cut evenly among the CTAs that
 // the GPU holds at once, so long and short sequences load it alike and nothing but the lengths on the device decides.  Each of the four warps takes
 // a quarter of a unit through a ring of its own (untiled bulk copies of 16-key pieces, the largest that never leave a page), without meeting the
 // others until a sequence's stretch ends.  Stretches that lie within one CTA are written out at once, the others as partial results that
@@ -35,7 +35,6 @@
 namespace ckb {
 
 constexpr int AQ_WARPS = 4, AQ_THREADS = 32 * AQ_WARPS;
-constexpr int AQ_MERGE_WARPS = 8;
 
 template <int HD, int NB>
 struct AqShape {
@@ -60,7 +59,7 @@ struct AqParams {
     int H, G, R, RC, window, *err;             // G heads a kv head, R = tokens * G query rows a kv head, RC blocks of them
     float scale;
     uint32_t page_mul, page_shift;             // position / page_tokens = (position * page_mul >> 32) >> page_shift
-    int4 *desc;                                // for each CTA: the stretch that begins in it and ends in a later one {last CTA, b, h, rc}, last CTA < 0: none
+    int2 *desc;                                // [batch][Hkv][RC]: the first and the last CTA of a stretch that several work on; last < 0: one did
     float *part;                               // [2 CTAs][8 NB][HD + 2]: the stretch that began before the CTA, the one that goes on after it
 };
 
@@ -178,6 +177,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
     float *ex = reinterpret_cast<float *>(aq_smem + S::RING + S::QF + S::QS) + warp * NB * 8 * S::SP;
     // for each key of the warp's chunk: d times 2^b, and the middle m + 8 d of the values that a block can say, as two pieces; [G4][keys] halves each
     __half *tab = reinterpret_cast<__half *>(aq_smem + S::RING + S::QF + S::QS + S::EX) + warp * 3 * G4 * S::CHUNK;
+    const int tab_at = (lane & 16) | (lane & 6) << 1 | (lane & 8) >> 2 | (lane & 1);      // keys 2t, 2t + 1, 2t + 8 and 2t + 9 of a tile side by side: one load for a thread
     const int N = gridDim.x, me = blockIdx.x;
 
     if (lane == 0) {
@@ -216,7 +216,16 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
         total += s_sum[w];
     }
     const int parts = (int)min((long long)N, total);                              // every CTA below has at least one unit
-    const long long first = me < parts ? total * me / parts : 0, last = me < parts ? total * (me + 1) / parts : 0;         // its units [first, last)
+    long long first = 0, last = 0;                                                // its units [first, last)
+    if (me < parts) {
+        if (total < 1 << 20) {                                                    // 64-bit divisions take as long as a trip to memory
+            first = (uint32_t)total * (uint32_t)me / (uint32_t)parts;
+            last = (uint32_t)total * (uint32_t)(me + 1) / (uint32_t)parts;
+        } else {
+            first = total * me / parts;
+            last = total * (me + 1) / parts;
+        }
+    }
     if (first < last && mine && before <= first && first < before + mine) {
         long long rest = first - before;
         int b = b0;
@@ -229,8 +238,6 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
         s_rest = rest;
     }
     __syncthreads();
-    if (tid == 0 && p.desc) p.desc[me] = make_int4(-1, 0, 0, 0);
-
     bool ok = true;
     if (first < last) {
         AqWalk w;                                              // the unit being computed
@@ -242,8 +249,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                 aq_range(p, ROWS, S::UNIT, w);
                 per_head += w.n;
             }
-            w.h = (int)(rest / per_head);
-            rest -= per_head * w.h;
+            for (w.h = 0; rest >= per_head; ++w.h) rest -= per_head;
             for (w.rc = 0;; ++w.rc) {
                 aq_range(p, ROWS, S::UNIT, w);
                 if (rest < w.n) break;
@@ -413,9 +419,9 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                         for (int j = 0; j < G4; ++j) {
                             const float mid = fmaf(8.0f, aq_lo(dm[y][j]), aq_hi(dm[y][j]));
                             const __half hi = __float2half_rn(mid), lo = __float2half_rn(mid - __half2float(hi));
-                            tab[j * S::CHUNK + 32 * y + lane] = __low2half(__hmul2_rn(aq_h2(dm[y][j]), d_scale));
-                            tab[(G4 + j) * S::CHUNK + 32 * y + lane] = hi;
-                            tab[(2 * G4 + j) * S::CHUNK + 32 * y + lane] = lo;
+                            tab[j * S::CHUNK + 32 * y + tab_at] = __low2half(__hmul2_rn(aq_h2(dm[y][j]), d_scale));
+                            tab[(G4 + j) * S::CHUNK + 32 * y + tab_at] = hi;
+                            tab[(2 * G4 + j) * S::CHUNK + 32 * y + tab_at] = lo;
                         }
                     // ---- scores of tiles of 16 keys.  A product waits long for the one before it in its sum: those of several tiles and blocks take turns.
                     {
@@ -524,13 +530,14 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                     }
                     // ---- values.  The tensor cores cut what they add to an accumulator instead of rounding it: a chunk's sums start from zero and are
                     // added up by the rounding adder, and codes are taken from their middle, so that the terms do not all have one sign.
-                    const uint8_t *at_t = reinterpret_cast<const uint8_t *>(tab) + 4 * t;
+                    const uint8_t *at_t = reinterpret_cast<const uint8_t *>(tab) + 8 * t;
                     {
                         float acc[NB][4];
 #pragma unroll
                         for (int x = 0; x < S::XT; ++x) {
                             const uint8_t *at_m = at_t + 32 * x + (G4 + min(g, G4 - 1)) * 2 * S::CHUNK;
-                            const uint32_t hi[4] = {aq_u32(at_m), 0, aq_u32(at_m + 16), 0}, lo[4] = {aq_u32(at_m + G4 * 2 * S::CHUNK), 0, aq_u32(at_m + G4 * 2 * S::CHUNK + 16), 0};
+                            const uint2 mh = *reinterpret_cast<const uint2 *>(at_m), ml = *reinterpret_cast<const uint2 *>(at_m + G4 * 2 * S::CHUNK);
+                            const uint32_t hi[4] = {mh.x, 0, mh.y, 0}, lo[4] = {ml.x, 0, ml.y, 0};
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
                                 if (x == 0) aq_mma_first(acc[nb], lo, ph[nb][0], ph[nb][1]);
@@ -551,20 +558,20 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                         float acc[NB][2][4];
 #pragma unroll
                         for (int x = 0; x < S::XT; ++x) {
-                            uint32_t w[2], d[2];
+                            uint32_t w[2];
+                            const uint2 d = *reinterpret_cast<const uint2 *>(at_t + j * 2 * S::CHUNK + 32 * x);
 #pragma unroll
                             for (int y = 0; y < 2; ++y) {
                                 const uint8_t *at = key_row + (16 * x + 8 * y) * ROW + j * KQ4_BLOCK;
                                 w[y] = __byte_perm(aq_u16(at), aq_u16(at + ROW), 0x5410);
-                                d[y] = aq_u32(at_t + j * 2 * S::CHUNK + 32 * x + 16 * y);
                             }
                             const uint32_t a0[4] = {aq_centred<0>(w[0]), aq_centred<1>(w[0]), aq_centred<0>(w[1]), aq_centred<1>(w[1])};
                             const uint32_t a1[4] = {aq_centred<2>(w[0]), aq_centred<3>(w[0]), aq_centred<2>(w[1]), aq_centred<3>(w[1])};
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
                                 uint32_t h0, l0, h1, l1;
-                                aq_weigh(ph[nb][2 * x], pl[nb][2 * x], d[0], h0, l0);
-                                aq_weigh(ph[nb][2 * x + 1], pl[nb][2 * x + 1], d[1], h1, l1);
+                                aq_weigh(ph[nb][2 * x], pl[nb][2 * x], d.x, h0, l0);
+                                aq_weigh(ph[nb][2 * x + 1], pl[nb][2 * x + 1], d.y, h1, l1);
                                 if (x == 0) {
                                     aq_mma_first(acc[nb][0], a0, l0, l1);
                                     aq_mma_first(acc[nb][1], a1, l0, l1);
@@ -664,8 +671,8 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                                 }
                     }
                 }
-                if (!whole && u_first == 0 && lane == 0)        // its last unit is n - u units behind the end of this CTA's part
-                    p.desc[me] = make_int4((int)(((last + w.n - w.u) * parts - 1) / total), w.b, w.h, w.rc);
+                if (u_first == 0 && lane == 0)                  // its last unit is n - u units behind the end of this CTA's part
+                    p.desc[((size_t)w.b * p.c.Hkv + w.h) * p.RC + w.rc] = make_int2(me, whole ? -1 : (int)(((last + w.n - w.u) * parts - 1) / total));
             }
             if (at < last) aq_next_stretch(p, ROWS, S::UNIT, w);
         }
@@ -680,6 +687,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
         w.len = aq_length(p, w.b);
         aq_range(p, ROWS, S::UNIT, w);
         if (w.n) continue;
+        for (int h = tid; h < p.c.Hkv; h += AQ_THREADS) p.desc[((size_t)w.b * p.c.Hkv + h) * p.RC + w.rc] = make_int2(me, -1);
         const int r0 = w.rc * ROWS, rows = min(p.R, r0 + ROWS) - r0;
         for (int y = tid; y < rows * p.c.Hkv * HD; y += AQ_THREADS) {
             const int c = y % HD, hr = y / HD, h = hr / rows, row = r0 + hr - h * rows, tok = row / p.G;
@@ -688,51 +696,69 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
     }
 }
 
-// One CTA per (stretch that spans CTAs, query row): its warps take every eighth partial result.
-template <int HD>
-__global__ void __launch_bounds__(32 * AQ_MERGE_WARPS) attn_q4_merge_kernel(const AqParams p, int nrows)
+// A CTA per (stretch, query row) of those that several CTAs worked on.  A warp has the weights of 32 partial results in its lanes and a channel for each lane, whose
+// parts it adds up LOADS at a time; groups of HD threads take every GROUPS-th 32 results.
+template <int HD, int GROUPS, int LOADS>
+__global__ void __launch_bounds__(GROUPS * HD) attn_q4_merge_kernel(const AqParams p, int nrows)
 {
-    constexpr int PER = HD / 32;
-    __shared__ float acc_s[AQ_MERGE_WARPS][HD], ref_s[AQ_MERGE_WARPS], l_s[AQ_MERGE_WARPS];
+    __shared__ float acc_s[GROUPS][HD], top_s[GROUPS], l_s[GROUPS];
     pdl_wait();
-    const int a = blockIdx.x, r = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int4 d = __ldcg(p.desc + a);
-    const int row = d.w * nrows + r;
-    if (d.x < 0 || row >= p.R) return;
-    const int count = d.x - a + 1;
-    auto slot = [&](int i) { return p.part + ((size_t)(2 * (a + i) + (i == 0)) * nrows + r) * (HD + 2); };
-    float ref = -INFINITY, l = 0.0f, acc[PER];
+    const int r = blockIdx.y, lane = threadIdx.x & 31, grp = threadIdx.x / HD, c = threadIdx.x - grp * HD;
+    for (int x = blockIdx.x; x < p.c.batch * p.c.Hkv * p.RC; x += gridDim.x) {
+        const int2 d = __ldcg(p.desc + x);
+        const int bh = x / p.RC, row = (x - bh * p.RC) * nrows + r;
+        if (d.y < 0 || row >= p.R) continue;
+        const int count = d.y - d.x + 1;
+        const size_t step = (size_t)2 * nrows * (HD + 2);
+        const float *base = p.part + (size_t)(2 * d.x) * nrows * (HD + 2) + r * (HD + 2), *first = base + step / 2;      // the first CTA's is its second
+        float top = -INFINITY, l = 0.0f, acc = 0.0f;
+        for (int i0 = 32 * grp; i0 < count; i0 += 32 * GROUPS) {
+            const int n = min(32, count - i0);
+            const float *mine = i0 + lane == 0 ? first : base + (i0 + min(lane, n - 1)) * step;
+            const float ref = lane < n ? __ldcg(mine + HD) : -INFINITY, part_l = __ldcg(mine + HD + 1);
+            float now = ref;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) acc[j] = 0.0f;
-    for (int i = warp; i < count; i += AQ_MERGE_WARPS) {
-        const float *s = slot(i);
-        const float ref2 = __ldcg(s + HD), l2 = __ldcg(s + HD + 1), both = fmaxf(ref, ref2);
-        const float f = ref == -INFINITY ? 0.0f : aq_exp2(ref - both), f2 = ref2 == -INFINITY ? 0.0f : aq_exp2(ref2 - both);
-        ref = both;
-        l = l * f + l2 * f2;
+            for (int o = 16; o; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+            now = fmaxf(now, top);
+            const float keep = top == -INFINITY ? 0.0f : aq_exp2(top - now), f = ref == -INFINITY ? 0.0f : aq_exp2(ref - now);
+            top = now;
+            float sum = lane < n ? f * part_l : 0.0f;           // 0 x NaN: scores that are no numbers have no maximum, and must be seen
 #pragma unroll
-        for (int j = 0; j < PER; ++j) acc[j] = acc[j] * f + __ldcg(s + 32 * j + lane) * f2;
-    }
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            l = l * keep + sum;
+            acc *= keep;
+            for (int k0 = 0; k0 < n; k0 += LOADS) {
+                float v[LOADS];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) acc_s[warp][32 * j + lane] = acc[j];
-    if (lane == 0) { ref_s[warp] = ref; l_s[warp] = l; }
-    __syncthreads();
-    float top = -INFINITY;
+                for (int u = 0; u < LOADS; ++u) v[u] = k0 + u < n ? __ldcg((i0 + k0 + u ? base + (i0 + k0 + u) * step : first) + c) : 0.0f;
 #pragma unroll
-    for (int w = 0; w < AQ_MERGE_WARPS; ++w) top = fmaxf(top, ref_s[w]);
-    const int tok = row / p.G;
-    float *to = p.out + ((long long)d.y * p.c.tokens + tok) * p.out_stride + (long long)(d.z * p.G + row - tok * p.G) * HD;
-    for (int c = threadIdx.x; c < HD; c += 32 * AQ_MERGE_WARPS) {
-        float sum = 0.0f, v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < AQ_MERGE_WARPS; ++w) {
-            const float f = ref_s[w] == -INFINITY ? 0.0f : aq_exp2(ref_s[w] - top);
-            sum += l_s[w] * f;
-            v += acc_s[w][c] * f;
+                for (int u = 0; u < LOADS; ++u) acc = fmaf(__shfl_sync(0xffffffffu, f, k0 + u), v[u], acc);
+            }
         }
-        to[c] = sum == 0.0f ? 0.0f : v / sum;
+        if (count > 32 && GROUPS > 1) {
+            acc_s[grp][c] = acc;
+            if (c == 0) { top_s[grp] = top; l_s[grp] = l; }
+            __syncthreads();
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) top = fmaxf(top, top_s[g]);
+            acc = l = 0.0f;
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                const float f = top_s[g] == -INFINITY ? 0.0f : aq_exp2(top_s[g] - top);
+                l += l_s[g] * f;
+                acc += acc_s[g][c] * f;
+            }
+            __syncthreads();
+        }
+        if (grp == 0) {
+            const int b = bh / p.c.Hkv, h = bh - b * p.c.Hkv, tok = row / p.G;
+            p.out[((long long)b * p.c.tokens + tok) * p.out_stride + (long long)(h * p.G + row - tok * p.G) * HD + c] = l == 0.0f ? 0.0f : acc / l;
+        }
     }
 }
+
+template <int HD, int NB>
+static size_t aq_desc_bytes(int batch, int Hkv, int R) { return ((size_t)batch * Hkv * ((R + AqShape<HD, NB>::ROWS - 1) / AqShape<HD, NB>::ROWS) * sizeof(int2) + 15) & ~(size_t)15; }
 
 template <int HD, int NB>
 static int aq_launch(AqParams p, void *ws, cudaStream_t st)
@@ -741,21 +767,29 @@ static int aq_launch(AqParams p, void *ws, cudaStream_t st)
     static_assert(S::SMEM <= 227 * 1024, "shared memory");
     const int N = ckb_sm_count() * S::CTAS;
     p.RC = (p.R + S::ROWS - 1) / S::ROWS;
-    p.desc = (int4 *)ws;
-    p.part = (float *)((uint8_t *)ws + sizeof(int4) * N);
-    if (ckb_check_cuda((int)cudaFuncSetAttribute(attn_q4_kernel<HD, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "attention_q4cache")) return CKB_ERR_CUDA;
+    p.desc = (int2 *)ws;
+    p.part = (float *)((uint8_t *)ws + aq_desc_bytes<HD, NB>(p.c.batch, p.c.Hkv, p.R));
+    static bool attr_set = false;
+    if (!attr_set) {
+        if (ckb_check_cuda((int)cudaFuncSetAttribute(attn_q4_kernel<HD, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "attention_q4cache")) return CKB_ERR_CUDA;
+        attr_set = true;
+    }
     attn_q4_kernel<HD, NB><<<N, AQ_THREADS, S::SMEM, st>>>(p);
     const int rc = ckb_check_launch("attention_q4cache");
     if (rc || p.c.stride * p.c.page_tokens <= S::UNIT) return rc;      // no stretch has two units
-    return launch_pdl("attention_q4cache", attn_q4_merge_kernel<HD>, dim3(N, S::ROWS < p.R ? S::ROWS : p.R), dim3(32 * AQ_MERGE_WARPS), 0, st, p, S::ROWS);
+    // Few stretches are in many parts each, and their CTAs few (64 of 32 parts: 6 us, 18 us with a load at a time); many are in two or three (2048 of them: 4 us, 32 us
+    // with the CTAs of the other kind).
+    const long long stretches = (long long)p.c.batch * p.c.Hkv * p.RC;
+    const dim3 grid((unsigned)(stretches < N ? stretches : N), S::ROWS < p.R ? S::ROWS : p.R);
+    if (stretches * 8 < N) return launch_pdl("attention_q4cache", attn_q4_merge_kernel<HD, 512 / HD, 16>, grid, dim3(512 / HD * HD), 0, st, p, S::ROWS);
+    return launch_pdl("attention_q4cache", attn_q4_merge_kernel<HD, 1, 4>, grid, dim3(HD), 0, st, p, S::ROWS);
 }
 
 template <int HD, int NB>
-static size_t aq_bytes()
+static size_t aq_bytes(int batch, int Hkv, int R)
 {
     using S = AqShape<HD, NB>;
-    const size_t N = (size_t)ckb_sm_count() * S::CTAS;
-    return N * (sizeof(int4) + 2 * sizeof(float) * S::ROWS * (HD + 2));
+    return aq_desc_bytes<HD, NB>(batch, Hkv, R) + (size_t)ckb_sm_count() * S::CTAS * 2 * sizeof(float) * S::ROWS * (HD + 2);
 }
 
 // Blocks of 8 query rows that share the codes a CTA unpacks.  A unit costs 1 : 1.45 : 2.3 with one, two and three (128 channels), so three are worth it only where
@@ -776,9 +810,9 @@ using namespace ckb;
 
 extern "C" size_t ckb200_attention_q4cache_workspace_bytes(int batch, int num_tokens, int num_heads, int num_kv_heads, int head_dim)
 {
-    if (batch <= 0 || num_tokens <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads || !ckb200_kv_q4_page_bytes(1, 16, head_dim)) return 0;
+    if (batch <= 0 || num_tokens <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads || (long long)batch * num_tokens * num_heads > 1 << 30 || !ckb200_kv_q4_page_bytes(1, 16, head_dim)) return 0;
     const int nb = aq_blocks((long long)num_tokens * (num_heads / num_kv_heads), head_dim);
-    return AQ_EACH(head_dim, nb, aq_bytes)();
+    return AQ_EACH(head_dim, nb, aq_bytes)(batch, num_kv_heads, num_tokens * (num_heads / num_kv_heads));
 }
 
 extern "C" int ckb200_dev_attention_q4cache(const float *q, long long q_stride, const void *k_pages, const void *v_pages, float *out, long long out_stride, const int *page_table,
@@ -797,11 +831,11 @@ extern "C" int ckb200_dev_attention_q4cache(const float *q, long long q_stride, 
     if (((uintptr_t)q | (uintptr_t)out) & 3) return ckb_fail(CKB_ERR_ALIGN, "%s: rows must be aligned to 4 bytes", what);
     if (rows * num_heads > 1 << 30 || num_heads > 1 << 20) return ckb_fail(CKB_ERR_LIMIT, "%s: %lld query rows in one call", what, rows * num_heads);
     if (!rows) return 0;
-    if (ckb_ensure_init()) return CKB_ERR_NO_DEVICE;
-    if ((rc = ckb_check_device(what))) return rc;
     if (!workspace || workspace_bytes < ckb200_attention_q4cache_workspace_bytes(batch, num_tokens, num_heads, num_kv_heads, head_dim))
         return ckb_fail(CKB_ERR_STATE, "%s: the workspace is too small", what);
     if ((uintptr_t)workspace & 15) return ckb_fail(CKB_ERR_ALIGN, "%s: the workspace must be aligned to 16 bytes", what);
+    if (ckb_ensure_init()) return CKB_ERR_NO_DEVICE;
+    if ((rc = ckb_check_device(what))) return rc;
     AqParams p = {};
     p.q = q;
     p.k = (const uint8_t *)k_pages;
@@ -813,7 +847,7 @@ extern "C" int ckb200_dev_attention_q4cache(const float *q, long long q_stride, 
     p.H = num_heads;
     p.G = num_heads / num_kv_heads;
     p.R = num_tokens * p.G;
-    p.window = sliding_window;
+    p.window = sliding_window < 1 << 30 ? sliding_window : 0;      // no sequence is longer
     p.scale = 1.0f / sqrtf((float)head_dim);
     p.err = ckb_device_error_word();
     p.page_shift = 3;                                          // 2^(page_shift + 1) >= page_tokens >= 16: exact for positions below 2^31

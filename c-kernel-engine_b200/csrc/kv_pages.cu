@@ -56,31 +56,69 @@ __device__ __forceinline__ int kp_before(int v, int *sh, int &total)
     return before;
 }
 
-// Each warp has a stretch of the reference counts: how many of them in [lo, hi) are zero.
-__device__ __forceinline__ int kp_count_free(const int *refs, int lo, int hi)
-{
-    int n = 0;
-    for (int p = lo + (int)(threadIdx.x & 31); p < hi; p += 32 * 8) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (p + 32 * i < hi) n += __ldcg(refs + p + 32 * i) == 0;
-    }
-    return __reduce_add_sync(0xffffffffu, n);
-}
-// Numbers of the pages of [lo, hi) that are free (or in use) into list[at ..), in their order, up to `most` entries of the list in all.
-__device__ __forceinline__ void kp_list(const int *refs, int lo, int hi, bool in_use, int *list, int at, int most)
+// A warp's stretch [lo, hi) of the reference counts, and which of them are zero: up to 256 pages as bits that stay in registers, a longer stretch is read again
+// where it is needed.
+struct KpStretch {
+    int lo, hi;
+    uint32_t free_bits[8];
+};
+__device__ __forceinline__ int kp_count_free(const int *refs, KpStretch &s)
 {
     const int lane = threadIdx.x & 31;
-    for (int p0 = lo; p0 < hi && at < most; p0 += 32) {
-        const int p = p0 + lane;
-        const bool is = p < hi && (__ldcg(refs + p) != 0) == in_use;
-        const uint32_t mask = __ballot_sync(0xffffffffu, is);
-        const int to = at + __popc(mask & ((1u << lane) - 1u));
-        if (is && to < most) list[to] = p;
-        at += __popc(mask);
+    int n = 0;
+    for (int p0 = s.lo; p0 < s.hi; p0 += 32 * 8) {
+        int ref[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ref[i] = p0 + 32 * i + lane < s.hi ? __ldcg(refs + p0 + 32 * i + lane) : 1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            s.free_bits[i] = __ballot_sync(0xffffffffu, ref[i] == 0);
+            n += __popc(s.free_bits[i]);
+        }
+    }
+    return n;
+}
+// Numbers of the pages of [lo, hi), a part of the stretch, that are free (or in use) into list[at ..), in their order, up to `most` entries of the list in all.
+__device__ __forceinline__ void kp_list(const int *refs, const KpStretch &s, int lo, int hi, bool in_use, int *list, int at, int most)
+{
+    const int lane = threadIdx.x & 31;
+    const bool kept = s.hi - s.lo <= 32 * 8;
+    for (int p0 = s.lo; p0 < hi && at < most; p0 += 32 * 8) {
+        uint32_t bits[8];
+        if (kept) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) bits[i] = s.free_bits[i];
+        } else {
+            int ref[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ref[i] = p0 + 32 * i + lane < hi ? __ldcg(refs + p0 + 32 * i + lane) : 1;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) bits[i] = __ballot_sync(0xffffffffu, ref[i] == 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int p = p0 + 32 * i + lane;
+            const bool is = p >= lo && p < hi && ((bits[i] >> lane & 1u) == 0) == in_use;
+            const uint32_t mask = __ballot_sync(0xffffffffu, is);
+            const int to = at + __popc(mask & ((1u << lane) - 1u));
+            if (is && to < most) list[to] = p;
+            at += __popc(mask);
+        }
     }
 }
-__device__ __forceinline__ int kp_span(int pages) { return (pages + KP_WARPS - 1) / KP_WARPS; }
+// how many of [s.lo, cut) are zero
+__device__ __forceinline__ int kp_free_below(const int *refs, const KpStretch &s, int cut)
+{
+    const int lane = threadIdx.x & 31;
+    int n = 0;
+    for (int p = s.lo + lane; p < cut; p += 32) n += __ldcg(refs + p) == 0;
+    return __reduce_add_sync(0xffffffffu, n);
+}
+__device__ __forceinline__ KpStretch kp_stretch(int pages)
+{
+    const int span = (pages + KP_WARPS - 1) / KP_WARPS, lo = min(pages, (int)(threadIdx.x >> 5) * span);
+    return {lo, min(pages, lo + span), {}};
+}
 
 // ---------------------------------------------------------------- the bytes
 
@@ -196,8 +234,8 @@ __global__ void __launch_bounds__(KP_THREADS) kv_pages_resize_kernel(KvTables t,
     if (threadIdx.x == 0) s_copies = total_copies;
     __syncthreads();
     if (total > 0) {
-        const int span = kp_span(t.pages), lo = min(t.pages, warp * span), hi = min(t.pages, lo + span);
-        const int n = kp_count_free(t.refs, lo, hi);
+        KpStretch pages = kp_stretch(t.pages);
+        const int n = kp_count_free(t.refs, pages);
         int have_free;
         const int before = kp_before(lane == 0 ? n : 0, sh, have_free);
         if (have_free < total) {                                // one by one: who finds no room leaves its claim to those behind
@@ -230,7 +268,7 @@ __global__ void __launch_bounds__(KP_THREADS) kv_pages_resize_kernel(KvTables t,
         }
         // the free pages themselves; a page whose count the loop above took down was shared before and still has a holder
         const int base = __shfl_sync(0xffffffffu, before, 0);
-        kp_list(t.refs, lo, hi, false, list, base, min(total, have_free));
+        kp_list(t.refs, pages, pages.lo, pages.hi, false, list, base, min(total, have_free));
         __syncthreads();
     }
     for (int b = warp; b < B; b += KP_WARPS) {
@@ -303,18 +341,18 @@ __global__ void __launch_bounds__(KP_THREADS) kv_pages_plan_kernel(KvTables t, i
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int *src = ws + 4, *dst = src + t.pages, *place = dst + t.pages;
     pdl_trigger();
-    const int span = kp_span(t.pages), lo = min(t.pages, warp * span), hi = min(t.pages, lo + span);
-    const int n = kp_count_free(t.refs, lo, hi);
+    KpStretch pages = kp_stretch(t.pages);
+    const int lo = pages.lo, hi = pages.hi, n = kp_count_free(t.refs, pages);
     int free_all;
     kp_before(lane == 0 ? n : 0, sh, free_all);
     const int live = t.pages - free_all, cut = min(hi, max(lo, live));
     // free ones below `live`, used ones from there on: as many of the one kind as of the other
-    const int holes = cut == hi ? n : (cut == lo ? 0 : kp_count_free(t.refs, lo, cut)), movers = (hi - cut) - (n - holes);
+    const int holes = cut == hi ? n : (cut == lo ? 0 : kp_free_below(t.refs, pages, cut)), movers = (hi - cut) - (n - holes);
     int count, same;
     const int hole0 = __shfl_sync(0xffffffffu, kp_before(lane == 0 ? holes : 0, sh, count), 0);
     const int mover0 = __shfl_sync(0xffffffffu, kp_before(lane == 0 ? movers : 0, sh, same), 0);
-    kp_list(t.refs, lo, cut, false, dst, hole0, count);
-    kp_list(t.refs, cut, hi, true, src, mover0, count);
+    kp_list(t.refs, pages, lo, cut, false, dst, hole0, count);
+    kp_list(t.refs, pages, cut, hi, true, src, mover0, count);
     for (int p = cut + lane; p < hi; p += 32) place[p] = -1;
     __syncthreads();
     for (int i = threadIdx.x; i < count; i += KP_THREADS) {
@@ -362,7 +400,12 @@ static int check_pool(const char *what, const void *pages, int planes, long long
     if ((uintptr_t)pages & 15) return ckb_fail(CKB_ERR_ALIGN, "%s: pools must be aligned to 16 bytes", what);
     return 0;
 }
-static int copy_grid() { return ckb_sm_count() * (2048 / KC_THREADS); }
+// CTAs for up to `pairs` pages of every plane: no more than can be resident, no more than have a piece to copy
+static unsigned copy_grid(long long pairs, int planes, long long page_bytes)
+{
+    const long long most = (long long)ckb_sm_count() * (2048 / KC_THREADS), pieces = pairs * planes * ((page_bytes + 512 * KC_UNROLL - 1) / (512 * KC_UNROLL)), n = (pieces + KC_THREADS / 32 - 1) / (KC_THREADS / 32);
+    return (unsigned)(n < 1 ? 1 : (n < most ? n : most));
+}
 
 extern "C" int ckb200_dev_kv_pages_copy(void *pages, int planes, long long plane_stride, long long page_bytes, const int *src, const int *dst, int count, int num_pages, void *stream)
 {
@@ -376,7 +419,7 @@ extern "C" int ckb200_dev_kv_pages_copy(void *pages, int planes, long long plane
     if (ckb_ensure_init()) return CKB_ERR_NO_DEVICE;
     if ((rc = ckb_check_device(what))) return rc;
     const KvPool pool = {(uint8_t *)pages, plane_stride, page_bytes, planes, num_pages};
-    kv_pages_copy_kernel<<<copy_grid(), KC_THREADS, 0, ckb_stream(stream)>>>(pool, src, dst, NULL, count, KvTables{}, NULL);
+    kv_pages_copy_kernel<<<copy_grid(count, planes, page_bytes), KC_THREADS, 0, ckb_stream(stream)>>>(pool, src, dst, NULL, count, KvTables{}, NULL);
     return ckb_check_launch(what);
 }
 
@@ -400,7 +443,7 @@ extern "C" int ckb200_dev_kv_pages_resize(int *page_table, int table_stride, int
     kv_pages_resize_kernel<<<1, KP_THREADS, smem, st>>>(t, new_lens, status, ws);
     if ((rc = ckb_check_launch(what)) || !planes) return rc;
     const KvPool pool = {(uint8_t *)pages, plane_stride, page_bytes, planes, num_pages};
-    return launch_pdl(what, kv_pages_copy_kernel, dim3(copy_grid()), dim3(KC_THREADS), 0, st, pool, (const int *)(ws + 4), (const int *)(ws + 4 + batch), (const int *)ws, 0, KvTables{},
+    return launch_pdl(what, kv_pages_copy_kernel, dim3(copy_grid(batch, planes, page_bytes)), dim3(KC_THREADS), 0, st, pool, (const int *)(ws + 4), (const int *)(ws + 4 + batch), (const int *)ws, 0, KvTables{},
                       (const int *)NULL);
 }
 
@@ -438,6 +481,7 @@ extern "C" int ckb200_dev_kv_pages_compact(int *page_table, int table_stride, co
     kv_pages_plan_kernel<<<1, KP_THREADS, 0, st>>>(t, live, ws);
     if ((rc = ckb_check_launch(what))) return rc;
     const KvPool pool = {(uint8_t *)pages, plane_stride, page_bytes, planes, num_pages};
-    return launch_pdl(what, kv_pages_copy_kernel, dim3(copy_grid()), dim3(KC_THREADS), 0, st, pool, (const int *)(ws + 4), (const int *)(ws + 4 + num_pages), (const int *)ws, 0, t,
+    const unsigned pieces = copy_grid(num_pages / 2, planes, page_bytes), grid = pieces > (unsigned)batch ? pieces : (unsigned)batch;      // each also takes rows of the table
+    return launch_pdl(what, kv_pages_copy_kernel, dim3(grid), dim3(KC_THREADS), 0, st, pool, (const int *)(ws + 4), (const int *)(ws + 4 + num_pages), (const int *)ws, 0, t,
                       (const int *)(ws + 4 + 2 * (size_t)num_pages));
 }

@@ -1,8 +1,7 @@
 // Rows of a paged 4-bit KV cache: quantised into it, and read back.
 //
-// A block of 32 values is the work of eight lanes, four values (16 bytes) each, for K and for V: the lanes find the block's least and
-// largest value by shuffles; a lane's four codes make four bytes' nibbles, and since byte j holds values j and j + 16, lane l and lane l + 4
-// share them: one more shuffle, and lanes 0..3 write the 16 code bytes, lane 4 the (d, m) pair.  A warp's writes are consecutive.
+// A block of 32 values is the work of four lanes, for K and for V: lane l has values 4l .. 4l + 3 and 16 + 4l .. 16 + 4l + 3, which are the nibbles of code bytes
+// 4l .. 4l + 3, so that only the block's least and largest value cross lanes (two shuffles each).  A warp's loads and stores are of whole 32-byte sectors.
 // Bound by HBM, 4.625 bytes a value either way: reading 4 bytes when storing, writing them when loading.
 #include <cuda_fp16.h>
 #include <float.h>
@@ -18,34 +17,36 @@ namespace ckb {
 
 constexpr int KR_THREADS = 256;
 
-// lanes 0..7 of a group hold values 4l .. 4l + 3 of a block; the word that lane l < 4 (codes 4l ..) or lane 4 (d, m) writes
-__device__ __forceinline__ uint32_t kr_quantise(const float4 &x, int l)
+// the word of codes of lane l of the four, and the block's (d, m)
+__device__ __forceinline__ uint32_t kr_quantise(const float4 &x, const float4 &y, uint32_t &dm)
 {
-    float lo = fminf(fminf(x.x, x.y), fminf(x.z, x.w)), hi = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
-    // minimum and maximum pass over NaN: it is looked for by itself
-    int bad = !(fabsf(x.x) <= FLT_MAX && fabsf(x.y) <= FLT_MAX && fabsf(x.z) <= FLT_MAX && fabsf(x.w) <= FLT_MAX);
+    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    float lo = v[0], hi = v[0];
+    bool fine = true;
 #pragma unroll
-    for (int o = 4; o; o >>= 1) {
+    for (int i = 0; i < 8; ++i) {
+        lo = fminf(lo, v[i]);
+        hi = fmaxf(hi, v[i]);
+        fine &= fabsf(v[i]) <= FLT_MAX;                        // minimum and maximum pass over NaN: it is looked for by itself
+    }
+    if (!fine) hi = INFINITY;                                  // no code can say the block: d becomes infinite, below
+#pragma unroll
+    for (int o = 2; o; o >>= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        bad |= __shfl_xor_sync(0xffffffffu, bad, o);
     }
     // the two roundings to fp16 that the format asks for; codes are then taken against the rounded pair, so that each is the nearest that the block can say
     const __half mh = __float2half_rn(lo), dh = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f));
-    const float m = __half2float(mh), d = __half2float(dh);
-    bad |= !(fabsf(m) <= 65504.0f && d <= 65504.0f);
-    const float inv = d > 0.0f ? __frcp_rn(d) : 0.0f;
-    const float v[4] = {x.x, x.y, x.z, x.w};
+    const float m = __half2float(mh), d = __half2float(dh), inv = d > 0.0f ? __frcp_rn(d) : 0.0f;
     uint32_t codes = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
         const float t = floorf(__fadd_rn(__fmul_rn(__fsub_rn(v[i], m), inv), 0.5f));
-        codes |= (uint32_t)fminf(fmaxf(t, 0.0f), 15.0f) << (8 * i);
+        codes |= (uint32_t)fminf(fmaxf(t, 0.0f), 15.0f) << (8 * (i & 3) + 4 * (i >> 2));
     }
-    if (bad) codes = 0;
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, codes, 4);
-    const uint32_t dm = bad ? 0x7fff7fffu : ((uint32_t)__half_as_ushort(mh) << 16 | __half_as_ushort(dh));
-    return l < 4 ? codes | other << 4 : dm;
+    const bool good = fabsf(m) <= 65504.0f && d <= 65504.0f;
+    dm = good ? (uint32_t)__half_as_ushort(mh) << 16 | __half_as_ushort(dh) : 0x7fff7fffu;
+    return good ? codes : 0;
 }
 
 template <bool VEC>
@@ -67,66 +68,87 @@ __device__ __forceinline__ void kr_store4(float *p, const float4 &v)
     }
 }
 
-// group (8 lanes) -> (row, block of the row); where the row lies in the pools, -1: nowhere
-__device__ __forceinline__ bool kr_where(const KvQ4 &c, long long rows, long long &row, int &block, long long &at)
+// n / d and n % d by a multiplication, n below 2^31
+struct KrDivide {
+    uint32_t d, mul, shift;
+    __device__ __forceinline__ int operator()(uint32_t n) const { return (int)(d == 1 ? n : __umulhi(n, mul) >> shift); }
+};
+struct KrRows {
+    KvQ4 c;
+    long long k_stride, v_stride;
+    uint32_t groups;                           // blocks of 32 values of all rows
+    KrDivide by_items, by_tokens, by_nb, by_page;
+};
+
+// where block `grp` of all rows lies: its row's number, its place in the row, and its place in the pools in bytes (-1: nowhere)
+__device__ __forceinline__ void kr_where(const KrRows &p, uint32_t grp, int &row, int &block, long long &at)
 {
-    const long long grp = ((long long)blockIdx.x * KR_THREADS + threadIdx.x) >> 3;
-    const int items = c.Hkv * c.nb;
-    row = grp / items;
-    block = (int)(grp - row * items);
+    row = p.by_items(grp);
+    block = (int)(grp - (uint32_t)row * p.by_items.d);
+    const int b = p.by_tokens(row), t = row - b * p.c.tokens, head = p.by_nb(block);
+    const int pos = kv_len(__ldg(p.c.lens + b), p.c.stride, p.c.page_tokens) - p.c.tokens + t;
     at = -1;
-    if (row >= rows) return false;
-    const int b = (int)(row / c.tokens), t = (int)(row - (long long)b * c.tokens);
-    const int pos = kv_len(__ldg(c.lens + b), c.stride, c.page_tokens) - c.tokens + t;
-    const int page = kv_page(c.table + (size_t)b * c.stride, c.stride, c.pages, c.page_tokens, pos);
-    const int head = block / c.nb;
-    if (page >= 0) at = (long long)kv_row(page, head, pos % c.page_tokens, c.Hkv, c.page_tokens, c.nb) + (block - head * c.nb) * KQ4_BLOCK;
-    return true;
+    if (pos < 0) return;
+    const int column = p.by_page(pos), page = kv_entry(__ldg(p.c.table + (size_t)b * p.c.stride + column), p.c.pages);      // pos is below the length: the column exists
+    if (page >= 0) at = (long long)kv_row(page, head, pos - column * p.c.page_tokens, p.c.Hkv, p.c.page_tokens, p.c.nb) + (block - head * p.c.nb) * KQ4_BLOCK;
 }
 
 template <bool VEC>
-__global__ void __launch_bounds__(KR_THREADS) kv_store_q4_kernel(uint8_t *__restrict__ kp, uint8_t *__restrict__ vp, const float *__restrict__ k, const float *__restrict__ v,
-                                                                 long long ks, long long vs, KvQ4 c, long long rows)
+__global__ void __launch_bounds__(KR_THREADS) kv_store_q4_kernel(uint8_t *__restrict__ kp, uint8_t *__restrict__ vp, const float *__restrict__ k, const float *__restrict__ v, KrRows p)
 {
-    long long row, at;
-    int block;
-    const int l = threadIdx.x & 7;
-    const bool in = kr_where(c, rows, row, block, at);
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-    if (in) {
-        a = kr_load4<VEC>(k + row * ks + block * 32 + 4 * l);
-        b = kr_load4<VEC>(v + row * vs + block * 32 + 4 * l);
+    const int l = threadIdx.x & 3;
+    const uint32_t grp = blockIdx.x * (KR_THREADS / 4) + (threadIdx.x >> 2);
+    float4 a[2], b[2];
+    a[0] = a[1] = b[0] = b[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    long long at = -1;
+    if (grp < p.groups) {
+        int row, block;
+        kr_where(p, grp, row, block, at);
+        const float *x = k + row * p.k_stride + block * 32 + 4 * l, *y = v + row * p.v_stride + block * 32 + 4 * l;
+        a[0] = kr_load4<VEC>(x);
+        a[1] = kr_load4<VEC>(x + 16);
+        b[0] = kr_load4<VEC>(y);
+        b[1] = kr_load4<VEC>(y + 16);
     }
-    const uint32_t wk = kr_quantise(a, l), wv = kr_quantise(b, l);
-    if (at < 0 || l > 4) return;
-    const size_t to = (size_t)at + (l < 4 ? 4 + 4 * l : 0);
-    *reinterpret_cast<uint32_t *>(kp + to) = wk;
-    *reinterpret_cast<uint32_t *>(vp + to) = wv;
+    uint32_t dmk, dmv;
+    const uint32_t wk = kr_quantise(a[0], a[1], dmk), wv = kr_quantise(b[0], b[1], dmv);
+    if (at < 0) return;
+    uint32_t *x = reinterpret_cast<uint32_t *>(kp + at), *y = reinterpret_cast<uint32_t *>(vp + at);
+    x[1 + l] = wk;
+    y[1 + l] = wv;
+    if (l == 0) x[0] = dmk;
+    if (l == 1) y[0] = dmv;
 }
 
-__device__ __forceinline__ float4 kr_values(const uint8_t *p, int l)
+__device__ __forceinline__ float4 kr_values(uint32_t dm, uint32_t w)       // of the low nibbles of w
 {
-    const uint32_t dm = __ldg(reinterpret_cast<const uint32_t *>(p)), w = __ldg(reinterpret_cast<const uint32_t *>(p + 4 + 4 * (l & 3))) >> (l < 4 ? 0 : 4);
     const float d = half_bits_to_float(dm & 0xffffu), m = half_bits_to_float(dm >> 16);
     return make_float4(__fadd_rn(__fmul_rn(d, (float)(w & 15u)), m), __fadd_rn(__fmul_rn(d, (float)(w >> 8 & 15u)), m), __fadd_rn(__fmul_rn(d, (float)(w >> 16 & 15u)), m),
                        __fadd_rn(__fmul_rn(d, (float)(w >> 24 & 15u)), m));
 }
 
 template <bool VEC>
-__global__ void __launch_bounds__(KR_THREADS) kv_load_q4_kernel(float *__restrict__ k, float *__restrict__ v, long long ks, long long vs, const uint8_t *__restrict__ kp,
-                                                                const uint8_t *__restrict__ vp, KvQ4 c, long long rows)
+__global__ void __launch_bounds__(KR_THREADS) kv_load_q4_kernel(float *__restrict__ k, float *__restrict__ v, const uint8_t *__restrict__ kp, const uint8_t *__restrict__ vp, KrRows p)
 {
-    long long row, at;
-    int block;
-    const int l = threadIdx.x & 7;
-    if (!kr_where(c, rows, row, block, at)) return;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    const int l = threadIdx.x & 3;
+    const uint32_t grp = blockIdx.x * (KR_THREADS / 4) + (threadIdx.x >> 2);
+    if (grp >= p.groups) return;
+    long long at;
+    int row, block;
+    kr_where(p, grp, row, block, at);
+    uint32_t dmk = 0, dmv = 0, wk = 0, wv = 0;
     if (at >= 0) {
-        a = kr_values(kp + at, l);
-        b = kr_values(vp + at, l);
+        const uint32_t *x = reinterpret_cast<const uint32_t *>(kp + at), *y = reinterpret_cast<const uint32_t *>(vp + at);
+        dmk = __ldg(x);
+        wk = __ldg(x + 1 + l);
+        dmv = __ldg(y);
+        wv = __ldg(y + 1 + l);
     }
-    kr_store4<VEC>(k + row * ks + block * 32 + 4 * l, a);
-    kr_store4<VEC>(v + row * vs + block * 32 + 4 * l, b);
+    float *x = k + row * p.k_stride + block * 32 + 4 * l, *y = v + row * p.v_stride + block * 32 + 4 * l;
+    kr_store4<VEC>(x, kr_values(dmk, wk));
+    kr_store4<VEC>(x + 16, kr_values(dmk, wk >> 4));
+    kr_store4<VEC>(y, kr_values(dmv, wv));
+    kr_store4<VEC>(y + 16, kr_values(dmv, wv >> 4));
 }
 
 }  // namespace ckb
@@ -174,11 +196,22 @@ static int check_rows(const char *what, const float *k, const float *v, long lon
 
 static bool rows_vectors(const float *k, const float *v, long long ks, long long vs) { return !(((uintptr_t)k | (uintptr_t)v) & 15) && !((ks | vs) & 3); }
 
-static int rows_grid(const char *what, const KvQ4 &c, long long rows, unsigned *grid)
+static KrDivide kr_divide(uint32_t d)
 {
-    const long long n = (rows * c.Hkv * c.nb * 8 + KR_THREADS - 1) / KR_THREADS;
-    if (n > 0x7fffffffLL) return ckb_fail(CKB_ERR_LIMIT, "%s: %lld rows in one call", what, rows);
-    *grid = (unsigned)n;
+    KrDivide x = {d, 0, 0};
+    if (d > 1) {
+        while (2u << x.shift < d) ++x.shift;                   // 2^shift < d <= 2^(shift + 1)
+        x.mul = (uint32_t)((((uint64_t)1 << (32 + x.shift)) + d - 1) / d);
+    }
+    return x;
+}
+// 0 and the launch's parameters, or an error
+static int rows_params(const char *what, const KvQ4 &c, long long rows, long long ks, long long vs, KrRows *p, unsigned *grid)
+{
+    const long long groups = rows * c.Hkv * c.nb;
+    if (groups > 0x7fffffffLL) return ckb_fail(CKB_ERR_LIMIT, "%s: %lld rows in one call", what, rows);
+    *p = {c, ks, vs, (uint32_t)groups, kr_divide((uint32_t)(c.Hkv * c.nb)), kr_divide((uint32_t)(c.tokens > 0 ? c.tokens : 1)), kr_divide((uint32_t)c.nb), kr_divide((uint32_t)c.page_tokens)};
+    *grid = (unsigned)((groups + KR_THREADS / 4 - 1) / (KR_THREADS / 4));
     return 0;
 }
 
@@ -191,15 +224,16 @@ extern "C" int ckb200_dev_kv_cache_store_q4(void *k_pages, void *v_pages, const 
     const long long rows = (long long)batch * num_tokens;
     if (rc || (rc = check_rows(what, k, v, k_stride, v_stride, rows > 1 ? 2 : 1, num_kv_heads * head_dim))) return rc;
     const KvQ4 c = {page_table, kv_lens, table_stride, batch, num_tokens, num_pages, page_tokens, num_kv_heads, head_dim / 32};
+    KrRows p;
     unsigned grid;
-    if ((rc = rows_grid(what, c, rows, &grid))) return rc;
+    if ((rc = rows_params(what, c, rows, k_stride, v_stride, &p, &grid))) return rc;
     if (!rows) return 0;
     if (ckb_ensure_init()) return CKB_ERR_NO_DEVICE;
     if ((rc = ckb_check_device(what))) return rc;
     if (rows_vectors(k, v, k_stride, v_stride))
-        kv_store_q4_kernel<true><<<grid, KR_THREADS, 0, ckb_stream(stream)>>>((uint8_t *)k_pages, (uint8_t *)v_pages, k, v, k_stride, v_stride, c, rows);
+        kv_store_q4_kernel<true><<<grid, KR_THREADS, 0, ckb_stream(stream)>>>((uint8_t *)k_pages, (uint8_t *)v_pages, k, v, p);
     else
-        kv_store_q4_kernel<false><<<grid, KR_THREADS, 0, ckb_stream(stream)>>>((uint8_t *)k_pages, (uint8_t *)v_pages, k, v, k_stride, v_stride, c, rows);
+        kv_store_q4_kernel<false><<<grid, KR_THREADS, 0, ckb_stream(stream)>>>((uint8_t *)k_pages, (uint8_t *)v_pages, k, v, p);
     return ckb_check_launch(what);
 }
 
@@ -212,14 +246,15 @@ extern "C" int ckb200_dev_kv_cache_load_q4(float *k, float *v, long long k_strid
     const long long rows = (long long)batch * num_tokens;
     if (rc || (rc = check_rows(what, k, v, k_stride, v_stride, rows > 1 ? 2 : 1, num_kv_heads * head_dim))) return rc;
     const KvQ4 c = {page_table, kv_lens, table_stride, batch, num_tokens, num_pages, page_tokens, num_kv_heads, head_dim / 32};
+    KrRows p;
     unsigned grid;
-    if ((rc = rows_grid(what, c, rows, &grid))) return rc;
+    if ((rc = rows_params(what, c, rows, k_stride, v_stride, &p, &grid))) return rc;
     if (!rows) return 0;
     if (ckb_ensure_init()) return CKB_ERR_NO_DEVICE;
     if ((rc = ckb_check_device(what))) return rc;
     if (rows_vectors(k, v, k_stride, v_stride))
-        kv_load_q4_kernel<true><<<grid, KR_THREADS, 0, ckb_stream(stream)>>>(k, v, k_stride, v_stride, (const uint8_t *)k_pages, (const uint8_t *)v_pages, c, rows);
+        kv_load_q4_kernel<true><<<grid, KR_THREADS, 0, ckb_stream(stream)>>>(k, v, (const uint8_t *)k_pages, (const uint8_t *)v_pages, p);
     else
-        kv_load_q4_kernel<false><<<grid, KR_THREADS, 0, ckb_stream(stream)>>>(k, v, k_stride, v_stride, (const uint8_t *)k_pages, (const uint8_t *)v_pages, c, rows);
+        kv_load_q4_kernel<false><<<grid, KR_THREADS, 0, ckb_stream(stream)>>>(k, v, (const uint8_t *)k_pages, (const uint8_t *)v_pages, p);
     return ckb_check_launch(what);
 }

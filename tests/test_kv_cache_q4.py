@@ -40,7 +40,8 @@ COMMON = [(dict(k_pages=None), STATE), (dict(v_pages=None), STATE), (dict(page_t
           (dict(head_dim=32), SHAPE), (dict(k_pages=264), ALIGN), (dict(v_pages=257), ALIGN), (dict(kv_lens=258), ALIGN), (dict(table_stride=1 << 27), LIMIT), (dict(num_kv_heads=1025), LIMIT)]
 ROWS = [(dict(k=None), STATE), (dict(v=None), STATE), (dict(k=257), ALIGN), (dict(k_stride=255), SHAPE), (dict(v_stride=-256), SHAPE), (dict(batch=1 << 30, num_tokens=1 << 30), LIMIT)]
 OWN = [(dict(q=None), STATE), (dict(out=None), STATE), (dict(q=258), ALIGN), (dict(num_heads=0), SHAPE), (dict(num_heads=5), SHAPE), (dict(sliding_window=-1), SHAPE), (dict(q_stride=511), SHAPE),
-       (dict(out_stride=0), SHAPE), (dict(batch=1 << 20, num_tokens=1 << 20), LIMIT)]
+       (dict(out_stride=0), SHAPE), (dict(batch=1 << 20, num_tokens=1 << 20), LIMIT), (dict(batch=1 << 15, num_tokens=1 << 15), LIMIT), (dict(workspace=None), STATE),
+       (dict(workspace_bytes=1000), STATE), (dict(workspace=264), ALIGN)]
 REFUSED = [(name, change, code) for name in CALLS for change, code in COMMON + (OWN if "attention" in name else ROWS)]
 
 
@@ -239,6 +240,9 @@ ATTENTION_CASES = [
     (8, 1, 128, 64, [300, 64, 65], 1, 0), (32, 8, 128, 64, [513], 1, 0), (9, 1, 128, 32, [127, 128, 129], 1, 0), (24, 2, 64, 16, [250, 3], 1, 0), (2, 1, 192, 16, [90, 31], 1, 0),
     (10, 2, 256, 16, [100, 255, 1], 1, 0), (40, 1, 64, 16, [150], 1, 0), (4, 2, 128, 16, [400, 90, 20], 1, 33), (4, 2, 64, 128, [1000], 1, 1), (3, 1, 64, 16, [66], 1, 1000),
     (8, 2, 128, 64, [130, 5, 0, 64], 5, 0), (12, 4, 64, 16, [40, 39, 7, 8], 8, 0), (4, 4, 96, 16, [64], 64, 0), (8, 1, 128, 32, [200, 30], 33, 0), (6, 2, 256, 16, [70], 9, 0), (5, 5, 192, 32, [80], 21, 17),
+    # more parts of one sequence than a warp has lanes, sequences by the dozen, more of them than threads in a block
+    (3, 1, 64, 16, [9000], 1, 0), (2, 1, 128, 32, [5000, 17], 2, 0), (4, 2, 64, 16, [(37 * i) % 411 for i in range(90)], 1, 0), (1, 1, 64, 16, [i % 19 for i in range(700)], 1, 0),
+    (5, 1, 256, 16, [4500], 1, 2 ** 31 - 1),
     (16, 2, 64, 16, [300, 90], 17, 40), (2, 2, 128, 16, [130], 130, 16), (4, 1, 128, 16, [3000, 5, 2049], 1, 0), (8, 8, 64, 256, [2500], 3, 2048), (4, 1, 128, 64, [50], 100, 0),
 ]
 
@@ -365,6 +369,28 @@ def test_pool_beyond_32_bits(gpu):
         want = host.values(pool[small.table[1]].transpose(1, 0, 2, 3).reshape(hkv, 256, -1), np.float32).transpose(1, 0, 2).reshape(256, -1)
         assert np.array_equal(back[i, 256:].cpu().numpy(), want)
     near(out.cpu().numpy(), *small.attention(q, 1, hkv))
+
+
+@pytest.mark.gpu
+def test_sequences_of_millions_of_tokens(gpu):
+    """2^24 tokens whose table names one page over and over (and 16 more in a second sequence): the result is that of the page's tokens, whatever the number of units,
+    which passes 2^20 here, and of the partial results that are joined."""
+    rng = np.random.default_rng(17)
+    hkv, hd, columns = 8, 64, 1 << 20
+    small = random_cache(rng, hkv, hd, 16, [16, 16], spare=0)
+    dev = Device(gpu, small)
+    table = np.full((2, columns), small.table[0, 0], dtype=np.int32)
+    table[1, 0] = small.table[1, 0]
+    big, lens = up(table), up(np.array([columns * 16, 16], dtype=np.int32))
+    q = rng.standard_normal((2, 16 * hd)).astype(np.float32)
+    dq, out = up(q), torch.zeros(2, 16 * hd, device="cuda")
+    ws = dev.workspace(1, 16)
+    assert gpu.ckb200_dev_attention_q4cache(dq.data_ptr(), 16 * hd, dev.k.data_ptr(), dev.v.data_ptr(), out.data_ptr(), 16 * hd, big.data_ptr(), columns, lens.data_ptr(), 2, 1, 2, 16, 16, hkv,
+                                            hd, 0, ws.data_ptr(), ws.numel(), handle()) == 0
+    torch.cuda.synchronize()
+    want, off = small.attention(q, 1, 16)
+    # 2^24 weights are added by 444 CTAs in chunks of 32: 2^10 roundings in a row at the most, where the bound has 16
+    near(out.cpu().numpy(), want, off + 2.0 ** -13)
 
 
 @pytest.mark.gpu
