@@ -13,6 +13,7 @@ _CACHE_API = {
     "ckb200_kv_q4_row_offset": (_L, [_P] + [_I] * 7),
     "ckb200_dev_kv_cache_store_q4": (_I, [_P] * 4 + [_L] * 2 + [_P, _I, _P] + [_I] * 6 + [_P]),
     "ckb200_dev_kv_cache_load_q4": (_I, [_P] * 2 + [_L] * 2 + [_P] * 3 + [_I, _P] + [_I] * 6 + [_P]),
+    "ckb200_dev_rope_kv_store_q4": (_I, [_P] * 7 + [_I, _P, _I, _P] + [_I] * 6 + [_P]),
     "ckb200_attention_q4cache_workspace_bytes": (_Z, [_I] * 5),
     "ckb200_dev_attention_q4cache": (_I, [_P, _L, _P, _P, _P, _L, _P, _I, _P] + [_I] * 8 + [_P, _Z, _P]),
     "ckb200_kv_pages_workspace_bytes": (_Z, [_I] * 3),

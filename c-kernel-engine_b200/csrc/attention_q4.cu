@@ -75,7 +75,7 @@ __device__ __forceinline__ void aq_range(const AqParams &p, int nrows, int unit,
     w.begin = p.window > 0 ? max(0, at + t0 - p.window + 1) & ~15 : 0;
     w.n = w.end > w.begin ? (w.end - w.begin + unit - 1) / unit : 0;
 }
-__device__ __forceinline__ int aq_length(const AqParams &p, int b) { return kv_len(__ldg(p.c.lens + b), p.c.stride, p.c.page_tokens); }
+__device__ __forceinline__ int aq_length(const AqParams &p, int b) { return kv_len(__ldcg(p.c.lens + b), p.c.stride, p.c.page_tokens); }
 // the next stretch that has units; its first one.  False: there is none
 __device__ __forceinline__ bool aq_next_stretch(const AqParams &p, int nrows, int unit, AqWalk &w)
 {
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
         for (int i = 0; i < STAGES; ++i) mbar_init(smem_u32(&full[warp][i]), 1);
         mbar_fence_init();
     }
-    pdl_trigger();
+    pdl_wait();                                                // lengths, table, rows and cache come from the kernels before this one: read through L2
 
     // ---- this CTA's part of the line: units of all sequences are counted, each thread some consecutive ones
     const int each = (p.c.batch + AQ_THREADS - 1) / AQ_THREADS, b0 = min(p.c.batch, tid * each), b1 = min(p.c.batch, b0 + each);
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
         const bool one_page = p.c.page_tokens % S::CHUNK == 0 && p.window == 0;
         const size_t page_bytes = kv_row(1, 0, 0, p.c.Hkv, p.c.page_tokens, G4);
         int entry = -1;
-        auto look = [&](int pos) { return pos < f.end ? kv_entry(__ldg(p.c.table + (size_t)f.b * p.c.stride + page_of(pos)), p.c.pages) : -1; };
+        auto look = [&](int pos) { return pos < f.end ? kv_entry(__ldcg(p.c.table + (size_t)f.b * p.c.stride + page_of(pos)), p.c.pages) : -1; };
         const uint32_t ring = smem_u32(aq_smem) + warp * STAGES * S::STAGE;
         auto fetch = [&](int i) {                              // the i-th unit of this CTA into stage i % STAGES
             if (f_at >= last) return;
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                 const float *src = p.q + ((long long)w.b * p.c.tokens + tok) * p.q_stride + (long long)(w.h * p.G + row - tok * p.G) * HD;
 #pragma unroll
                 for (int j = 0; j < G4; ++j) {
-                    x[j] = row < p.R ? __ldg(src + 32 * j + lane) : 0.0f;
+                    x[j] = row < p.R ? __ldcg(src + 32 * j + lane) : 0.0f;
                     top = fmaxf(top, fabsf(x[j]));
                 }
                 const int ex_top = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23);      // biased exponent of the row's largest
@@ -679,6 +679,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
         if (!ok)                                               // a wait ran out: the copies still on their way end before the CTA does
             for (int s = max(0, i - STAGES); s < i; ++s) mbar_wait_spin(smem_u32(&full[warp][s % STAGES]), (uint32_t)(s / STAGES) & 1u);
     }
+    pdl_trigger();                                             // not earlier: what comes behind would only wait in this kernel's place
     // blocks of query rows that see no key
     for (int x = me; x < p.c.batch * p.RC; x += N) {
         AqWalk w;
@@ -774,8 +775,7 @@ static int aq_launch(AqParams p, void *ws, cudaStream_t st)
         if (ckb_check_cuda((int)cudaFuncSetAttribute(attn_q4_kernel<HD, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "attention_q4cache")) return CKB_ERR_CUDA;
         attr_set = true;
     }
-    attn_q4_kernel<HD, NB><<<N, AQ_THREADS, S::SMEM, st>>>(p);
-    const int rc = ckb_check_launch("attention_q4cache");
+    const int rc = launch_pdl("attention_q4cache", attn_q4_kernel<HD, NB>, dim3(N), dim3(AQ_THREADS), (size_t)S::SMEM, st, p);
     if (rc || p.c.stride * p.c.page_tokens <= S::UNIT) return rc;      // no stretch has two units
     // Few stretches are in many parts each, and their CTAs few (64 of 32 parts: 6 us, 18 us with a load at a time); many are in two or three (2048 of them: 4 us, 32 us
     // with the CTAs of the other kind).

@@ -11,6 +11,7 @@
 #include "device_common.cuh"
 #include "kv_q4.cuh"
 #include "launch.h"
+#include "pdl.cuh"
 #include "runtime.h"
 
 namespace ckb {
@@ -86,7 +87,7 @@ __device__ __forceinline__ void kr_where(const KrRows &p, uint32_t grp, int &row
     row = p.by_items(grp);
     block = (int)(grp - (uint32_t)row * p.by_items.d);
     const int b = p.by_tokens(row), t = row - b * p.c.tokens, head = p.by_nb(block);
-    const int pos = kv_len(__ldg(p.c.lens + b), p.c.stride, p.c.page_tokens) - p.c.tokens + t;
+    const int pos = kv_len(__ldcg(p.c.lens + b), p.c.stride, p.c.page_tokens) - p.c.tokens + t;
     at = -1;
     if (pos < 0) return;
     const int column = p.by_page(pos), page = kv_entry(__ldg(p.c.table + (size_t)b * p.c.stride + column), p.c.pages);      // pos is below the length: the column exists
@@ -149,6 +150,70 @@ __global__ void __launch_bounds__(KR_THREADS) kv_load_q4_kernel(float *__restric
     kr_store4<VEC>(x + 16, kr_values(dmk, wk >> 4));
     kr_store4<VEC>(y, kr_values(dmv, wv));
     kr_store4<VEC>(y + 16, kr_values(dmv, wv >> 4));
+}
+
+// One new token of each sequence: q rotated in place, k rotated and quantised, v quantised.  Four lanes a block as above; those of q come after those of the cache.
+// Channels i and i + head_dim / 2 turn together, and a lane's four channels lie on one side of the middle: their partners are one load more.
+__global__ void __launch_bounds__(KR_THREADS) rope_kv_store_q4_kernel(float *__restrict__ q, uint8_t *__restrict__ kp, uint8_t *__restrict__ vp, const float *__restrict__ k,
+                                                                      const float *__restrict__ v, const float *__restrict__ cos_cache, const float *__restrict__ sin_cache,
+                                                                      int positions, int H, int pairs, KrRows p)
+{
+    pdl_trigger();
+    pdl_wait();
+    const int l = threadIdx.x & 3, hd = 32 * p.c.nb, half = hd / 2;
+    const uint32_t grp = blockIdx.x * (KR_THREADS / 4) + (threadIdx.x >> 2);
+    const uint32_t stored = (p.groups + 7) & ~7u;              // whole warps: the shuffles below
+    if (grp >= stored) {
+        // eight channels of the first half of a row of q, and their partners
+        const uint32_t i = (grp - stored) * 4 + l, per_row = half / 8;
+        if (i >= (uint32_t)pairs) return;
+        const int row = (int)(i / per_row), c0 = (int)(i - row * per_row) * 8, b = row / H;
+        const int pos = kv_len(__ldcg(p.c.lens + b), p.c.stride, p.c.page_tokens) - 1;
+        if (pos < 0 || pos >= positions) return;
+        float *x = q + (size_t)row * hd + c0;
+        const float *cs = cos_cache + (size_t)pos * half + c0, *sn = sin_cache + (size_t)pos * half + c0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float a = __ldcg(x + e), z = __ldcg(x + e + half), c = cs[e], s = sn[e];
+            x[e] = __fsub_rn(__fmul_rn(a, c), __fmul_rn(z, s));
+            x[e + half] = __fadd_rn(__fmul_rn(a, s), __fmul_rn(z, c));
+        }
+        return;
+    }
+    float a[8] = {}, b[8] = {};
+    long long at = -1;
+    if (grp < p.groups) {
+        int row, block;
+        kr_where(p, grp, row, block, at);
+        const int pos = kv_len(__ldcg(p.c.lens + row), p.c.stride, p.c.page_tokens) - 1, head = p.by_nb(block), first = 32 * (block - head * p.c.nb) + 4 * l;
+        if (pos >= positions) at = -1;
+        if (at >= 0) {
+            const float *x = k + ((size_t)row * p.c.Hkv + head) * hd, *y = v + ((size_t)row * p.c.Hkv + head) * hd + first;
+            const float *cs = cos_cache + (size_t)pos * half, *sn = sin_cache + (size_t)pos * half;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int i = first + (e & 3) + 16 * (e >> 2), turn = i < half ? i : i - half;
+                const float u = __ldcg(x + turn), w = __ldcg(x + turn + half), c = cs[turn], s = sn[turn];
+                a[e] = i < half ? __fsub_rn(__fmul_rn(u, c), __fmul_rn(w, s)) : __fadd_rn(__fmul_rn(u, s), __fmul_rn(w, c));
+                b[e] = __ldcg(y + (e & 3) + 16 * (e >> 2));
+            }
+        }
+    }
+    uint32_t dmk, dmv;
+    const uint32_t wk = kr_quantise(make_float4(a[0], a[1], a[2], a[3]), make_float4(a[4], a[5], a[6], a[7]), dmk);
+    const uint32_t wv = kr_quantise(make_float4(b[0], b[1], b[2], b[3]), make_float4(b[4], b[5], b[6], b[7]), dmv);
+    if (at < 0) return;
+    uint32_t *x = reinterpret_cast<uint32_t *>(kp + at), *y = reinterpret_cast<uint32_t *>(vp + at);
+    x[1 + l] = wk;
+    y[1 + l] = wv;
+    if (l == 0) x[0] = dmk;
+    if (l == 1) y[0] = dmv;
+}
+
+// lengths of `batch` sequences that are all at *pos: its token counted
+__global__ void kv_lens_from_pos_kernel(int *lens, const int *pos, int batch)
+{
+    for (int b = threadIdx.x; b < batch; b += blockDim.x) lens[b] = *pos + 1;
 }
 
 }  // namespace ckb
@@ -257,4 +322,35 @@ extern "C" int ckb200_dev_kv_cache_load_q4(float *k, float *v, long long k_strid
     else
         kv_load_q4_kernel<false><<<grid, KR_THREADS, 0, ckb_stream(stream)>>>(k, v, (const uint8_t *)k_pages, (const uint8_t *)v_pages, p);
     return ckb_check_launch(what);
+}
+
+extern "C" int ckb200_dev_rope_kv_store_q4(float *q, const float *k, const float *v, void *k_pages, void *v_pages, const float *cos_cache, const float *sin_cache, int rope_positions,
+                                           const int *page_table, int table_stride, const int *kv_lens, int batch, int num_pages, int page_tokens, int num_heads, int num_kv_heads,
+                                           int head_dim, void *stream)
+{
+    const char *what = "rope_kv_store_q4";
+    int rc = ckb_check_kv_q4(what, k_pages, v_pages, page_table, table_stride, kv_lens, batch, 1, num_pages, page_tokens, num_kv_heads, head_dim);
+    if (rc || (rc = check_rows(what, k, v, 0, 0, 1, num_kv_heads * head_dim))) return rc;
+    if (!q || !cos_cache || !sin_cache) return ckb_fail(CKB_ERR_STATE, "%s: a pointer is NULL", what);
+    if (num_heads <= 0 || rope_positions <= 0) return ckb_fail(CKB_ERR_SHAPE, "%s: %d heads, tables of %d positions", what, num_heads, rope_positions);
+    if (((uintptr_t)q | (uintptr_t)cos_cache | (uintptr_t)sin_cache) & 3) return ckb_fail(CKB_ERR_ALIGN, "%s: rows must be aligned to 4 bytes", what);
+    const long long pairs = (long long)batch * num_heads * (head_dim / 16);
+    if (pairs > 0x3fffffffLL) return ckb_fail(CKB_ERR_LIMIT, "%s: %d sequences of %d heads", what, batch, num_heads);
+    const KvQ4 c = {page_table, kv_lens, table_stride, batch, 1, num_pages, page_tokens, num_kv_heads, head_dim / 32};
+    KrRows p;
+    unsigned grid;
+    if ((rc = rows_params(what, c, batch, 0, 0, &p, &grid))) return rc;
+    if (!batch) return 0;
+    if (ckb_ensure_init()) return CKB_ERR_NO_DEVICE;
+    if ((rc = ckb_check_device(what))) return rc;
+    grid = (unsigned)((((long long)p.groups + 7) / 8 * 8 + (pairs + 3) / 4 + KR_THREADS / 4 - 1) / (KR_THREADS / 4));
+    return launch_pdl(what, rope_kv_store_q4_kernel, dim3(grid), dim3(KR_THREADS), 0, ckb_stream(stream), q, (uint8_t *)k_pages, (uint8_t *)v_pages, k, v, cos_cache, sin_cache,
+                      rope_positions, num_heads, (int)pairs, p);
+}
+
+// kv_lens of sequences that are all at *pos_dev, for a step that begins (model_kquant.c)
+extern "C" int ckb_kv_lens_from_pos(int *kv_lens, const int *pos_dev, int batch, void *stream)
+{
+    kv_lens_from_pos_kernel<<<1, 256, 0, ckb_stream(stream)>>>(kv_lens, pos_dev, batch);
+    return ckb_check_launch("kv_lens_from_pos");
 }

@@ -30,6 +30,7 @@
 #include <string.h>
 
 #include "../../include/ckb200.h"
+#include "../../include/ckb200_cache.h"
 #include "../../include/ckb200_model.h"
 #include "launch.h"
 #include "model_internal.h"
@@ -89,9 +90,14 @@ typedef struct {
     size_t planar_bytes;
     int planar_ready;
     uint8_t *kv;            /* [L][2][B][Hkvl][S][d], elements of kv_eb bytes */
-    int kv_eb;              /* 4: fp32 cache; 2: IEEE fp16 cache (tune model_kv_f16 at creation: kv_cache_store_f16 and the
+    int kv_eb;              /* 4: fp32 cache; 1: 4-bit cache (tune model_kv_q4 at creation: Q4_1 rows, a sequence one page of the paged cache; strides in
+                             * bytes); 2: IEEE fp16 cache (tune model_kv_f16 at creation: kv_cache_store_f16 and the
                              * _f16cache attention of the reference, half the cache bytes per key) */
     long long kv_layer_stride, kv_batch_stride;     /* in elements */
+    int *kv_table, *kv_lens;    /* of the 4-bit cache: sequence b's only page is b; tokens of each with the step's own */
+    int kv_page_tokens;
+    void *kv_ws;
+    size_t kv_ws_bytes;
     float *rope_cos, *rope_sin;
     /* activations */
     float *x, *prev, *q, *k, *v, *att, *o, *gu, *attn_scratch;
@@ -136,6 +142,7 @@ static void *kv_at(const KqModel *m, int layer, int is_v)
     return m->kv + ((size_t)layer * (size_t)m->kv_layer_stride + (is_v ? (size_t)m->c.batch * (size_t)m->kv_batch_stride : 0)) * (size_t)m->kv_eb;
 }
 static int ps_build(KqModel *m, cudaStream_t st);
+int ckb_kv_lens_from_pos(int *kv_lens, const int *pos_dev, int batch, void *stream);        /* kv_q4_rows.cu */
 static int round256(int v) { return (v + 255) / 256 * 256; }
 
 static size_t fmt_row_bytes(int fmt, int cols)
@@ -196,7 +203,13 @@ CKB200Model *ckb200_model_create(const CKB200ModelConfig *cfg)
         free(m);
         return NULL;
     }
-    m->kv_eb = ckb_tune_get("model_kv_f16", 0) ? 2 : 4;
+    m->kv_eb = ckb_tune_get("model_kv_q4", 0) ? 1 : (ckb_tune_get("model_kv_f16", 0) ? 2 : 4);
+    m->kv_page_tokens = (cfg->max_seq_len + 15) & ~15;
+    if (m->kv_eb == 1 && !ckb200_kv_q4_page_bytes(m->Hkvl, m->kv_page_tokens, m->d)) {
+        ckb_fail(CKB_ERR_SHAPE, "model_create: the 4-bit cache needs a head size of 64, 96, 128, 192 or 256 (have %d)", m->d);
+        free(m);
+        return NULL;
+    }
     if (m->kv_eb == 2 && ((m->d != 64 && m->d != 128) || m->Hl / m->Hkvl > 8 || ((long long)m->Hkvl * cfg->max_seq_len * m->d) % 8)) {
         ckb_fail(CKB_ERR_SHAPE, "model_create: the fp16 cache needs a head size of 64 or 128 and at most 8 query heads per kv head (have %d, %d)", m->d,
                  m->Hl / m->Hkvl);
@@ -259,7 +272,7 @@ CKB200Model *ckb200_model_create(const CKB200ModelConfig *cfg)
 #define DEV_ALLOC(ptr, bytes) do { if (ok && ckb_check_cuda((int)cudaMalloc((void **)&(ptr), (bytes)), "cudaMalloc(model)")) ok = 0; } while (0)
     DEV_ALLOC(m->arena, m->arena_bytes);
     if (m->planar_bytes) DEV_ALLOC(m->planar_arena, m->planar_bytes);
-    m->kv_batch_stride = (long long)m->Hkvl * S * m->d;
+    m->kv_batch_stride = m->kv_eb == 1 ? (long long)ckb200_kv_q4_page_bytes(m->Hkvl, m->kv_page_tokens, m->d) : (long long)m->Hkvl * S * m->d;
     m->kv_layer_stride = 2LL * B * m->kv_batch_stride;
     DEV_ALLOC(m->kv, kv_bytes(m));
     DEV_ALLOC(m->rope_cos, (size_t)S * (m->d / 2) * sizeof(float));
@@ -288,7 +301,15 @@ CKB200Model *ckb200_model_create(const CKB200ModelConfig *cfg)
         m->gemm_ws_bytes = need;
         DEV_ALLOC(m->gemm_ws, need);
     }
-    m->attn_splits = ckb200_attention_decode_splits_kv(B, m->Hkvl, S, m->kv_eb);
+    m->attn_splits = m->kv_eb == 1 ? 1 : ckb200_attention_decode_splits_kv(B, m->Hkvl, S, m->kv_eb);
+    if (m->kv_eb == 1) {
+        m->kv_ws_bytes = ckb200_attention_q4cache_workspace_bytes(B, 1, m->Hl, m->Hkvl, m->d);
+        DEV_ALLOC(m->kv_ws, m->kv_ws_bytes);
+        DEV_ALLOC(m->kv_table, (size_t)B * sizeof(int));
+        DEV_ALLOC(m->kv_lens, (size_t)B * sizeof(int));
+        for (int b = 0; ok && b < B; ++b)
+            if (ckb_check_cuda((int)cudaMemcpy(m->kv_table + b, &b, sizeof b, cudaMemcpyHostToDevice), "page table")) ok = 0;
+    }
     {
         size_t sb = ckb200_attention_decode_scratch_bytes(B, m->Hl, m->d, m->attn_splits);
         DEV_ALLOC(m->attn_scratch, sb ? sb : 256);
@@ -332,7 +353,7 @@ static void kq_destroy(CKB200Model *model)
     KqModel *m = (KqModel *)model;
     void *ptrs[] = { m->arena, m->planar_arena, m->kv, m->rope_cos, m->rope_sin, m->x, m->prev, m->o, m->q, m->k, m->v, m->att, m->gu,
                      m->hq, m->aq, m->mq, m->attn_scratch, m->gemm_ws, m->mf, m->attn_counters,
-                     m->pf_arena, m->ps_table, m->ps_part, m->ps_sync };
+                     m->pf_arena, m->ps_table, m->ps_part, m->ps_sync, m->kv_table, m->kv_lens, m->kv_ws };
     for (size_t i = 0; i < sizeof ptrs / sizeof ptrs[0]; ++i) if (ptrs[i]) cudaFree(ptrs[i]);
     for (int i = 0; i < 2; ++i) {
         if (m->side[i]) cudaStreamDestroy(m->side[i]);
@@ -416,7 +437,23 @@ int ckb200_model_fill_kv_synthetic(CKB200Model *model, int tokens, unsigned long
     const int L = m->c.num_layers, B = m->c.batch, S = m->c.max_seq_len;
     cudaStream_t st = ckb_stream(NULL);
     cudaMemsetAsync(m->kv, 0, kv_bytes(m), st);
-    if (tokens > 0) {
+    if (tokens > 0 && m->kv_eb == 1) {
+        /* N(0,1) keys and values, sequence by sequence, through the store */
+        const size_t n = (size_t)tokens * m->Hkvl * m->d;
+        const int last = tokens - 1;
+        float *kv = NULL;
+        int rc = ckb_check_cuda((int)cudaMalloc((void **)&kv, 2 * n * sizeof(float)), "cudaMalloc(kv fill)") ||
+                 ckb_check_cuda((int)cudaMemcpyAsync(m->pos_dev, &last, sizeof last, cudaMemcpyHostToDevice, st), "kv fill") || ckb_kv_lens_from_pos(m->kv_lens, m->pos_dev, B, st);
+        for (int i = 0; !rc && i < L * B; ++i) {
+            const int l = i / B, b = i % B;
+            ckb200_dev_fill_normal(kv, (long long)(2 * n), 0, seed + (unsigned long long)i, st);
+            rc = ckb200_dev_kv_cache_store_q4(kv_at(m, l, 0), kv_at(m, l, 1), kv, kv + n, m->Hkvl * m->d, m->Hkvl * m->d, m->kv_table + b, 1, m->kv_lens + b, 1, tokens, B,
+                                              m->kv_page_tokens, m->Hkvl, m->d, st);
+        }
+        cudaStreamSynchronize(st);
+        cudaFree(kv);
+        if (rc) return CKB_ERR_CUDA;
+    } else if (tokens > 0) {
         /* N(0,1) in the first `tokens` positions of every head: fill a compact buffer, then strided copy */
         const size_t heads = (size_t)L * 2 * B * m->Hkvl, eb = (size_t)m->kv_eb;
         uint8_t *tmp = NULL;
@@ -622,7 +659,7 @@ static void ps_seg(PsSeg *s, const Tensor *t, int cta0, int ncta)
 static int ps_build(KqModel *m, cudaStream_t st)
 {
     const int L = m->c.num_layers, sms = ckb_sm_count();
-    if (m->c.batch != 1 || m->c.tp_size != 1 || (m->d != 64 && m->d != 128) || m->Hl / m->Hkvl > PS_MAX_GROUP || m->Hkvl > sms / 2 || L < 1 || sms < 3 || m->Il % 256) return 0;
+    if (m->c.batch != 1 || m->c.tp_size != 1 || m->kv_eb == 1 || (m->d != 64 && m->d != 128) || m->Hl / m->Hkvl > PS_MAX_GROUP || m->Hkvl > sms / 2 || L < 1 || sms < 3 || m->Il % 256) return 0;
     size_t stage = 0;
     PsLayer *table = (PsLayer *)calloc((size_t)L, sizeof *table);
     if (!table) return ckb_fail(CKB_ERR_STATE, "model step: out of memory");
@@ -697,6 +734,7 @@ static int issue_step(KqModel *m, void *st)
     /* embedding of the B current tokens -> x */
     rc = ckb200_dev_embedding_rows(m->tokens_dev, B, c->vocab_size, m->emb.w, m->emb.fmt, m->emb.cols, m->x, m->Da, m->D, st);
     if (rc) return rc;
+    if (m->kv_eb == 1 && (rc = ckb_kv_lens_from_pos(m->kv_lens, m->pos_dev, B, st))) return rc;
     float *delta = NULL;
     for (int l = 0; l < L; ++l) {
         Tensor *t = m->layers[l].t;
@@ -720,6 +758,14 @@ static int issue_step(KqModel *m, void *st)
             if ((rc = matvec(m, &t[CKB_T_WQ], m->hq, m->q, m->Al, st))) return rc;
             if ((rc = matvec(m, &t[CKB_T_WK], m->hq, m->k, m->Hkvl * m->d, st))) return rc;
             if ((rc = matvec(m, &t[CKB_T_WV], m->hq, m->v, m->Hkvl * m->d, st))) return rc;
+        }
+        if (m->kv_eb == 1) {
+            const int S16 = m->kv_page_tokens;
+            if ((rc = ckb200_dev_rope_kv_store_q4(m->q, m->k, m->v, kc, vc, m->rope_cos, m->rope_sin, c->max_seq_len, m->kv_table, 1, m->kv_lens, B, B, S16, m->Hl, m->Hkvl, m->d, st)))
+                return rc;
+            if ((rc = ckb200_dev_attention_q4cache(m->q, m->Al, kc, vc, m->att, m->Al, m->kv_table, 1, m->kv_lens, B, 1, B, S16, m->Hl, m->Hkvl, m->d, 0, m->kv_ws, m->kv_ws_bytes, st)))
+                return rc;
+            goto attention_done;
         }
         if (m->kv_eb == 2) {
             /* fp16 caches: the rotation stays fp32, k and v are rounded once on the store, attention widens them again */

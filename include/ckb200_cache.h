@@ -51,6 +51,13 @@ int ckb200_dev_kv_cache_load_q4(float *k, float *v, long long k_stride, long lon
                                 int table_stride, const int *kv_lens, int batch, int num_tokens, int num_pages, int page_tokens, int num_kv_heads, int head_dim,
                                 void *stream);
 
+/* A decode step's turn: one new token of each sequence, at position kv_lens[b] - 1.  q [batch][num_heads][head_dim] is rotated in place, k [batch][num_kv_heads][head_dim]
+ * rotated and stored, v stored: rope_forward_qk (src/kernels/rope_kernels.c:806-819) and the store above, as ckb200_dev_rope_kv_store_f16.  Tables of rope_positions rows of
+ * head_dim / 2 values; a sequence whose position lies outside them is left as it is. */
+int ckb200_dev_rope_kv_store_q4(float *q, const float *k, const float *v, void *k_pages, void *v_pages, const float *cos_cache, const float *sin_cache, int rope_positions,
+                                const int *page_table, int table_stride, const int *kv_lens, int batch, int num_pages, int page_tokens, int num_heads, int num_kv_heads,
+                                int head_dim, void *stream);
+
 /* Causal attention of the T new tokens (one for a decode step, several for drafted tokens or a portion of a prompt) of every sequence over its cache, the new
  * tokens' own rows among it: attention_forward_decode_head_major_gqa_flash_f16cache (src/kernels/attention_kernels.c:3450-3557) over Q4_1 rows.
  * q, out: rows of [num_heads][head_dim] floats, q_stride and out_stride floats apart; scale 1 / sqrt(head_dim).  The token at position p sees keys

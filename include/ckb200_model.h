@@ -96,7 +96,9 @@ float *ckb200_model_logits_device(CKB200Model *m);
 void *ckb200_model_kv_device(CKB200Model *m, int layer, int is_v);       /* [batch][Hkv][max_seq][head_dim], fp32 unless ... */
 int ckb200_model_kv_element_bytes(CKB200Model *m);                       /* ... 2: the model was created with tune model_kv_f16 = 1 (IEEE fp16
                                                                           * cache: kv_cache_store_f16 + the _f16cache decode attention,
-                                                                          * src/kernels/kv_cache_kernels.c, attention_kernels.c:3450-3557) */
+                                                                          * src/kernels/kv_cache_kernels.c, attention_kernels.c:3450-3557); 1: with
+                                                                          * tune model_kv_q4 = 1: rows of Q4_1 blocks, [batch][Hkv][max_seq rounded
+                                                                          * up to 16][head_dim / 32 x 20 bytes] (ckb200_cache.h) */
 size_t ckb200_model_weight_bytes(CKB200Model *m);                        /* quantised bytes one step streams */
 
 

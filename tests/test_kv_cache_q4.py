@@ -34,7 +34,9 @@ LOAD = {n: STORE[n] for n in ("k", "v", "k_stride", "v_stride", "k_pages", "v_pa
                               "num_kv_heads", "head_dim", "stream")}
 ATTEND = dict(q=256, q_stride=512, k_pages=256, v_pages=256, out=256, out_stride=512, page_table=256, table_stride=4, kv_lens=256, batch=2, num_tokens=1, num_pages=8, page_tokens=16,
               num_heads=4, num_kv_heads=2, head_dim=128, sliding_window=0, workspace=256, workspace_bytes=1 << 40, stream=None)
-CALLS = {"ckb200_dev_kv_cache_store_q4": STORE, "ckb200_dev_kv_cache_load_q4": LOAD, "ckb200_dev_attention_q4cache": ATTEND}
+ROPE = dict(q=256, k=256, v=256, k_pages=256, v_pages=256, cos_cache=256, sin_cache=256, rope_positions=100, page_table=256, table_stride=4, kv_lens=256, batch=2, num_pages=8, page_tokens=16,
+            num_heads=4, num_kv_heads=2, head_dim=128, stream=None)
+CALLS = {"ckb200_dev_rope_kv_store_q4": ROPE, "ckb200_dev_kv_cache_store_q4": STORE, "ckb200_dev_kv_cache_load_q4": LOAD, "ckb200_dev_attention_q4cache": ATTEND}
 COMMON = [(dict(k_pages=None), STATE), (dict(v_pages=None), STATE), (dict(page_table=None), STATE), (dict(kv_lens=None), STATE), (dict(batch=-1), SHAPE), (dict(num_tokens=-1), SHAPE),
           (dict(num_pages=0), SHAPE), (dict(table_stride=0), SHAPE), (dict(page_tokens=0), SHAPE), (dict(page_tokens=24), SHAPE), (dict(num_kv_heads=0), SHAPE), (dict(head_dim=80), SHAPE),
           (dict(head_dim=32), SHAPE), (dict(k_pages=264), ALIGN), (dict(v_pages=257), ALIGN), (dict(kv_lens=258), ALIGN), (dict(table_stride=1 << 27), LIMIT), (dict(num_kv_heads=1025), LIMIT)]
@@ -42,7 +44,9 @@ ROWS = [(dict(k=None), STATE), (dict(v=None), STATE), (dict(k=257), ALIGN), (dic
 OWN = [(dict(q=None), STATE), (dict(out=None), STATE), (dict(q=258), ALIGN), (dict(num_heads=0), SHAPE), (dict(num_heads=5), SHAPE), (dict(sliding_window=-1), SHAPE), (dict(q_stride=511), SHAPE),
        (dict(out_stride=0), SHAPE), (dict(batch=1 << 20, num_tokens=1 << 20), LIMIT), (dict(batch=1 << 15, num_tokens=1 << 15), LIMIT), (dict(workspace=None), STATE),
        (dict(workspace_bytes=1000), STATE), (dict(workspace=264), ALIGN)]
-REFUSED = [(name, change, code) for name in CALLS for change, code in COMMON + (OWN if "attention" in name else ROWS)]
+TURN = [(dict(q=None), STATE), (dict(k=None), STATE), (dict(cos_cache=None), STATE), (dict(sin_cache=257), ALIGN), (dict(v=258), ALIGN), (dict(rope_positions=0), SHAPE), (dict(num_heads=0), SHAPE),
+        (dict(batch=1 << 28), LIMIT)]
+REFUSED = [(name, change, code) for name, args in CALLS.items() for change, code in COMMON + (OWN if "attention" in name else (TURN if "rope" in name else ROWS)) if set(change) <= set(args)]
 
 
 @pytest.mark.parametrize("name,change,code", REFUSED, ids=lambda v: v if isinstance(v, str) else (" ".join(v) if isinstance(v, dict) else ""))
@@ -56,7 +60,8 @@ def test_calls_that_are_refused(lib, name, change, code):
 @pytest.mark.parametrize("name", CALLS)
 def test_calls_without_rows_do_nothing(lib, name):
     for change in (dict(batch=0), dict(num_tokens=0)):
-        assert getattr(lib, name)(*{**CALLS[name], **change}.values()) == 0
+        if set(change) <= set(CALLS[name]):
+            assert getattr(lib, name)(*{**CALLS[name], **change}.values()) == 0
 
 
 def test_where_rows_lie(lib):
@@ -232,6 +237,39 @@ def near(got, want, off):
     # errors of single roundings do not add up to the worst case: together they stay within the square root of their number
     if np.linalg.norm(want):
         assert np.linalg.norm(got - want) <= 2e-5 * np.linalg.norm(want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,head_dim,page_tokens,lens", [(1, 1, 64, 16, [1]), (14, 2, 64, 16, [5, 0, 48, 49]), (5, 5, 96, 48, [100]), (32, 8, 128, 64, [64, 65, 3]), (3, 1, 192, 16, [20, 31]),
+                                                                      (6, 3, 256, 32, [33, 150, -1])])
+def test_a_turn_rotates_and_stores(gpu, heads, kv_heads, head_dim, page_tokens, lens):
+    """q and the pools after one call are, bit for bit, those of the rotation in fp32 and of the host's store; the last sequence's position is behind the tables and
+    it stays as it is, as does one of length 0."""
+    rng = np.random.default_rng(heads + head_dim)
+    c = random_cache(rng, kv_heads, head_dim, page_tokens, lens)
+    dev, batch, half = Device(gpu, c), len(lens), head_dim // 2
+    positions = max(lens) if batch > 1 and lens[-1] == max(lens) else max(lens) + 2
+    positions = lens[-1] - 1 if batch > 2 and lens[-1] == max(lens) else positions
+    angle = np.arange(positions)[:, None] * (10000.0 ** (-np.arange(half) / half))[None]
+    cos, sin = np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
+    q, k, v = (rng.standard_normal((batch, n, head_dim)).astype(np.float32) for n in (heads, kv_heads, kv_heads))
+
+    def turned(x):
+        y = x.copy()
+        for b, n in enumerate(lens):
+            if 0 < n <= positions:
+                u, w, co, si = x[b, :, :half], x[b, :, half:], cos[n - 1], sin[n - 1]
+                y[b, :, :half], y[b, :, half:] = u * co - w * si, u * si + w * co
+        return y
+
+    d = [up(a) for a in (q, k, v, cos, sin)]
+    assert gpu.ckb200_dev_rope_kv_store_q4(d[0].data_ptr(), d[1].data_ptr(), d[2].data_ptr(), dev.k.data_ptr(), dev.v.data_ptr(), d[3].data_ptr(), d[4].data_ptr(), positions,
+                                           dev.table.data_ptr(), c.table.shape[1], dev.lens.data_ptr(), batch, c.pages, page_tokens, heads, kv_heads, head_dim, handle()) == 0
+    torch.cuda.synchronize()
+    assert np.array_equal(d[0].cpu().numpy(), turned(q)) and np.array_equal(d[1].cpu().numpy(), k)
+    c.lens = np.where(c.lens > positions, 0, c.lens).astype(np.int32)
+    c.store(turned(k).reshape(batch, -1), v.reshape(batch, -1), 1)
+    assert np.array_equal(dev.k.cpu().numpy().reshape(c.k.shape), c.k) and np.array_equal(dev.v.cpu().numpy().reshape(c.v.shape), c.v)
 
 
 ATTENTION_CASES = [
