@@ -1,14 +1,17 @@
 // Causal attention over a paged 4-bit KV cache (include/ckb200_cache.h), one or several new tokens of each sequence, on the tensor cores at fp32
 // accuracy.
 //
-// Mathematics.  A key block of 32 channels is k = d c + m with 4-bit codes c, so a score is sum over blocks of d (q . c) + m (sum q), and
-// the output of a block's channels is sum over keys of (p d) c + sum p m.  Both inner products have a 4-bit integer on one side, which as an
-// fp16 operand is exact; the other side, fp32, goes in as two fp16 pieces (x = hi + lo, 22 bits), whose products add up in the same fp32
-// accumulators.  The codes are never converted: a nibble in bits 4..7 of a half IS the subnormal 16 c * 2^-24, so masks and shifts of a
-// 32-bit word of codes make A operands, and the power of two is taken out of the result.  (Not in bits 0..3: the tensor cores line products
-// up without normalising them, and what a subnormal has in leading zeros is lost below: 2e-5 of the result at 500 keys.)  Queries are scaled so
-// that the largest of a row is in [2^14, 2^15); weights p d by 2^e, e from the largest d so far, kept with the running maximum as one reference
-// (accumulators hold values relative to 2^ref, ref = max - e): neither piece falls out of fp16's range whatever the cache's magnitude.
+// Mathematics.  A block of 32 key channels is k = d c + m with 4-bit codes c, so a score is the sum over blocks of d (q . c) + m (sum q); a
+// block of value channels is v = d (c - 8) + (m + 8 d), so its part of the output is the sum over keys of (p d) (c - 8) + p (m + 8 d).  Every inner
+// product has a small integer or a number of the block on one side, exact in fp16 (the middle m + 8 d as two pieces), and on the other an fp32 number
+// that goes in as two fp16 pieces, x = hi + lo, 22 bits, whose products add up in the same fp32 accumulator.
+//   * Key codes are not converted at all: a nibble in bits 4..7 of a half IS the subnormal 16 c * 2^-24, so masks and shifts of a word of codes make
+//     operands, and the power of two is taken out of the result.  (Not in bits 0..3: the tensor cores line products up without normalising them, and what a
+//     subnormal has in leading zeros is lost below: 2e-5 of the result at 500 keys.)
+//   * Value codes are taken from their middle.  With c in place of c - 8 all terms of the sum have one sign, the tensor cores cut what they add to an accumulator
+//     instead of rounding it, and the error adds up: 2.3e-5 of the result at 131072 keys, 7e-7 as it is here.
+//   * Ranges: queries are scaled so that the largest of a row is in [2^14, 2^15), weights by 2^12, steps d by 2^b with the largest of them so far in [1, 2): no
+//     piece falls out of fp16's range whatever the cache's magnitude.  A weight times a step is a rounded half-precision product and its exact remainder.
 //
 //   scores  S^T = K Q^T   mma.m16n8k16: 16 keys x 8 query rows; a thread's A words are 4 bytes of codes of keys g and g + 8 (lane = 4 g + t), which
 //                         settles which channel sits at which k: the query's fragments are laid out to match
@@ -19,9 +22,15 @@
 //
 // Work.  A unit is 128 keys of one (sequence, kv head, 8 NB rows); the units of all sequences form one line that is cut evenly among the CTAs that
 // the GPU holds at once, so long and short sequences load it alike and nothing but the lengths on the device decides.  Each of the four warps takes
-// a quarter of a unit through a ring of its own (untiled bulk copies of 16-key pieces, the largest that never leave a page), without meeting the
+// a quarter of a unit through a ring of its own (untiled bulk copies: 32 rows of K and of V, or 16 where pages may end between), without meeting the
 // others until a sequence's stretch ends.  Stretches that lie within one CTA are written out at once, the others as partial results that
 // a second kernel joins (log-sum-exp).
+//
+// What bounds it.  Not HBM: the ring alone, without the arithmetic, takes 113 us for four sequences of 131072 tokens (64 heads over 8 of 128 channels,
+// 667 MB, 102 us at the measured copy rate), the whole kernel 221 us, 3.0 TB/s.  A chunk of 32 keys is 1009 warp instructions, 74 of them products, issued at 2.1 an
+// SM and cycle: half-rate logic (codes, 300 of them), half-precision and conversion instructions and the products, each alone at 15 to 30 % of its pipe, hinder one another.
+// Two, three or four CTAs an SM (8 to 16 warps, 255 to 128 registers): 239 / 221 / 223 us; chunks of 64 keys 213 us, but 10.2 us instead of 9.2 for 77 keys; a warp that
+// fetches for four others, which takes the registers of four: 217 us.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -65,14 +74,14 @@ struct AqParams {
 
 // where a CTA is on the line of units
 struct AqWalk {
-    int b, h, rc, u, n, begin, end, len;       // unit u of n; keys [begin, end), begin a multiple of 16
+    int b, h, rc, u, n, begin, end, len;       // unit u of n; keys [begin, end), begin a multiple of 32
 };
 // tokens r0 / G .. of block rc: the keys that any of them sees
 __device__ __forceinline__ void aq_range(const AqParams &p, int nrows, int unit, AqWalk &w)
 {
     const int t0 = w.rc * nrows / p.G, t1 = (min(p.R, (w.rc + 1) * nrows) - 1) / p.G, at = w.len - p.c.tokens;
     w.end = max(0, at + t1 + 1);
-    w.begin = p.window > 0 ? max(0, at + t0 - p.window + 1) & ~15 : 0;
+    w.begin = p.window > 0 ? max(0, at + t0 - p.window + 1) & ~31 : 0;      // a chunk's beginning
     w.n = w.end > w.begin ? (w.end - w.begin + unit - 1) / unit : 0;
 }
 __device__ __forceinline__ int aq_length(const AqParams &p, int b) { return kv_len(__ldcg(p.c.lens + b), p.c.stride, p.c.page_tokens); }
@@ -170,7 +179,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
     __shared__ long long s_sum[AQ_WARPS], s_rest;
     __shared__ int s_b;
     uint4 *qf = reinterpret_cast<uint4 *>(aq_smem + S::RING);                     // [NB][KS][lane] {hi b0, hi b1, lo b0, lo b1}
-    uint2 *qsum = reinterpret_cast<uint2 *>(aq_smem + S::RING + S::QF);           // [NB][lane] {hi, lo} sums of the scaled query over blocks 2t and 2t + 1, times 2^-20
+    uint2 *qsum = reinterpret_cast<uint2 *>(aq_smem + S::RING + S::QF);           // [NB][lane] {hi, lo} sums of the scaled query over blocks 2t and 2t + 1, times 2^-6: both in fp16's normal range
     __shared__ float q_factor[ROWS];
     float *dump = reinterpret_cast<float *>(aq_smem + S::RING);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -262,7 +271,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
         auto page_of = [&](int pos) { return (int)(__umulhi((uint32_t)pos, p.page_mul) >> p.page_shift); };
         // Lane 0 fetches: the table's entry for the start of the next chunk is read one chunk ahead.  A chunk that cannot span pages is one copy
         // of K rows and one of V rows, another one as many as it has pieces of 16.
-        const bool one_page = p.c.page_tokens % S::CHUNK == 0 && p.window == 0;
+        const bool one_page = p.c.page_tokens % S::CHUNK == 0;
         const size_t page_bytes = kv_row(1, 0, 0, p.c.Hkv, p.c.page_tokens, G4);
         int entry = -1;
         auto look = [&](int pos) { return pos < f.end ? kv_entry(__ldcg(p.c.table + (size_t)f.b * p.c.stride + page_of(pos)), p.c.pages) : -1; };
@@ -329,7 +338,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
 #pragma unroll
                 for (int j = 0; j < G4; ++j) {
                     const float y = x[j] * up;
-                    const float sum = group_sum<32>(y) * (1.0f / AQ_UNSCALE);
+                    const float sum = group_sum<32>(y) * 0.015625f;
                     if (lane == j / 2) (j & 1 ? sum1 : sum0) = sum;
                     // channel c of the block: k-step c / 16, thread t = (c % 16) / 4, place c % 4: b0 holds places 0 and 2, b1 places 1 and 3
                     const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
@@ -437,6 +446,8 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                                 s[x][nb][0] = s[x][nb][1] = s[x][nb][2] = s[x][nb][3] = 0.0f;
                                 aq_mma_k8(s[x][nb], m0, m1, b.y);
                                 aq_mma_k8(s[x][nb], m0, m1, b.x);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) s[x][nb][e] *= 64.0f / AQ_UNSCALE;
                             }
                         }
 #pragma unroll
@@ -588,8 +599,8 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
 #pragma unroll
                             for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] += acc[nb][e >> 2][e & 3];
                     }
-                    __syncwarp();                              // the stage, the exchange and the table are free again
                 }
+                __syncwarp();                                  // the stage and its word, the exchange and the table are free again
                 ++i;
                 ++at;
                 if (++w.u >= w.n || at >= last) break;

@@ -82,15 +82,17 @@ struct KrRows {
 };
 
 // where block `grp` of all rows lies: its row's number, its place in the row, and its place in the pools in bytes (-1: nowhere)
+// FRESH: the lengths come from a kernel that may still have been running when this one was launched
+template <bool FRESH>
 __device__ __forceinline__ void kr_where(const KrRows &p, uint32_t grp, int &row, int &block, long long &at)
 {
     row = p.by_items(grp);
     block = (int)(grp - (uint32_t)row * p.by_items.d);
     const int b = p.by_tokens(row), t = row - b * p.c.tokens, head = p.by_nb(block);
-    const int pos = kv_len(__ldcg(p.c.lens + b), p.c.stride, p.c.page_tokens) - p.c.tokens + t;
+    const int pos = kv_len(FRESH ? __ldcg(p.c.lens + b) : __ldg(p.c.lens + b), p.c.stride, p.c.page_tokens) - p.c.tokens + t;
     at = -1;
     if (pos < 0) return;
-    const int column = p.by_page(pos), page = kv_entry(__ldg(p.c.table + (size_t)b * p.c.stride + column), p.c.pages);      // pos is below the length: the column exists
+    const int column = p.by_page(pos), page = kv_entry(FRESH ? __ldcg(p.c.table + (size_t)b * p.c.stride + column) : __ldg(p.c.table + (size_t)b * p.c.stride + column), p.c.pages);      // pos is below the length: the column exists
     if (page >= 0) at = (long long)kv_row(page, head, pos - column * p.c.page_tokens, p.c.Hkv, p.c.page_tokens, p.c.nb) + (block - head * p.c.nb) * KQ4_BLOCK;
 }
 
@@ -104,7 +106,7 @@ __global__ void __launch_bounds__(KR_THREADS) kv_store_q4_kernel(uint8_t *__rest
     long long at = -1;
     if (grp < p.groups) {
         int row, block;
-        kr_where(p, grp, row, block, at);
+        kr_where<false>(p, grp, row, block, at);
         const float *x = k + row * p.k_stride + block * 32 + 4 * l, *y = v + row * p.v_stride + block * 32 + 4 * l;
         a[0] = kr_load4<VEC>(x);
         a[1] = kr_load4<VEC>(x + 16);
@@ -136,7 +138,7 @@ __global__ void __launch_bounds__(KR_THREADS) kv_load_q4_kernel(float *__restric
     if (grp >= p.groups) return;
     long long at;
     int row, block;
-    kr_where(p, grp, row, block, at);
+    kr_where<false>(p, grp, row, block, at);
     uint32_t dmk = 0, dmv = 0, wk = 0, wv = 0;
     if (at >= 0) {
         const uint32_t *x = reinterpret_cast<const uint32_t *>(kp + at), *y = reinterpret_cast<const uint32_t *>(vp + at);
@@ -184,7 +186,7 @@ __global__ void __launch_bounds__(KR_THREADS) rope_kv_store_q4_kernel(float *__r
     long long at = -1;
     if (grp < p.groups) {
         int row, block;
-        kr_where(p, grp, row, block, at);
+        kr_where<true>(p, grp, row, block, at);
         const int pos = kv_len(__ldcg(p.c.lens + row), p.c.stride, p.c.page_tokens) - 1, head = p.by_nb(block), first = 32 * (block - head * p.c.nb) + 4 * l;
         if (pos >= positions) at = -1;
         if (at >= 0) {
