@@ -10,8 +10,8 @@
 //     subnormal has in leading zeros is lost below: 2e-5 of the result at 500 keys.)
 //   * Value codes are taken from their middle.  With c in place of c - 8 all terms of the sum have one sign, the tensor cores cut what they add to an accumulator
 //     instead of rounding it, and the error adds up: 2.3e-5 of the result at 131072 keys, 7e-7 as it is here.
-//   * Ranges: queries are scaled so that the largest of a row is in [2^14, 2^15), weights by 2^12, steps d by 2^b with the largest of them so far in [1, 2): no
-//     piece falls out of fp16's range whatever the cache's magnitude.  A weight times a step is a rounded half-precision product and its exact remainder.
+//   * Ranges: queries are scaled so that the largest of a row is in [2^14, 2^15), weights, relative to a reference that may lag 2^3 behind the largest, by 2^10, steps d by
+//     2^b with the largest of them so far in [1, 2): no piece falls out of fp16's range whatever the cache's magnitude.  A weight times a step is a rounded half-precision product and its exact remainder.
 //
 //   scores  S^T = K Q^T   mma.m16n8k16: 16 keys x 8 query rows; a thread's A words are 4 bytes of codes of keys g and g + 8 (lane = 4 g + t), which
 //                         settles which channel sits at which k: the query's fragments are laid out to match
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
             }
             __syncthreads();
             float om[NB][2];                                   // row g: block g's sum of weight times middle
-            float o[NB][G4][2][4], m_run[NB], l_run[NB], fac[NB];
+            float o[NB][G4][2][4], m_run[NB], l_run[NB], fac[NB];      // m_run: the reference of the weights, in powers of two
             int pos_row[NB], b_run = 14;                       // pos_row: the position of row g of each block, -1 where there is none
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                     for (int y = 0; y < KL; ++y)
 #pragma unroll
                         for (int j = 0; j < G4; ++j) dtop = max(dtop, (dm[y][j] & 0x7c00u) == 0x7c00u ? 0u : dm[y][j] & 0x7fffu);
-                    // the largest d so far times 2^b is in [1, 2): its products with weights of up to 2^12 stay in fp16's range, their remainders above its least step
+                    // the largest d so far times 2^b is in [1, 2): its products with weights of up to 2^13 stay in fp16's range, their remainders above its least step
                     const int b_new = min(b_run, 15 - (int)min(29u, max(1u, __reduce_max_sync(0xffffffffu, dtop) >> 10)));
                     const __half2 d_scale = aq_h2((uint32_t)(15 + b_new) << 10);
 #pragma unroll
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                     }
                     __syncwarp();
 
-                    // ---- from (keys g, rows 2t) to (row g, keys 2t): weights times 2^12, as two pieces
+                    // ---- from (keys g, rows 2t) to (row g, keys 2t): weights times 2^10, as two pieces
                     uint32_t ph[NB][2 * S::XT], pl[NB][2 * S::XT];             // keys 8y + 2t and 8y + 2t + 1
                     float alpha[NB];
                     bool moved = b_new != b_run;
@@ -513,15 +513,18 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                         }
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                        const float m_new = fmaxf(m_run[nb], top * fac[nb]);
-                        moved |= m_new != m_run[nb];
+                        // the reference follows the maximum when it is more than 2^3 behind: each time costs every accumulator a product
+                        top *= fac[nb];
+                        const bool far = top > m_run[nb] + 3.0f;
+                        const float m_new = far ? top : m_run[nb];
+                        moved |= far;
                         const float ref = m_new == -INFINITY ? 0.0f : m_new;
                         alpha[nb] = m_run[nb] == -INFINITY ? 0.0f : aq_exp2(m_run[nb] - ref);
                         m_run[nb] = m_new;
                         float sum = 0.0f;
 #pragma unroll
                         for (int y = 0; y < 2 * S::XT; ++y) {
-                            const float2 e = make_float2(aq_exp2(fmaf(v[y].x, fac[nb], 12.0f - ref)), aq_exp2(fmaf(v[y].y, fac[nb], 12.0f - ref)));
+                            const float2 e = make_float2(aq_exp2(fmaf(v[y].x, fac[nb], 10.0f - ref)), aq_exp2(fmaf(v[y].y, fac[nb], 10.0f - ref)));
                             sum += e.x + e.y;
                             aq_split(e, ph[nb][y], pl[nb][y]);
                         }
