@@ -45,9 +45,11 @@ namespace ckb {
 
 constexpr int AQ_WARPS = 4, AQ_THREADS = 32 * AQ_WARPS;
 
-template <int HD, int NB>
+// BLOCKS 0: up to four query rows, whose hi pieces are columns 0 .. 3 of a product and whose lo pieces are columns 4 .. 7
+template <int HD, int BLOCKS>
 struct AqShape {
-    static constexpr int G4 = HD / 32, KS = HD / 16, ROW = G4 * KQ4_BLOCK, ROWS = 8 * NB;
+    static constexpr bool PACK = BLOCKS == 0;
+    static constexpr int NB = PACK ? 1 : BLOCKS, G4 = HD / 32, KS = HD / 16, ROW = G4 * KQ4_BLOCK, ROWS = PACK ? 4 : 8 * NB;
     static constexpr int XT = 2, CHUNK = 16 * XT, UNIT = AQ_WARPS * CHUNK;      // a warp takes XT tiles of 16 keys at a time
     static constexpr int SP = CHUNK + 8;                                          // floats between rows of the score exchange: 8 lanes' float2 loads touch every bank once
     static constexpr int STAGE = 2 * CHUNK * ROW;                              // K rows, then V rows
@@ -168,21 +170,23 @@ __device__ __forceinline__ float aq_lo(uint32_t dm) { return __low2float(*reinte
 __device__ __forceinline__ float aq_hi(uint32_t dm) { return __high2float(*reinterpret_cast<const __half2 *>(&dm)); }
 __device__ __forceinline__ bool aq_no_number(uint32_t dm) { return (dm & 0x7c00u) == 0x7c00u || (dm & 0x7c000000u) == 0x7c000000u; }
 
-template <int HD, int NB>
-__global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_kernel(const AqParams p)
+template <int HD, int BLOCKS>
+__global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4_kernel(const AqParams p)
 {
-    using S = AqShape<HD, NB>;
-    constexpr int G4 = S::G4, KS = S::KS, ROW = S::ROW, ROWS = S::ROWS, STAGES = S::STAGES;
+    using S = AqShape<HD, BLOCKS>;
+    constexpr bool PACK = S::PACK;
+    constexpr int NB = S::NB, G4 = S::G4, KS = S::KS, ROW = S::ROW, ROWS = S::ROWS, STAGES = S::STAGES;
     extern __shared__ __align__(128) uint8_t aq_smem[];
     __shared__ __align__(8) uint64_t full[AQ_WARPS][STAGES];
     __shared__ int pieces[AQ_WARPS][STAGES];
     __shared__ long long s_sum[AQ_WARPS], s_rest;
     __shared__ int s_b;
-    uint4 *qf = reinterpret_cast<uint4 *>(aq_smem + S::RING);                     // [NB][KS][lane] {hi b0, hi b1, lo b0, lo b1}
+    uint4 *qf = reinterpret_cast<uint4 *>(aq_smem + S::RING);                     // [NB][KS][lane] {hi b0, hi b1, lo b0, lo b1}; PACK: [KS][lane] {b0, b1}
+    const uint2 *qf2 = reinterpret_cast<const uint2 *>(qf);
     uint2 *qsum = reinterpret_cast<uint2 *>(aq_smem + S::RING + S::QF);           // [NB][lane] {hi, lo} sums of the scaled query over blocks 2t and 2t + 1, times 2^-6: both in fp16's normal range
     __shared__ float q_factor[ROWS];
     float *dump = reinterpret_cast<float *>(aq_smem + S::RING);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, g_row = PACK ? g & 3 : g;
     float *ex = reinterpret_cast<float *>(aq_smem + S::RING + S::QF + S::QS) + warp * NB * 8 * S::SP;
     // for each key of the warp's chunk: d times 2^b, and the middle m + 8 d of the values that a block can say, as two pieces; [G4][keys] halves each
     __half *tab = reinterpret_cast<__half *>(aq_smem + S::RING + S::QF + S::QS + S::EX) + warp * 3 * G4 * S::CHUNK;
@@ -266,58 +270,70 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
             }
             w.u = (int)rest;
         }
-        AqWalk f = w;                                          // the unit being fetched, up to STAGES - 1 further on
-        long long f_at = first;
-        auto page_of = [&](int pos) { return (int)(__umulhi((uint32_t)pos, p.page_mul) >> p.page_shift); };
-        // Lane 0 fetches: the table's entry for the start of the next chunk is read one chunk ahead.  A chunk that cannot span pages is one copy
-        // of K rows and one of V rows, another one as many as it has pieces of 16.
+        // Lane 0 fetches, up to STAGES - 1 units ahead: the table's entry for a chunk's beginning is read one chunk ahead.  A chunk that cannot span pages is one copy
+        // of K rows and one of V rows, another one as many as it has pieces of 16.  What stays the same in a stretch is worked out once for it.
+        AqWalk f = w;
+        int f_left = (int)(last - first), f_stage = 0, f_pos, f_slot = 0, entry = -1;
+        const int *f_table;
+        uint32_t f_head;
         const bool one_page = p.c.page_tokens % S::CHUNK == 0;
-        const size_t page_bytes = kv_row(1, 0, 0, p.c.Hkv, p.c.page_tokens, G4);
-        int entry = -1;
-        auto look = [&](int pos) { return pos < f.end ? kv_entry(__ldcg(p.c.table + (size_t)f.b * p.c.stride + page_of(pos)), p.c.pages) : -1; };
-        const uint32_t ring = smem_u32(aq_smem) + warp * STAGES * S::STAGE;
-        auto fetch = [&](int i) {                              // the i-th unit of this CTA into stage i % STAGES
-            if (f_at >= last) return;
+        const uint32_t page_bytes = (uint32_t)kv_row(1, 0, 0, p.c.Hkv, p.c.page_tokens, G4), ring = smem_u32(aq_smem) + warp * STAGES * S::STAGE, bars = smem_u32(&full[warp][0]);
+        auto look = [&](int pos, int &slot) {                  // the page of a position, and its place in it
+            if (pos >= f.end) return -1;
+            const int column = (int)(__umulhi((uint32_t)pos, p.page_mul) >> p.page_shift);
+            slot = pos - column * p.c.page_tokens;
+            return kv_entry(__ldcg(f_table + column), p.c.pages);
+        };
+        auto enter = [&]() {                                   // a stretch
+            f_table = p.c.table + (size_t)f.b * p.c.stride;
+            f_head = (uint32_t)(f.h * p.c.page_tokens * ROW);
+            f_pos = f.begin + f.u * S::UNIT + warp * S::CHUNK;
+        };
+        auto fetch = [&]() {                                   // the next unit into the next stage
+            if (f_left == 0) return;
             if (lane == 0) {
-                const int stage = i % STAGES, pos = f.begin + f.u * S::UNIT + warp * S::CHUNK;
-                const uint32_t bar = smem_u32(&full[warp][stage]), to = ring + stage * S::STAGE;
+                const uint32_t bar = bars + 8 * f_stage, to = ring + f_stage * S::STAGE;
+                auto copy = [&](uint32_t at, int page, int slot, uint32_t bytes) {
+                    const size_t src = (size_t)page * page_bytes + (f_head + (uint32_t)(slot * ROW));
+                    bulk_g2s(at, p.k + src, bytes, bar);
+                    bulk_g2s(at + S::CHUNK * ROW, p.v + src, bytes, bar);
+                };
                 if (one_page) {
-                    const int n = entry < 0 ? 0 : min(S::XT, (f.end - pos + 15) >> 4);
-                    pieces[warp][stage] = (1 << n) - 1;
+                    const int n = entry < 0 ? 0 : min(S::XT, (f.end - f_pos + 15) >> 4);
+                    pieces[warp][f_stage] = (1 << n) - 1;
                     mbar_arrive_expect_tx(bar, n * 2 * 16 * ROW);
-                    if (n) {
-                        const size_t at = (size_t)entry * page_bytes + (uint32_t)((f.h * p.c.page_tokens + pos - page_of(pos) * p.c.page_tokens) * ROW);
-                        bulk_g2s(to, p.k + at, n * 16 * ROW, bar);
-                        bulk_g2s(to + S::CHUNK * ROW, p.v + at, n * 16 * ROW, bar);
-                    }
+                    if (n) copy(to, entry, f_slot, n * 16 * ROW);
                 } else {
-                    int e[S::XT], there = 0;
+                    int e[S::XT], at[S::XT], there = 0;
 #pragma unroll
                     for (int x = 0; x < S::XT; ++x) {
-                        e[x] = x ? look(pos + 16 * x) : entry;
+                        at[x] = f_slot;
+                        e[x] = x ? look(f_pos + 16 * x, at[x]) : entry;
                         there |= (e[x] >= 0) << x;
                     }
-                    pieces[warp][stage] = there;
+                    pieces[warp][f_stage] = there;
                     mbar_arrive_expect_tx(bar, __popc(there) * 2 * 16 * ROW);
 #pragma unroll
                     for (int x = 0; x < S::XT; ++x)
-                        if (e[x] >= 0) {
-                            const int at_pos = pos + 16 * x;
-                            const size_t at = kv_row(e[x], f.h, at_pos - page_of(at_pos) * p.c.page_tokens, p.c.Hkv, p.c.page_tokens, G4);
-                            bulk_g2s(to + 16 * x * ROW, p.k + at, 16 * ROW, bar);
-                            bulk_g2s(to + (S::CHUNK + 16 * x) * ROW, p.v + at, 16 * ROW, bar);
-                        }
+                        if (e[x] >= 0) copy(to + 16 * x * ROW, e[x], at[x], 16 * ROW);
                 }
             }
-            ++f_at;
-            if (++f.u >= f.n && f_at < last) aq_next_stretch(p, ROWS, S::UNIT, f);
-            if (lane == 0 && f_at < last) entry = look(f.begin + f.u * S::UNIT + warp * S::CHUNK);
+            if (++f_stage == STAGES) f_stage = 0;
+            f_pos += S::UNIT;
+            if (--f_left == 0) return;
+            if (++f.u >= f.n) {
+                aq_next_stretch(p, ROWS, S::UNIT, f);
+                enter();
+            }
+            if (lane == 0) entry = look(f_pos, f_slot);
         };
-        if (lane == 0) entry = look(f.begin + f.u * S::UNIT + warp * S::CHUNK);
-        for (int i = 0; i < STAGES - 1; ++i) fetch(i);
+        enter();
+        if (lane == 0) entry = look(f_pos, f_slot);
+        for (int i = 0; i < STAGES - 1; ++i) fetch();
 
-        int i = 0;
-        for (long long at = first; at < last;) {
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int left = (int)(last - first); left;) {
             // ---- a stretch: query fragments of its rows
             const int r0 = w.rc * ROWS, u_first = w.u;
             __syncthreads();                                   // the stretch before is done with them
@@ -343,13 +359,20 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                     // channel c of the block: k-step c / 16, thread t = (c % 16) / 4, place c % 4: b0 holds places 0 and 2, b1 places 1 and 3
                     const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
                     const int place = lane & 3, to = ((((r >> 3) * KS + 2 * j + (lane >> 4)) * 32 + 4 * (r & 7) + ((lane & 15) >> 2)) * 8) + (place & 1) * 2 + (place >> 1);
-                    reinterpret_cast<__half *>(qf)[to] = hi;
-                    reinterpret_cast<__half *>(qf)[to + 4] = lo;
+                    if constexpr (PACK) {
+                        const int at = ((2 * j + (lane >> 4)) * 32 + 4 * r + ((lane & 15) >> 2)) * 4 + (place & 1) * 2 + (place >> 1);
+                        reinterpret_cast<__half *>(qf)[at] = hi;
+                        reinterpret_cast<__half *>(qf)[at + 64] = lo;          // four columns on
+                    } else {
+                        reinterpret_cast<__half *>(qf)[to] = hi;
+                        reinterpret_cast<__half *>(qf)[to + 4] = lo;
+                    }
                 }
                 if (lane < 4) {
                     uint2 v;
                     aq_split(make_float2(sum0, sum1), v.x, v.y);
                     qsum[(r >> 3) * 32 + 4 * (r & 7) + lane] = v;
+                    if constexpr (PACK) qsum[16 + 4 * r + lane].x = v.y;
                 }
             }
             __syncthreads();
@@ -358,9 +381,9 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
             int pos_row[NB], b_run = 14;                       // pos_row: the position of row g of each block, -1 where there is none
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                const int row = r0 + 8 * nb + g;
+                const int row = r0 + 8 * nb + g_row;
                 pos_row[nb] = row < p.R ? w.len - p.c.tokens + row / p.G : -1;
-                fac[nb] = q_factor[8 * nb + g];
+                fac[nb] = q_factor[8 * nb + g_row];
                 m_run[nb] = -INFINITY;
                 l_run[nb] = 0.0f;
                 om[nb][0] = om[nb][1] = 0.0f;
@@ -371,15 +394,13 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
             const int pos_first = w.len - p.c.tokens + r0 / p.G, pos_last = w.len - p.c.tokens + (min(p.R, r0 + ROWS) - 1) / p.G;
             const int all_to = pos_first + 1, all_from = p.window > 0 ? pos_last - p.window + 1 : 0;
 
-            for (;;) {
-                fetch(i + STAGES - 1);
-                const int stage = i % STAGES;
-                if (ok && !mbar_wait_spin(smem_u32(&full[warp][stage]), (uint32_t)(i / STAGES) & 1u)) {
+            for (int key0 = w.begin + w.u * S::UNIT + warp * S::CHUNK;; key0 += S::UNIT) {
+                fetch();
+                if (ok && !mbar_wait_spin(bars + 8 * stage, phase)) {
                     ok = false;
                     if (lane == 0) atomicExch(p.err, DEV_ERR_FULL_WAIT);
                 }
                 const uint32_t there = pieces[warp][stage];
-                const int key0 = w.begin + w.u * S::UNIT + warp * S::CHUNK;
                 if (there) {
                     const uint8_t *kb = aq_smem + (warp * STAGES + stage) * S::STAGE, *vb = kb + S::CHUNK * ROW;
                     const bool mixed = there != (1u << S::XT) - 1u || key0 < all_from || key0 + S::CHUNK > all_to;
@@ -444,7 +465,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                             for (int nb = 0; nb < NB; ++nb) {
                                 const uint2 b = qsum[nb * 32 + lane];
                                 s[x][nb][0] = s[x][nb][1] = s[x][nb][2] = s[x][nb][3] = 0.0f;
-                                aq_mma_k8(s[x][nb], m0, m1, b.y);
+                                if (!PACK) aq_mma_k8(s[x][nb], m0, m1, b.y);
                                 aq_mma_k8(s[x][nb], m0, m1, b.x);
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) s[x][nb][e] *= 64.0f / AQ_UNSCALE;
@@ -464,7 +485,15 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                                 }
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
-                                const uint4 q0 = qf[(nb * KS + 2 * j) * 32 + lane], q1 = qf[(nb * KS + 2 * j + 1) * 32 + lane];
+                                uint4 q0, q1;
+                                if constexpr (PACK) {
+                                    const uint2 u = qf2[2 * j * 32 + lane], w2 = qf2[(2 * j + 1) * 32 + lane];
+                                    q0 = make_uint4(0, 0, u.x, u.y);
+                                    q1 = make_uint4(0, 0, w2.x, w2.y);
+                                } else {
+                                    q0 = qf[(nb * KS + 2 * j) * 32 + lane];
+                                    q1 = qf[(nb * KS + 2 * j + 1) * 32 + lane];
+                                }
                                 float acc[S::XT][4];
 #pragma unroll
                                 for (int half = 0; half < 2; ++half)           // of the block
@@ -475,7 +504,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                                                                half ? aq_codes<3>(c[x][0]) : aq_codes<2>(c[x][0]), half ? aq_codes<3>(c[x][1]) : aq_codes<2>(c[x][1])};
                                         if (half == 0) aq_mma_first(acc[x], a, q.z, q.w);
                                         else aq_mma(acc[x], a, q.z, q.w);
-                                        aq_mma(acc[x], a, q.x, q.y);
+                                        if (!PACK) aq_mma(acc[x], a, q.x, q.y);
                                     }
 #pragma unroll
                                 for (int x = 0; x < S::XT; ++x)
@@ -502,7 +531,12 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                         float top = -INFINITY;
 #pragma unroll
                         for (int y = 0; y < 2 * S::XT; ++y) {
-                            v[y] = *reinterpret_cast<const float2 *>(ex + (nb * 8 + g) * S::SP + 8 * y + 2 * t);
+                            v[y] = *reinterpret_cast<const float2 *>(ex + (nb * 8 + g_row) * S::SP + 8 * y + 2 * t);
+                            if constexpr (PACK) {
+                                const float2 rest = *reinterpret_cast<const float2 *>(ex + (g_row + 4) * S::SP + 8 * y + 2 * t);
+                                v[y].x += rest.x;
+                                v[y].y += rest.y;
+                            }
                             if (mixed) {
                                 const int key = key0 + 8 * y + 2 * t, from = p.window > 0 ? pos_row[nb] - p.window : -1;
                                 const bool page = there >> (y >> 1) & 1u;
@@ -554,10 +588,11 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                             const uint32_t hi[4] = {mh.x, 0, mh.y, 0}, lo[4] = {ml.x, 0, ml.y, 0};
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
-                                if (x == 0) aq_mma_first(acc[nb], lo, ph[nb][0], ph[nb][1]);
-                                else aq_mma(acc[nb], lo, ph[nb][2 * x], ph[nb][2 * x + 1]);
-                                aq_mma(acc[nb], hi, pl[nb][2 * x], pl[nb][2 * x + 1]);
-                                aq_mma(acc[nb], hi, ph[nb][2 * x], ph[nb][2 * x + 1]);
+                                const uint32_t b0 = PACK && g >= 4 ? pl[nb][2 * x] : ph[nb][2 * x], b1 = PACK && g >= 4 ? pl[nb][2 * x + 1] : ph[nb][2 * x + 1];
+                                if (x == 0) aq_mma_first(acc[nb], lo, b0, b1);
+                                else aq_mma(acc[nb], lo, b0, b1);
+                                if (!PACK) aq_mma(acc[nb], hi, pl[nb][2 * x], pl[nb][2 * x + 1]);
+                                aq_mma(acc[nb], hi, b0, b1);
                             }
                         }
 #pragma unroll
@@ -586,6 +621,17 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                                 uint32_t h0, l0, h1, l1;
                                 aq_weigh(ph[nb][2 * x], pl[nb][2 * x], d.x, h0, l0);
                                 aq_weigh(ph[nb][2 * x + 1], pl[nb][2 * x + 1], d.y, h1, l1);
+                                if constexpr (PACK) {
+                                    const uint32_t b0 = g >= 4 ? l0 : h0, b1 = g >= 4 ? l1 : h1;
+                                    if (x == 0) {
+                                        aq_mma_first(acc[nb][0], a0, b0, b1);
+                                        aq_mma_first(acc[nb][1], a1, b0, b1);
+                                    } else {
+                                        aq_mma(acc[nb][0], a0, b0, b1);
+                                        aq_mma(acc[nb][1], a1, b0, b1);
+                                    }
+                                    continue;
+                                }
                                 if (x == 0) {
                                     aq_mma_first(acc[nb][0], a0, l0, l1);
                                     aq_mma_first(acc[nb][1], a1, l0, l1);
@@ -604,9 +650,9 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                     }
                 }
                 __syncwarp();                                  // the stage and its word, the exchange and the table are free again
-                ++i;
-                ++at;
-                if (++w.u >= w.n || at >= last) break;
+                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                --left;
+                if (++w.u >= w.n || left == 0) break;
             }
 
             // ---- the stretch ends here: the four warps' results, relative to 2^ref, become one
@@ -622,6 +668,10 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                     const float a0 = __shfl_sync(0xffffffffu, om[nb][0], 4 * j + t), a1 = __shfl_sync(0xffffffffu, om[nb][1], 4 * j + t);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] = fmaf(o[nb][j][e >> 2][e & 3], unscale, e & 1 ? a1 : a0);
+                    if constexpr (PACK) {                      // what hi and lo pieces gave, column c and c + 4
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] += __shfl_xor_sync(0xffffffffu, o[nb][j][e >> 2][e & 3], 2);
+                    }
                 }
             }
             auto put = [&](float *to) {
@@ -663,7 +713,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                 float *part = whole ? nullptr : p.part + (size_t)(2 * me + (u_first == 0)) * ROWS * (HD + 2);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    if (part && t == 0) {
+                    if (part && t == 0 && 8 * nb + g < ROWS) {
                         part[(8 * nb + g) * (HD + 2) + HD] = ref[nb];
                         part[(8 * nb + g) * (HD + 2) + HD + 1] = l_run[nb];
                     }
@@ -672,7 +722,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                         const int r = 8 * nb + 2 * t + e, row = r0 + r, tok = row / p.G;
                         const float l = __shfl_sync(0xffffffffu, l_run[nb], 8 * t + 4 * e);
                         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                        if (row >= p.R) continue;
+                        if (r >= ROWS || row >= p.R) continue;
                         float *to = part ? part + r * (HD + 2) : p.out + ((long long)w.b * p.c.tokens + tok) * p.out_stride + (long long)(w.h * p.G + row - tok * p.G) * HD;
 #pragma unroll
                         for (int j = 0; j < G4; ++j)
@@ -688,10 +738,17 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, NB>::CTAS) attn_q4_ker
                 if (u_first == 0 && lane == 0)                  // its last unit is n - u units behind the end of this CTA's part
                     p.desc[((size_t)w.b * p.c.Hkv + w.h) * p.RC + w.rc] = make_int2(me, whole ? -1 : (int)(((last + w.n - w.u) * parts - 1) / total));
             }
-            if (at < last) aq_next_stretch(p, ROWS, S::UNIT, w);
+            if (left) aq_next_stretch(p, ROWS, S::UNIT, w);
         }
-        if (!ok)                                               // a wait ran out: the copies still on their way end before the CTA does
-            for (int s = max(0, i - STAGES); s < i; ++s) mbar_wait_spin(smem_u32(&full[warp][s % STAGES]), (uint32_t)(s / STAGES) & 1u);
+        // a wait ran out: the copies still on their way, of the last STAGES units, end before the CTA does
+        if (!ok)
+            for (int i = 0; i < STAGES; ++i) {
+                if (i < (int)(last - first)) {
+                    const int at = stage ? stage - 1 : STAGES - 1;
+                    mbar_wait_spin(bars + 8 * at, stage ? phase : phase ^ 1u);
+                }
+                if (stage-- == 0) { stage = STAGES - 1; phase ^= 1u; }
+            }
     }
     pdl_trigger();                                             // not earlier: what comes behind would only wait in this kernel's place
     // blocks of query rows that see no key
@@ -772,24 +829,24 @@ __global__ void __launch_bounds__(GROUPS * HD) attn_q4_merge_kernel(const AqPara
     }
 }
 
-template <int HD, int NB>
-static size_t aq_desc_bytes(int batch, int Hkv, int R) { return ((size_t)batch * Hkv * ((R + AqShape<HD, NB>::ROWS - 1) / AqShape<HD, NB>::ROWS) * sizeof(int2) + 15) & ~(size_t)15; }
+template <int HD, int BLOCKS>
+static size_t aq_desc_bytes(int batch, int Hkv, int R) { return ((size_t)batch * Hkv * ((R + AqShape<HD, BLOCKS>::ROWS - 1) / AqShape<HD, BLOCKS>::ROWS) * sizeof(int2) + 15) & ~(size_t)15; }
 
-template <int HD, int NB>
+template <int HD, int BLOCKS>
 static int aq_launch(AqParams p, void *ws, cudaStream_t st)
 {
-    using S = AqShape<HD, NB>;
+    using S = AqShape<HD, BLOCKS>;
     static_assert(S::SMEM <= 227 * 1024, "shared memory");
     const int N = ckb_sm_count() * S::CTAS;
     p.RC = (p.R + S::ROWS - 1) / S::ROWS;
     p.desc = (int2 *)ws;
-    p.part = (float *)((uint8_t *)ws + aq_desc_bytes<HD, NB>(p.c.batch, p.c.Hkv, p.R));
+    p.part = (float *)((uint8_t *)ws + aq_desc_bytes<HD, BLOCKS>(p.c.batch, p.c.Hkv, p.R));
     static bool attr_set = false;
     if (!attr_set) {
-        if (ckb_check_cuda((int)cudaFuncSetAttribute(attn_q4_kernel<HD, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "attention_q4cache")) return CKB_ERR_CUDA;
+        if (ckb_check_cuda((int)cudaFuncSetAttribute(attn_q4_kernel<HD, BLOCKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM), "attention_q4cache")) return CKB_ERR_CUDA;
         attr_set = true;
     }
-    const int rc = launch_pdl("attention_q4cache", attn_q4_kernel<HD, NB>, dim3(N), dim3(AQ_THREADS), (size_t)S::SMEM, st, p);
+    const int rc = launch_pdl("attention_q4cache", attn_q4_kernel<HD, BLOCKS>, dim3(N), dim3(AQ_THREADS), (size_t)S::SMEM, st, p);
     if (rc || p.c.stride * p.c.page_tokens <= S::UNIT) return rc;      // no stretch has two units
     // Few stretches are in many parts each, and their CTAs few (64 of 32 parts: 6 us, 18 us with a load at a time); many are in two or three (2048 of them: 4 us, 32 us
     // with the CTAs of the other kind).
@@ -799,28 +856,29 @@ static int aq_launch(AqParams p, void *ws, cudaStream_t st)
     return launch_pdl("attention_q4cache", attn_q4_merge_kernel<HD, 1, 4>, grid, dim3(HD), 0, st, p, S::ROWS);
 }
 
-template <int HD, int NB>
+template <int HD, int BLOCKS>
 static size_t aq_bytes(int batch, int Hkv, int R)
 {
-    using S = AqShape<HD, NB>;
-    return aq_desc_bytes<HD, NB>(batch, Hkv, R) + (size_t)ckb_sm_count() * S::CTAS * 2 * sizeof(float) * S::ROWS * (HD + 2);
+    using S = AqShape<HD, BLOCKS>;
+    return aq_desc_bytes<HD, BLOCKS>(batch, Hkv, R) + (size_t)ckb_sm_count() * S::CTAS * 2 * sizeof(float) * S::ROWS * (HD + 2);
 }
 
-// Blocks of 8 query rows that share the codes a CTA unpacks.  A unit costs 1 : 1.45 : 2.3 with one, two and three (128 channels), so three are worth it only where
-// they hold all the rows: 20 rows of 16 sequences (five drafts, up to 8190 tokens) 119 us with three, 152 us with two and two; 516 rows 55 us in blocks of two, 61 us
-// in blocks of three.
-static int aq_blocks(long long rows, int hd) { return rows <= 8 ? 1 : (rows > 16 && rows <= 24 && hd <= 128 ? 3 : 2); }
+// Blocks of 8 query rows that share the codes a CTA unpacks; 0: up to four, with both pieces of a row in one product (32 heads over 8, four sequences of 131072
+// tokens 188 us, 218 us in a block of 8; 32 of up to 4096 51 and 57).  A unit costs 1 : 1.45 : 2.3 with one, two and three blocks (128 channels), so three are worth
+// it only where they hold all the rows: 20 rows of 16 sequences (five drafts, up to 8190 tokens) 119 us with three, 152 us with two and two; 516 rows 55 us in blocks
+// of two, 61 us in blocks of three.
+static int aq_blocks(long long rows, int hd) { return rows <= 4 ? 0 : rows <= 8 ? 1 : (rows > 16 && rows <= 24 && hd <= 128 ? 3 : 2); }
 
 }  // namespace ckb
 
 using namespace ckb;
 
-#define AQ_EACH(hd, nb, F)                                                          \
-    (hd == 64 ? (nb == 1 ? F<64, 1> : nb == 2 ? F<64, 2> : F<64, 3>)                \
-     : hd == 96 ? (nb == 1 ? F<96, 1> : nb == 2 ? F<96, 2> : F<96, 3>)              \
-     : hd == 128 ? (nb == 1 ? F<128, 1> : nb == 2 ? F<128, 2> : F<128, 3>)          \
-     : hd == 192 ? (nb == 1 ? F<192, 1> : F<192, 2>)                                \
-                 : (nb == 1 ? F<256, 1> : F<256, 2>))
+#define AQ_EACH(hd, nb, F)                                                                                              \
+    (hd == 64 ? (nb == 0 ? F<64, 0> : nb == 1 ? F<64, 1> : nb == 2 ? F<64, 2> : F<64, 3>)                               \
+     : hd == 96 ? (nb == 0 ? F<96, 0> : nb == 1 ? F<96, 1> : nb == 2 ? F<96, 2> : F<96, 3>)                             \
+     : hd == 128 ? (nb == 0 ? F<128, 0> : nb == 1 ? F<128, 1> : nb == 2 ? F<128, 2> : F<128, 3>)                        \
+     : hd == 192 ? (nb == 0 ? F<192, 0> : nb == 1 ? F<192, 1> : F<192, 2>)                                              \
+                 : (nb == 0 ? F<256, 0> : nb == 1 ? F<256, 1> : F<256, 2>))
 
 extern "C" size_t ckb200_attention_q4cache_workspace_bytes(int batch, int num_tokens, int num_heads, int num_kv_heads, int head_dim)
 {
