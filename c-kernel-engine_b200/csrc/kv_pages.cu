@@ -386,6 +386,7 @@ static int check_tables(const char *what, const int *table, int stride, const in
     if (batch < 0 || stride <= 0 || pages <= 0 || page_tokens <= 0) return ckb_fail(CKB_ERR_SHAPE, "%s: batch %d, table columns %d, pages %d of %d tokens", what, batch, stride, pages, page_tokens);
     if (batch > KP_MAX_BATCH) return ckb_fail(CKB_ERR_LIMIT, "%s: %d sequences, at most %d", what, batch, KP_MAX_BATCH);
     if ((long long)stride * page_tokens > 1 << 30 || pages > 1 << 30) return ckb_fail(CKB_ERR_LIMIT, "%s: a sequence may have up to 2^30 tokens, a pool 2^30 pages", what);
+    if ((long long)batch * stride > 0x7fffffffLL) return ckb_fail(CKB_ERR_LIMIT, "%s: a table of %lld entries, at most 2^31 - 1", what, (long long)batch * stride);
     if (((uintptr_t)table | (uintptr_t)lens | (uintptr_t)refs) & 3) return ckb_fail(CKB_ERR_ALIGN, "%s: tables must be aligned to 4 bytes", what);
     if (batch && (!ws || ws_bytes < ckb200_kv_pages_workspace_bytes(batch, stride, pages))) return ckb_fail(CKB_ERR_STATE, "%s: the workspace is too small", what);
     if ((uintptr_t)ws & 15) return ckb_fail(CKB_ERR_ALIGN, "%s: the workspace must be aligned to 16 bytes", what);

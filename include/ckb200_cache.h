@@ -84,7 +84,8 @@ int ckb200_dev_kv_pages_copy(void *pages, int planes, long long plane_stride, lo
  * refused), a larger one makes room for rows to be stored.  First all that shrink give back their pages; then those that grow, in the order of b, get theirs:
  * each the free pages of lowest number, for its new columns in their order.  A growing sequence whose last page has room but is named by others too gets a
  * copy of that page first (the last one that names it keeps it).  Where the free pages do not suffice or the table has too few columns, the sequence
- * stays as it is and status[b] is 1, else 0; later ones may still grow.  batch at most 4096. */
+ * stays as it is and status[b] is 1, else 0; later ones may still grow.
+ * This call and the two below: batch at most 4096, batch * table_stride below 2^31. */
 int ckb200_dev_kv_pages_resize(int *page_table, int table_stride, int *kv_lens, int *page_refs, const int *new_lens, int batch, int num_pages, int page_tokens,
                                void *pages, int planes, long long plane_stride, long long page_bytes, int *status, void *workspace, size_t workspace_bytes, void *stream);
 /* Sequence b becomes what sequence parent[b] was before the call (a parent outside 0 .. batch - 1, or b itself: it stays as it is): its own pages are

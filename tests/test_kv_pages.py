@@ -23,7 +23,7 @@ CHANGES = [(dict(page_table=None), STATE), (dict(kv_lens=None), STATE), (dict(pa
            (dict(page_refs=257), ALIGN), (dict(pages=264), ALIGN), (dict(live=257), ALIGN), (dict(parent=257), ALIGN), (dict(dst=257), ALIGN), (dict(new_lens=258), ALIGN),
            (dict(batch=-1), SHAPE), (dict(count=-1), SHAPE), (dict(table_stride=0), SHAPE), (dict(num_pages=0), SHAPE), (dict(page_tokens=0), SHAPE), (dict(planes=-1), SHAPE),
            (dict(page_bytes=1288), SHAPE), (dict(page_bytes=0), SHAPE), (dict(plane_stride=7 * 1280), SHAPE), (dict(plane_stride=8 * 1280 + 8), SHAPE), (dict(batch=4097), LIMIT),
-           (dict(table_stride=1 << 27), LIMIT)]
+           (dict(table_stride=1 << 27), LIMIT), (dict(table_stride=1 << 26, batch=32), LIMIT)]
 REFUSED = [(name, change, code) for name, args in CALLS.items() for change, code in CHANGES if set(change) <= set(args)]
 
 
