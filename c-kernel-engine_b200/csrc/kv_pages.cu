@@ -13,7 +13,7 @@
 
 namespace ckb {
 
-constexpr int KP_THREADS = 1024, KP_WARPS = KP_THREADS / 32, KP_MAX_BATCH = 4096;
+constexpr int KP_THREADS = 1024, KP_WARPS = KP_THREADS / 32, KP_MAX_BATCH = 4096, KP_KEPT = 32 * 8, KP_LIST = 2048, KP_FORK = 8;
 constexpr int KC_THREADS = 256, KC_UNROLL = 8;
 
 struct KvTables {
@@ -26,34 +26,41 @@ struct KvPool {
     int planes, pages;
 };
 
-// sum over the CTA of the threads before this one; total: of all.  `sh`: KP_WARPS + 1 ints, free again after the call
-__device__ __forceinline__ int kp_before(int v, int *sh, int &total)
+// sums over the CTA of N numbers of the threads before this one; total: of all.  `sh`: N rows of KP_WARPS + 1 ints, free again after the call
+template <int N>
+__device__ __forceinline__ void kp_before(const int (&v)[N], int (&before)[N], int (&total)[N], int (*sh)[KP_WARPS + 1])
 {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int x = v;
+    int x[N];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+    for (int i = 0; i < N; ++i) {
+        x[i] = v[i];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x[i], o);
+            if (lane >= o) x[i] += y;
+        }
+        if (lane == 31) sh[i][warp] = x[i];
     }
-    if (lane == 31) sh[warp] = x;
     __syncthreads();
-    if (warp == 0) {
-        const int w = lane < KP_WARPS ? sh[lane] : 0;
+    if (warp < N) {
+        const int w = lane < KP_WARPS ? sh[warp][lane] : 0;
         int s = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, s, o);
             if (lane >= o) s += y;
         }
-        sh[lane] = s - w;
-        if (lane == 31) sh[KP_WARPS] = s;
+        sh[warp][lane] = s - w;
+        if (lane == 31) sh[warp][KP_WARPS] = s;
     }
     __syncthreads();
-    const int before = sh[warp] + x - v;
-    total = sh[KP_WARPS];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        before[i] = sh[i][warp] + x[i] - v[i];
+        total[i] = sh[i][KP_WARPS];
+    }
     __syncthreads();
-    return before;
 }
 
 // A warp's stretch [lo, hi) of the reference counts, and which of them are zero: up to 256 pages as bits that stay in registers, a longer stretch is read again
@@ -62,19 +69,28 @@ struct KpStretch {
     int lo, hi;
     uint32_t free_bits[8];
 };
+__device__ __forceinline__ void kp_load(const int *refs, int p0, int hi, int (&ref)[8])
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ref[i] = p0 + 32 * i + (threadIdx.x & 31) < hi ? __ldcg(refs + p0 + 32 * i + (threadIdx.x & 31)) : 1;
+}
+__device__ __forceinline__ int kp_bits(const int (&ref)[8], uint32_t (&bits)[8])
+{
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        bits[i] = __ballot_sync(0xffffffffu, ref[i] == 0);
+        n += __popc(bits[i]);
+    }
+    return n;
+}
 __device__ __forceinline__ int kp_count_free(const int *refs, KpStretch &s)
 {
-    const int lane = threadIdx.x & 31;
     int n = 0;
-    for (int p0 = s.lo; p0 < s.hi; p0 += 32 * 8) {
+    for (int p0 = s.lo; p0 < s.hi; p0 += KP_KEPT) {
         int ref[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ref[i] = p0 + 32 * i + lane < s.hi ? __ldcg(refs + p0 + 32 * i + lane) : 1;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            s.free_bits[i] = __ballot_sync(0xffffffffu, ref[i] == 0);
-            n += __popc(s.free_bits[i]);
-        }
+        kp_load(refs, p0, s.hi, ref);
+        n += kp_bits(ref, s.free_bits);
     }
     return n;
 }
@@ -82,18 +98,16 @@ __device__ __forceinline__ int kp_count_free(const int *refs, KpStretch &s)
 __device__ __forceinline__ void kp_list(const int *refs, const KpStretch &s, int lo, int hi, bool in_use, int *list, int at, int most)
 {
     const int lane = threadIdx.x & 31;
-    const bool kept = s.hi - s.lo <= 32 * 8;
-    for (int p0 = s.lo; p0 < hi && at < most; p0 += 32 * 8) {
+    const bool kept = s.hi - s.lo <= KP_KEPT;
+    for (int p0 = s.lo; p0 < hi && at < most; p0 += KP_KEPT) {
         uint32_t bits[8];
         if (kept) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) bits[i] = s.free_bits[i];
         } else {
             int ref[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) ref[i] = p0 + 32 * i + lane < hi ? __ldcg(refs + p0 + 32 * i + lane) : 1;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) bits[i] = __ballot_sync(0xffffffffu, ref[i] == 0);
+            kp_load(refs, p0, hi, ref);
+            kp_bits(ref, bits);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -165,28 +179,30 @@ __global__ void __launch_bounds__(KC_THREADS) kv_pages_copy_kernel(KvPool pool, 
 
 // ---------------------------------------------------------------- resize
 
-// ws: [0] number of pages to copy, [4 ..) their sources, [4 + batch ..) their copies, [4 + 2 batch ..) free pages
+// ws: [0] number of pages to copy, [4 ..) their sources, [4 + batch ..) their copies, [4 + 2 batch ..) free pages where they are more than KP_LIST
 __global__ void __launch_bounds__(KP_THREADS) kv_pages_resize_kernel(KvTables t, const int *__restrict__ new_lens, int *__restrict__ status, int *__restrict__ ws)
 {
     extern __shared__ int kp_sm[];
-    __shared__ int sh[KP_WARPS + 1], s_copies, s_slow;
+    __shared__ int sh[3][KP_WARPS + 1], s_copies, s_slow, list_s[KP_LIST];
     const int B = t.batch, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pt = t.page_tokens;
     // for each sequence: its length now and then, the shared page that it would write into (-1: none), pages wanted (-1: stays as it is), where its pages begin in the list
     int *len_s = kp_sm, *new_s = len_s + B, *part_s = new_s + B, *want_s = part_s + B, *first_s = want_s + B, *cow_s = first_s + B;
-    int *src = ws + 4, *dst = src + B, *list = dst + B;
+    int *src = ws + 4, *dst = src + B;
     pdl_trigger();
     if (threadIdx.x == 0) s_slow = 0;
+    int shrinks = 0;
     for (int b = threadIdx.x; b < B; b += KP_THREADS) {
         const int len = kv_len(t.lens[b], t.stride, pt);
         int nl = new_lens[b], bad = 0;
         if (nl > t.stride * pt) { nl = -1; bad = 1; }
         len_s[b] = len;
-        new_s[b] = nl < 0 ? len : nl;
+        new_s[b] = nl = nl < 0 ? len : nl;
         status[b] = bad;
+        shrinks |= nl < len;
     }
-    __syncthreads();
+    shrinks = __syncthreads_or(shrinks);
     // those that shrink give back their pages
-    for (int b = warp; b < B; b += KP_WARPS) {
+    for (int b = warp; shrinks && b < B; b += KP_WARPS) {
         const int have = kv_columns(len_s[b], pt), need = kv_columns(new_s[b], pt);
         int *row = t.table + (size_t)b * t.stride;
         for (int i = need + lane; i < have; i += 32) {
@@ -195,9 +211,12 @@ __global__ void __launch_bounds__(KP_THREADS) kv_pages_resize_kernel(KvTables t,
             row[i] = -1;
         }
     }
-    __syncthreads();
-    // those that grow: is the page that the next row goes into shared?
-    int shares = 0;
+    if (shrinks) __syncthreads();
+    // those that grow: is the page that the next row goes into shared?  Meanwhile the counts of a pool of up to 8192 pages are on their way
+    KpStretch pages = kp_stretch(t.pages);
+    const bool kept = t.pages <= KP_WARPS * KP_KEPT;
+    int ref[8], shares = 0;
+    if (kept) kp_load(t.refs, pages.lo, pages.hi, ref);
     for (int b = threadIdx.x; b < B; b += KP_THREADS) {
         int page = -1;
         if (new_s[b] > len_s[b] && len_s[b] % pt) {
@@ -223,21 +242,32 @@ __global__ void __launch_bounds__(KP_THREADS) kv_pages_resize_kernel(KvTables t,
         mine += max(0, want_s[b]);
         copies += cow;
     }
-    int total, total_copies;
-    int at = kp_before(mine, sh, total);
-    int cat = kp_before(copies, sh, total_copies);
+    // the first page of the list that is this thread's, its first copy, its warp's first free page
+    int sums[3] = {mine, copies, 0}, before[3], all[3];
+    if (kept) {
+        const int n = kp_bits(ref, pages.free_bits);
+        if (lane == 0) sums[2] = n;
+    }
+    kp_before(sums, before, all, sh);
+    const int total = all[0];
+    int at = before[0], cat = before[1];
     for (int b = b0; b < b1; ++b) {
         first_s[b] = at;
         at += max(0, want_s[b]);
         if (cow_s[b]) cow_s[b] = 1 + cat++;                     // 1 + its place in the list of copies
     }
-    if (threadIdx.x == 0) s_copies = total_copies;
-    __syncthreads();
+    if (threadIdx.x == 0) s_copies = all[1];
+    int *list = total <= KP_LIST ? list_s : dst + B;
     if (total > 0) {
-        KpStretch pages = kp_stretch(t.pages);
-        const int n = kp_count_free(t.refs, pages);
-        int have_free;
-        const int before = kp_before(lane == 0 ? n : 0, sh, have_free);
+        if (!kept) {
+            const int n = kp_count_free(t.refs, pages), mine_free[1] = {lane == 0 ? n : 0};
+            int at_free[1], all_free[1];
+            kp_before(mine_free, at_free, all_free, sh);
+            before[2] = at_free[0];
+            all[2] = all_free[0];
+        }
+        const int have_free = all[2];
+        if (have_free < total) __syncthreads();                 // what the threads have written about the sequences
         if (have_free < total) {                                // one by one: who finds no room leaves its claim to those behind
             if (threadIdx.x == 0) {
                 int used = 0, nc = 0;
@@ -267,10 +297,10 @@ __global__ void __launch_bounds__(KP_THREADS) kv_pages_resize_kernel(KvTables t,
             }
         }
         // the free pages themselves; a page whose count the loop above took down was shared before and still has a holder
-        const int base = __shfl_sync(0xffffffffu, before, 0);
+        const int base = __shfl_sync(0xffffffffu, before[2], 0);
         kp_list(t.refs, pages, pages.lo, pages.hi, false, list, base, min(total, have_free));
-        __syncthreads();
     }
+    __syncthreads();
     for (int b = warp; b < B; b += KP_WARPS) {
         int *row = t.table + (size_t)b * t.stride;
         if (want_s[b] > 0) {
@@ -332,31 +362,75 @@ __global__ void __launch_bounds__(128) kv_pages_fork_write_kernel(KvTables t, co
     if (threadIdx.x == 0) t.lens[b] = len;
 }
 
+// Tables of up to KP_THREADS * KP_FORK entries, by one CTA that holds what every entry was: 2.8 us, where the two kernels above take 2.3 us each
+__global__ void __launch_bounds__(KP_THREADS) kv_pages_fork_kernel(KvTables t, const int *__restrict__ parent)
+{
+    extern __shared__ int kp_sm[];
+    int *len_s = kp_sm, *parent_s = len_s + t.batch;            // a parent: -1 for none
+    for (int b = threadIdx.x; b < t.batch; b += KP_THREADS) {
+        const int from = parent[b];
+        len_s[b] = kv_len(t.lens[b], t.stride, t.page_tokens);
+        parent_s[b] = from < 0 || from >= t.batch || from == b ? -1 : from;
+    }
+    __syncthreads();
+    int now[KP_FORK], next[KP_FORK];                            // -1: no page; -2: stays as it is
+#pragma unroll
+    for (int u = 0; u < KP_FORK; ++u) {
+        const int x = threadIdx.x + u * KP_THREADS, b = x / t.stride, i = x - b * t.stride;
+        now[u] = -1;
+        next[u] = -2;
+        if (b >= t.batch || parent_s[b] < 0) continue;
+        const int had = kv_columns(len_s[b], t.page_tokens), n = kv_columns(len_s[parent_s[b]], t.page_tokens);
+        if (i < had) now[u] = t.table[x];
+        if (i < n) next[u] = t.table[parent_s[b] * t.stride + i];
+        else if (i < had) next[u] = -1;
+        if (i < n) next[u] = max(-1, next[u]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < KP_FORK; ++u) {
+        if (next[u] == -2) continue;
+        const int to = kv_entry(next[u], t.pages), old = kv_entry(now[u], t.pages);
+        if (to >= 0) atomicAdd(t.refs + to, 1);
+        if (old >= 0) atomicSub(t.refs + old, 1);
+        t.table[threadIdx.x + u * KP_THREADS] = to;
+    }
+    for (int b = threadIdx.x; b < t.batch; b += KP_THREADS)
+        if (parent_s[b] >= 0) t.lens[b] = len_s[parent_s[b]];
+}
+
 // ---------------------------------------------------------------- compact
 
 // ws: [0] pages that move, [1] pages in use, [4 ..) which, [4 + pages ..) where to, [4 + 2 pages ..) for each page from [1] on: where it goes or -1
 __global__ void __launch_bounds__(KP_THREADS) kv_pages_plan_kernel(KvTables t, int *__restrict__ live_out, int *__restrict__ ws)
 {
-    __shared__ int sh[KP_WARPS + 1];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ int sh[2][KP_WARPS + 1], src_s[KP_LIST], dst_s[KP_LIST];
+    const int lane = threadIdx.x & 31;
     int *src = ws + 4, *dst = src + t.pages, *place = dst + t.pages;
     pdl_trigger();
     KpStretch pages = kp_stretch(t.pages);
     const int lo = pages.lo, hi = pages.hi, n = kp_count_free(t.refs, pages);
-    int free_all;
-    kp_before(lane == 0 ? n : 0, sh, free_all);
-    const int live = t.pages - free_all, cut = min(hi, max(lo, live));
+    const int free_here[1] = {lane == 0 ? n : 0};
+    int free_before[1], free_all[1];
+    kp_before(free_here, free_before, free_all, sh);
+    const int live = t.pages - free_all[0], cut = min(hi, max(lo, live));
     // free ones below `live`, used ones from there on: as many of the one kind as of the other
     const int holes = cut == hi ? n : (cut == lo ? 0 : kp_free_below(t.refs, pages, cut)), movers = (hi - cut) - (n - holes);
-    int count, same;
-    const int hole0 = __shfl_sync(0xffffffffu, kp_before(lane == 0 ? holes : 0, sh, count), 0);
-    const int mover0 = __shfl_sync(0xffffffffu, kp_before(lane == 0 ? movers : 0, sh, same), 0);
-    kp_list(t.refs, pages, lo, cut, false, dst, hole0, count);
-    kp_list(t.refs, pages, cut, hi, true, src, mover0, count);
+    const int sums[2] = {lane == 0 ? holes : 0, lane == 0 ? movers : 0};
+    int before[2], all[2];
+    kp_before(sums, before, all, sh);
+    const int count = all[0];
+    const bool near = count <= KP_LIST;                         // the lists are read back from shared memory
+    kp_list(t.refs, pages, lo, cut, false, near ? dst_s : dst, __shfl_sync(0xffffffffu, before[0], 0), count);
+    kp_list(t.refs, pages, cut, hi, true, near ? src_s : src, __shfl_sync(0xffffffffu, before[1], 0), count);
     for (int p = cut + lane; p < hi; p += 32) place[p] = -1;
     __syncthreads();
     for (int i = threadIdx.x; i < count; i += KP_THREADS) {
-        const int s = src[i], d = dst[i];
+        const int s = near ? src_s[i] : src[i], d = near ? dst_s[i] : dst[i];
+        if (near) {
+            src[i] = s;
+            dst[i] = d;
+        }
         place[s] = d;
         t.refs[d] = t.refs[s];
         t.refs[s] = 0;
@@ -386,6 +460,7 @@ static int check_tables(const char *what, const int *table, int stride, const in
     if (batch < 0 || stride <= 0 || pages <= 0 || page_tokens <= 0) return ckb_fail(CKB_ERR_SHAPE, "%s: batch %d, table columns %d, pages %d of %d tokens", what, batch, stride, pages, page_tokens);
     if (batch > KP_MAX_BATCH) return ckb_fail(CKB_ERR_LIMIT, "%s: %d sequences, at most %d", what, batch, KP_MAX_BATCH);
     if ((long long)stride * page_tokens > 1 << 30 || pages > 1 << 30) return ckb_fail(CKB_ERR_LIMIT, "%s: a sequence may have up to 2^30 tokens, a pool 2^30 pages", what);
+    if ((long long)batch * stride > 0x7fffffffLL) return ckb_fail(CKB_ERR_LIMIT, "%s: a table of %lld entries, at most 2^31 - 1", what, (long long)batch * stride);
     if ((long long)batch * stride > 0x7fffffffLL) return ckb_fail(CKB_ERR_LIMIT, "%s: a table of %lld entries, at most 2^31 - 1", what, (long long)batch * stride);
     if (((uintptr_t)table | (uintptr_t)lens | (uintptr_t)refs) & 3) return ckb_fail(CKB_ERR_ALIGN, "%s: tables must be aligned to 4 bytes", what);
     if (batch && (!ws || ws_bytes < ckb200_kv_pages_workspace_bytes(batch, stride, pages))) return ckb_fail(CKB_ERR_STATE, "%s: the workspace is too small", what);
@@ -461,6 +536,10 @@ extern "C" int ckb200_dev_kv_pages_fork(int *page_table, int table_stride, int *
     if ((rc = ckb_check_device(what))) return rc;
     const KvTables t = {page_table, kv_lens, page_refs, table_stride, batch, num_pages, page_tokens};
     cudaStream_t st = ckb_stream(stream);
+    if ((long long)batch * table_stride <= KP_THREADS * KP_FORK) {
+        kv_pages_fork_kernel<<<1, KP_THREADS, 2 * sizeof(int) * (size_t)batch, st>>>(t, parent);
+        return ckb_check_launch(what);
+    }
     kv_pages_fork_read_kernel<<<batch, 128, 0, st>>>(t, parent, (int *)workspace);
     if ((rc = ckb_check_launch(what))) return rc;
     return launch_pdl(what, kv_pages_fork_write_kernel, dim3(batch), dim3(128), 0, st, t, (const int *)workspace);

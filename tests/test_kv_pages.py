@@ -94,7 +94,8 @@ def make(lib, rng, batch, stride, pages, page_tokens, planes=3, page_bytes=160, 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("batch,stride,pages,page_tokens,planes,page_bytes", [(1, 1, 1, 16, 1, 16), (3, 4, 9, 16, 2, 320), (8, 6, 40, 16, 3, 5120), (33, 5, 90, 48, 1, 4112), (70, 9, 500, 16, 2, 160),
-                                                                             (5, 300, 12, 16, 1, 32), (1100, 3, 2100, 16, 1, 16), (6, 5, 31, 64, 160, 2560), (4, 3, 12, 16, 0, 0)])
+                                                                             (5, 300, 12, 16, 1, 32), (1100, 3, 2100, 16, 1, 16), (6, 5, 31, 64, 160, 2560), (4, 3, 12, 16, 0, 0),
+                                                                             (310, 28, 9000, 16, 1, 16), (128, 64, 700, 16, 1, 16), (4096, 2, 4500, 16, 1, 16)])
 def test_any_order_of_calls(gpu, batch, stride, pages, page_tokens, planes, page_bytes):  # noqa: F811
     """Grown, shrunk, freed, forked onto one another, compacted, with too little room now and then: after each call everything is what the host's walk gives."""
     rng = np.random.default_rng(batch * 7 + pages)
@@ -172,6 +173,22 @@ def test_many_pages(gpu):  # noqa: F811
     d.compact()
     d.same()
     assert int(d.live) == live > 20000
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pages", [8192, 8193])
+@pytest.mark.parametrize("columns", [512, 513])
+def test_thousands_at_once(gpu, pages, columns):  # noqa: F811
+    """2048 pages and some more wanted by one call, forked, then as many moved by one compaction."""
+    m, d = make(gpu, np.random.default_rng(7), 8, 1040, pages, 16, planes=1, page_bytes=16)
+    for call, arg in (("resize", [16 * columns] * 4 + [0] * 4), ("resize", [-1] * 4 + [16 * columns] * 4), ("fork", [-1, -1, -1, -1, 5, -1, -1, 0]), ("resize", [0] * 4 + [16 * columns + 1] * 4)):
+        getattr(m, call)(arg)
+        getattr(d, call)(arg)
+        d.same()
+    live = m.compact()
+    d.compact()
+    d.same()
+    assert int(d.live) == live
 
 
 @pytest.mark.gpu
