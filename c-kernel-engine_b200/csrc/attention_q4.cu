@@ -337,15 +337,21 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
             // ---- a stretch: query fragments of its rows
             const int r0 = w.rc * ROWS, u_first = w.u;
             __syncthreads();                                   // the stretch before is done with them
-            for (int r = warp; r < ROWS; r += AQ_WARPS) {      // a warp per row, a lane the channels 4 (lane % 4 ..) of its blocks
-                float x[G4], top = 0.0f;
-                const int row = r0 + r, tok = row / p.G;
+            float qx[(ROWS + AQ_WARPS - 1) / AQ_WARPS][G4];    // all on their way before the first is used
+#pragma unroll
+            for (int i = 0; i < (ROWS + AQ_WARPS - 1) / AQ_WARPS; ++i) {
+                const int row = r0 + warp + i * AQ_WARPS, tok = row / p.G;
                 const float *src = p.q + ((long long)w.b * p.c.tokens + tok) * p.q_stride + (long long)(w.h * p.G + row - tok * p.G) * HD;
 #pragma unroll
-                for (int j = 0; j < G4; ++j) {
-                    x[j] = row < p.R ? __ldcg(src + 32 * j + lane) : 0.0f;
-                    top = fmaxf(top, fabsf(x[j]));
-                }
+                for (int j = 0; j < G4; ++j) qx[i][j] = row < p.R ? __ldcg(src + 32 * j + lane) : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < (ROWS + AQ_WARPS - 1) / AQ_WARPS; ++i) {      // a warp per row, a lane the channels 4 (lane % 4 ..) of its blocks
+                const int r = warp + i * AQ_WARPS;
+                const float (&x)[G4] = qx[i];
+                float top = 0.0f;
+#pragma unroll
+                for (int j = 0; j < G4; ++j) top = fmaxf(top, fabsf(x[j]));
                 const int ex_top = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23);      // biased exponent of the row's largest
                 const int sh = max(-126, min(126, 141 - ex_top));                                           // largest into [2^14, 2^15)
                 const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
