@@ -67,11 +67,11 @@ struct AqParams {
     float *out;
     long long q_stride, out_stride;
     KvQ4 c;
-    int H, G, R, RC, window, *err;             // G heads a kv head, R = tokens * G query rows a kv head, RC blocks of them
+    int G, R, RC, window, *err;                // G heads a kv head, R = tokens * G query rows a kv head, RC blocks of them
     float scale;
-    uint32_t page_mul, page_shift;             // position / page_tokens = (position * page_mul >> 32) >> page_shift
+    KvDivide by_page, by_group;                // by page_tokens and by G
     int2 *desc;                                // [batch][Hkv][RC]: the first and the last CTA of a stretch that several work on; last < 0: one did
-    float *part;                               // [2 CTAs][8 NB][HD + 2]: the stretch that began before the CTA, the one that goes on after it
+    float *part;                               // [2 CTAs][ROWS][HD + 2]: the stretch that began before the CTA, the one that goes on after it
 };
 
 // where a CTA is on the line of units
@@ -81,28 +81,30 @@ struct AqWalk {
 // tokens r0 / G .. of block rc: the keys that any of them sees
 __device__ __forceinline__ void aq_range(const AqParams &p, int nrows, int unit, AqWalk &w)
 {
-    const int t0 = w.rc * nrows / p.G, t1 = (min(p.R, (w.rc + 1) * nrows) - 1) / p.G, at = w.len - p.c.tokens;
+    const int t0 = p.by_group(w.rc * nrows), t1 = p.by_group(min(p.R, (w.rc + 1) * nrows) - 1), at = w.len - p.c.tokens;
     w.end = max(0, at + t1 + 1);
     w.begin = p.window > 0 ? max(0, at + t0 - p.window + 1) & ~31 : 0;      // a chunk's beginning
     w.n = w.end > w.begin ? (w.end - w.begin + unit - 1) / unit : 0;
 }
 __device__ __forceinline__ int aq_length(const AqParams &p, int b) { return kv_len(__ldcg(p.c.lens + b), p.c.stride, p.c.page_tokens); }
-// the next stretch that has units; its first one.  False: there is none
-__device__ __forceinline__ bool aq_next_stretch(const AqParams &p, int nrows, int unit, AqWalk &w)
+// the next block of rows
+__device__ __forceinline__ void aq_next_block(const AqParams &p, int nrows, int unit, AqWalk &w)
+{
+    if (++w.rc == p.RC) {
+        w.rc = 0;
+        ++w.b;
+        w.len = w.b < p.c.batch ? aq_length(p, w.b) : 0;
+    }
+    aq_range(p, nrows, unit, w);
+}
+// the first unit of the next stretch that has units, if there is one
+__device__ __forceinline__ void aq_next_stretch(const AqParams &p, int nrows, int unit, AqWalk &w)
 {
     w.u = 0;
-    for (;;) {
-        if (++w.rc == p.RC) {
-            w.rc = 0;
-            if (++w.h == p.c.Hkv) {
-                w.h = 0;
-                if (++w.b >= p.c.batch) return false;
-                w.len = aq_length(p, w.b);
-            }
-        }
-        aq_range(p, nrows, unit, w);
-        if (w.n) return true;
-    }
+    if (++w.h < p.c.Hkv) return;
+    w.h = 0;
+    do aq_next_block(p, nrows, unit, w);
+    while (w.n == 0 && w.b < p.c.batch);
 }
 
 __device__ __forceinline__ void aq_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
@@ -179,8 +181,8 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
     extern __shared__ __align__(128) uint8_t aq_smem[];
     __shared__ __align__(8) uint64_t full[AQ_WARPS][STAGES];
     __shared__ int pieces[AQ_WARPS][STAGES];
-    __shared__ long long s_sum[AQ_WARPS], s_rest;
-    __shared__ int s_b;
+    __shared__ long long s_sum[AQ_WARPS];
+    __shared__ AqWalk s_walk;
     uint4 *qf = reinterpret_cast<uint4 *>(aq_smem + S::RING);                     // [NB][KS][lane] {hi b0, hi b1, lo b0, lo b1}; PACK: [KS][lane] {b0, b1}
     const uint2 *qf2 = reinterpret_cast<const uint2 *>(qf);
     uint2 *qsum = reinterpret_cast<uint2 *>(aq_smem + S::RING + S::QF);           // [NB][lane] {hi, lo} sums of the scaled query over blocks 2t and 2t + 1, times 2^-6: both in fp16's normal range
@@ -199,21 +201,26 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
     }
     pdl_wait();                                                // lengths, table, rows and cache come from the kernels before this one: read through L2
 
-    // ---- this CTA's part of the line: units of all sequences are counted, each thread some consecutive ones
-    const int each = (p.c.batch + AQ_THREADS - 1) / AQ_THREADS, b0 = min(p.c.batch, tid * each), b1 = min(p.c.batch, b0 + each);
-    auto units_of = [&](int b) {
-        AqWalk w;
-        w.b = b;
-        w.len = aq_length(p, b);
-        long long n = 0;
-        for (w.rc = 0; w.rc < p.RC; ++w.rc) {
-            aq_range(p, ROWS, S::UNIT, w);
-            n += w.n;
-        }
-        return n * p.c.Hkv;
+    // ---- this CTA's part of the line.  On it lie the sequences, their blocks of rows, for each its stretches of the kv heads; each thread counts the units of
+    // some consecutive blocks.
+    const int blocks = p.c.batch * p.RC, each = (blocks + AQ_THREADS - 1) / AQ_THREADS, x0 = min(blocks, tid * each), x1 = min(blocks, x0 + each);
+    auto at_block = [&](int x, AqWalk &w) {
+        w.b = x / p.RC;
+        w.rc = x - w.b * p.RC;
+        w.len = aq_length(p, w.b);
+        aq_range(p, ROWS, S::UNIT, w);
     };
     long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += units_of(b);
+    if (x0 < x1) {
+        AqWalk w;
+        at_block(x0, w);
+        mine = w.n;
+        for (int x = x0 + 1; x < x1; ++x) {
+            aq_next_block(p, ROWS, S::UNIT, w);
+            mine += w.n;
+        }
+        mine *= p.c.Hkv;
+    }
     long long before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -241,35 +248,16 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
     }
     if (first < last && mine && before <= first && first < before + mine) {
         long long rest = first - before;
-        int b = b0;
-        for (;; ++b) {
-            const long long n = units_of(b);
-            if (rest < n) break;
-            rest -= n;
-        }
-        s_b = b;
-        s_rest = rest;
+        AqWalk w;
+        for (at_block(x0, w); rest >= (long long)w.n * p.c.Hkv; aq_next_block(p, ROWS, S::UNIT, w)) rest -= (long long)w.n * p.c.Hkv;
+        w.h = rest >> 31 ? (int)(rest / w.n) : (int)((uint32_t)rest / (uint32_t)w.n);
+        w.u = (int)(rest - (long long)w.h * w.n);
+        s_walk = w;
     }
     __syncthreads();
     bool ok = true;
     if (first < last) {
-        AqWalk w;                                              // the unit being computed
-        w.b = s_b;
-        w.len = aq_length(p, w.b);
-        {
-            long long rest = s_rest, per_head = 0;
-            for (w.rc = 0; w.rc < p.RC; ++w.rc) {
-                aq_range(p, ROWS, S::UNIT, w);
-                per_head += w.n;
-            }
-            for (w.h = 0; rest >= per_head; ++w.h) rest -= per_head;
-            for (w.rc = 0;; ++w.rc) {
-                aq_range(p, ROWS, S::UNIT, w);
-                if (rest < w.n) break;
-                rest -= w.n;
-            }
-            w.u = (int)rest;
-        }
+        AqWalk w = s_walk;                                     // the unit being computed
         // Lane 0 fetches, up to STAGES - 1 units ahead: the table's entry for a chunk's beginning is read one chunk ahead.  A chunk that cannot span pages is one copy
         // of K rows and one of V rows, another one as many as it has pieces of 16.  What stays the same in a stretch is worked out once for it.
         AqWalk f = w;
@@ -280,7 +268,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
         const uint32_t page_bytes = (uint32_t)kv_row(1, 0, 0, p.c.Hkv, p.c.page_tokens, G4), ring = smem_u32(aq_smem) + warp * STAGES * S::STAGE, bars = smem_u32(&full[warp][0]);
         auto look = [&](int pos, int &slot) {                  // the page of a position, and its place in it
             if (pos >= f.end) return -1;
-            const int column = (int)(__umulhi((uint32_t)pos, p.page_mul) >> p.page_shift);
+            const int column = p.by_page(pos);
             slot = pos - column * p.c.page_tokens;
             return kv_entry(__ldcg(f_table + column), p.c.pages);
         };
@@ -340,7 +328,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
             float qx[(ROWS + AQ_WARPS - 1) / AQ_WARPS][G4];    // all on their way before the first is used
 #pragma unroll
             for (int i = 0; i < (ROWS + AQ_WARPS - 1) / AQ_WARPS; ++i) {
-                const int row = r0 + warp + i * AQ_WARPS, tok = row / p.G;
+                const int row = r0 + warp + i * AQ_WARPS, tok = p.by_group(row);
                 const float *src = p.q + ((long long)w.b * p.c.tokens + tok) * p.q_stride + (long long)(w.h * p.G + row - tok * p.G) * HD;
 #pragma unroll
                 for (int j = 0; j < G4; ++j) qx[i][j] = row < p.R ? __ldcg(src + 32 * j + lane) : 0.0f;
@@ -388,7 +376,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 const int row = r0 + 8 * nb + g_row;
-                pos_row[nb] = row < p.R ? w.len - p.c.tokens + row / p.G : -1;
+                pos_row[nb] = row < p.R ? w.len - p.c.tokens + p.by_group(row) : -1;
                 fac[nb] = q_factor[8 * nb + g_row];
                 m_run[nb] = -INFINITY;
                 l_run[nb] = 0.0f;
@@ -397,7 +385,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                 for (int e = 0; e < G4 * 8; ++e) o[nb][e >> 3][e >> 2 & 1][e & 3] = 0.0f;
             }
             // chunks in [all_from, all_to) are seen by every row
-            const int pos_first = w.len - p.c.tokens + r0 / p.G, pos_last = w.len - p.c.tokens + (min(p.R, r0 + ROWS) - 1) / p.G;
+            const int pos_first = w.len - p.c.tokens + p.by_group(r0), pos_last = w.len - p.c.tokens + p.by_group(min(p.R, r0 + ROWS) - 1);
             const int all_to = pos_first + 1, all_from = p.window > 0 ? pos_last - p.window + 1 : 0;
 
             for (int key0 = w.begin + w.u * S::UNIT + warp * S::CHUNK;; key0 += S::UNIT) {
@@ -725,7 +713,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const int r = 8 * nb + 2 * t + e, row = r0 + r, tok = row / p.G;
+                        const int r = 8 * nb + 2 * t + e, row = r0 + r, tok = p.by_group(row);
                         const float l = __shfl_sync(0xffffffffu, l_run[nb], 8 * t + 4 * e);
                         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                         if (r >= ROWS || row >= p.R) continue;
@@ -760,10 +748,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
     // blocks of query rows that see no key
     for (int x = me; x < p.c.batch * p.RC; x += N) {
         AqWalk w;
-        w.b = x / p.RC;
-        w.rc = x - w.b * p.RC;
-        w.len = aq_length(p, w.b);
-        aq_range(p, ROWS, S::UNIT, w);
+        at_block(x, w);
         if (w.n) continue;
         for (int h = tid; h < p.c.Hkv; h += AQ_THREADS) p.desc[((size_t)w.b * p.c.Hkv + h) * p.RC + w.rc] = make_int2(me, -1);
         const int r0 = w.rc * ROWS, rows = min(p.R, r0 + ROWS) - r0;
@@ -922,15 +907,13 @@ extern "C" int ckb200_dev_attention_q4cache(const float *q, long long q_stride, 
     p.q_stride = q_stride;
     p.out_stride = out_stride;
     p.c = {page_table, kv_lens, table_stride, batch, num_tokens, num_pages, page_tokens, num_kv_heads, head_dim / 32};
-    p.H = num_heads;
     p.G = num_heads / num_kv_heads;
     p.R = num_tokens * p.G;
     p.window = sliding_window < 1 << 30 ? sliding_window : 0;      // no sequence is longer
     p.scale = 1.0f / sqrtf((float)head_dim);
     p.err = ckb_device_error_word();
-    p.page_shift = 3;                                          // 2^(page_shift + 1) >= page_tokens >= 16: exact for positions below 2^31
-    while (2u << p.page_shift < (uint32_t)page_tokens) ++p.page_shift;
-    p.page_mul = (uint32_t)((((uint64_t)1 << (32 + p.page_shift)) + page_tokens - 1) / page_tokens);
+    p.by_page = kv_divide((uint32_t)page_tokens);
+    p.by_group = kv_divide((uint32_t)p.G);
     const int nb = aq_blocks(p.R, head_dim);
     return AQ_EACH(head_dim, nb, aq_launch)(p, workspace, ckb_stream(stream));
 }

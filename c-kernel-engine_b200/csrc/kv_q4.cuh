@@ -32,6 +32,21 @@ __host__ __device__ __forceinline__ size_t kv_row(int page, int head, int slot, 
     return (((size_t)page * Hkv + head) * page_tokens + slot) * (size_t)(nb * KQ4_BLOCK);
 }
 
+// n / d by a multiplication, n below 2^31
+struct KvDivide {
+    uint32_t d, mul, shift;
+    __device__ __forceinline__ int operator()(uint32_t n) const { return (int)(d == 1 ? n : __umulhi(n, mul) >> shift); }
+};
+inline KvDivide kv_divide(uint32_t d)
+{
+    KvDivide x = {d, 0, 0};
+    if (d > 1) {
+        while (2u << x.shift < d) ++x.shift;                   // 2^shift < d <= 2^(shift + 1)
+        x.mul = (uint32_t)((((uint64_t)1 << (32 + x.shift)) + d - 1) / d);
+    }
+    return x;
+}
+
 }  // namespace ckb
 
 #ifdef __cplusplus

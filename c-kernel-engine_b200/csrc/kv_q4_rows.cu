@@ -69,16 +69,11 @@ __device__ __forceinline__ void kr_store4(float *p, const float4 &v)
     }
 }
 
-// n / d and n % d by a multiplication, n below 2^31
-struct KrDivide {
-    uint32_t d, mul, shift;
-    __device__ __forceinline__ int operator()(uint32_t n) const { return (int)(d == 1 ? n : __umulhi(n, mul) >> shift); }
-};
 struct KrRows {
     KvQ4 c;
     long long k_stride, v_stride;
     uint32_t groups;                           // blocks of 32 values of all rows
-    KrDivide by_items, by_tokens, by_nb, by_page;
+    KvDivide by_items, by_tokens, by_nb, by_page;
 };
 
 // where block `grp` of all rows lies: its row's number, its place in the row, and its place in the pools in bytes (-1: nowhere)
@@ -263,21 +258,12 @@ static int check_rows(const char *what, const float *k, const float *v, long lon
 
 static bool rows_vectors(const float *k, const float *v, long long ks, long long vs) { return !(((uintptr_t)k | (uintptr_t)v) & 15) && !((ks | vs) & 3); }
 
-static KrDivide kr_divide(uint32_t d)
-{
-    KrDivide x = {d, 0, 0};
-    if (d > 1) {
-        while (2u << x.shift < d) ++x.shift;                   // 2^shift < d <= 2^(shift + 1)
-        x.mul = (uint32_t)((((uint64_t)1 << (32 + x.shift)) + d - 1) / d);
-    }
-    return x;
-}
 // 0 and the launch's parameters, or an error
 static int rows_params(const char *what, const KvQ4 &c, long long rows, long long ks, long long vs, KrRows *p, unsigned *grid)
 {
     const long long groups = rows * c.Hkv * c.nb;
     if (groups > 0x7fffffffLL) return ckb_fail(CKB_ERR_LIMIT, "%s: %lld rows in one call", what, rows);
-    *p = {c, ks, vs, (uint32_t)groups, kr_divide((uint32_t)(c.Hkv * c.nb)), kr_divide((uint32_t)(c.tokens > 0 ? c.tokens : 1)), kr_divide((uint32_t)c.nb), kr_divide((uint32_t)c.page_tokens)};
+    *p = {c, ks, vs, (uint32_t)groups, kv_divide((uint32_t)(c.Hkv * c.nb)), kv_divide((uint32_t)(c.tokens > 0 ? c.tokens : 1)), kv_divide((uint32_t)c.nb), kv_divide((uint32_t)c.page_tokens)};
     *grid = (unsigned)((groups + KR_THREADS / 4 - 1) / (KR_THREADS / 4));
     return 0;
 }
