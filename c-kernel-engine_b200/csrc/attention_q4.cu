@@ -759,25 +759,87 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
     }
 }
 
-// A CTA per (stretch, query row) of those that several CTAs worked on.  A warp has the weights of 32 partial results in its lanes and a channel for each lane, whose
-// parts it adds up LOADS at a time; groups of HD threads take every GROUPS-th 32 results.
-template <int HD, int GROUPS, int LOADS>
-__global__ void __launch_bounds__(GROUPS * HD) attn_q4_merge_kernel(const AqParams p, int nrows)
+// The results of a stretch that several CTAs worked on become one, row by row.  Two forms: few stretches are in many parts each, many in two or three.
+struct AqParts {
+    const float *first, *base;                 // the first CTA's is its second one
+    size_t step;
+    int count;
+    float *out;
+};
+template <int HD>
+__device__ __forceinline__ bool aq_parts(const AqParams &p, int nrows, int x, int r, AqParts &a)
 {
+    const int2 d = __ldcg(p.desc + x);
+    const int bh = x / p.RC, row = (x - bh * p.RC) * nrows + r;
+    if (d.y < 0 || row >= p.R) return false;
+    a.count = d.y - d.x + 1;
+    a.step = (size_t)2 * nrows * (HD + 2);
+    a.base = p.part + (size_t)(2 * d.x) * nrows * (HD + 2) + r * (HD + 2);
+    a.first = a.base + a.step / 2;
+    const int b = bh / p.c.Hkv, h = bh - b * p.c.Hkv, tok = p.by_group(row);
+    a.out = p.out + ((long long)b * p.c.tokens + tok) * p.out_stride + (long long)(h * p.G + row - tok * p.G) * HD;
+    return true;
+}
+
+// A warp for a row, four parts at a time.
+template <int HD>
+__global__ void __launch_bounds__(128) attn_q4_merge_rows_kernel(const AqParams p, int nrows, int rows)
+{
+    constexpr int PARTS = 4;
+    pdl_wait();
+    const int lane = threadIdx.x & 31, all = p.c.batch * p.c.Hkv * p.RC;
+    const int warp = (int)(threadIdx.x >> 5), x = blockIdx.x, r0 = blockIdx.y * 4 + warp;
+    for (int s = x; s < all; s += gridDim.x) {
+        AqParts a;
+        if (r0 >= rows || !aq_parts<HD>(p, nrows, s, r0, a)) continue;
+        float top = -INFINITY, l = 0.0f, acc[HD / 32] = {};
+        for (int i0 = 0; i0 < a.count; i0 += PARTS) {
+            float ref[PARTS], part_l[PARTS], v[PARTS][HD / 32], now = top;
+#pragma unroll
+            for (int u = 0; u < PARTS; ++u) {
+                const float *from = i0 + u ? a.base + (i0 + u) * a.step : a.first;
+                const bool is = i0 + u < a.count;
+                ref[u] = is ? __ldcg(from + HD) : -INFINITY;
+                part_l[u] = is ? __ldcg(from + HD + 1) : 0.0f;
+#pragma unroll
+                for (int k = 0; k < HD / 32; ++k) v[u][k] = is ? __ldcg(from + 32 * k + lane) : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < PARTS; ++u) now = fmaxf(now, ref[u]);
+            const float keep = top == -INFINITY ? 0.0f : aq_exp2(top - now);
+            top = now;
+            l *= keep;
+#pragma unroll
+            for (int k = 0; k < HD / 32; ++k) acc[k] *= keep;
+#pragma unroll
+            for (int u = 0; u < PARTS; ++u) {
+                const float f = ref[u] == -INFINITY ? 0.0f : aq_exp2(ref[u] - top);
+                l = fmaf(f, part_l[u], l);                      // 0 x NaN: scores that are no numbers have no maximum, and must be seen
+#pragma unroll
+                for (int k = 0; k < HD / 32; ++k) acc[k] = fmaf(f, v[u][k], acc[k]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < HD / 32; ++k) a.out[32 * k + lane] = l == 0.0f ? 0.0f : acc[k] / l;
+    }
+}
+
+// A CTA for a row: a warp has the weights of 32 parts in its lanes and a channel for each lane, whose parts it adds up LOADS at a time; groups of HD threads take
+// every GROUPS-th 32 parts.
+template <int HD>
+__global__ void __launch_bounds__(512 / HD * HD) attn_q4_merge_kernel(const AqParams p, int nrows)
+{
+    constexpr int GROUPS = 512 / HD, LOADS = 16;
     __shared__ float acc_s[GROUPS][HD], top_s[GROUPS], l_s[GROUPS];
     pdl_wait();
     const int r = blockIdx.y, lane = threadIdx.x & 31, grp = threadIdx.x / HD, c = threadIdx.x - grp * HD;
     for (int x = blockIdx.x; x < p.c.batch * p.c.Hkv * p.RC; x += gridDim.x) {
-        const int2 d = __ldcg(p.desc + x);
-        const int bh = x / p.RC, row = (x - bh * p.RC) * nrows + r;
-        if (d.y < 0 || row >= p.R) continue;
-        const int count = d.y - d.x + 1;
-        const size_t step = (size_t)2 * nrows * (HD + 2);
-        const float *base = p.part + (size_t)(2 * d.x) * nrows * (HD + 2) + r * (HD + 2), *first = base + step / 2;      // the first CTA's is its second
+        AqParts a;
+        if (!aq_parts<HD>(p, nrows, x, r, a)) continue;
         float top = -INFINITY, l = 0.0f, acc = 0.0f;
-        for (int i0 = 32 * grp; i0 < count; i0 += 32 * GROUPS) {
-            const int n = min(32, count - i0);
-            const float *mine = i0 + lane == 0 ? first : base + (i0 + min(lane, n - 1)) * step;
+        for (int i0 = 32 * grp; i0 < a.count; i0 += 32 * GROUPS) {
+            const int n = min(32, a.count - i0);
+            const float *mine = i0 + lane == 0 ? a.first : a.base + (i0 + min(lane, n - 1)) * a.step;
             const float ref = lane < n ? __ldcg(mine + HD) : -INFINITY, part_l = __ldcg(mine + HD + 1);
             float now = ref;
 #pragma unroll
@@ -785,7 +847,7 @@ __global__ void __launch_bounds__(GROUPS * HD) attn_q4_merge_kernel(const AqPara
             now = fmaxf(now, top);
             const float keep = top == -INFINITY ? 0.0f : aq_exp2(top - now), f = ref == -INFINITY ? 0.0f : aq_exp2(ref - now);
             top = now;
-            float sum = lane < n ? f * part_l : 0.0f;           // 0 x NaN: scores that are no numbers have no maximum, and must be seen
+            float sum = lane < n ? f * part_l : 0.0f;           // 0 x NaN, as above
 #pragma unroll
             for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             l = l * keep + sum;
@@ -793,12 +855,12 @@ __global__ void __launch_bounds__(GROUPS * HD) attn_q4_merge_kernel(const AqPara
             for (int k0 = 0; k0 < n; k0 += LOADS) {
                 float v[LOADS];
 #pragma unroll
-                for (int u = 0; u < LOADS; ++u) v[u] = k0 + u < n ? __ldcg((i0 + k0 + u ? base + (i0 + k0 + u) * step : first) + c) : 0.0f;
+                for (int u = 0; u < LOADS; ++u) v[u] = k0 + u < n ? __ldcg((i0 + k0 + u ? a.base + (i0 + k0 + u) * a.step : a.first) + c) : 0.0f;
 #pragma unroll
                 for (int u = 0; u < LOADS; ++u) acc = fmaf(__shfl_sync(0xffffffffu, f, k0 + u), v[u], acc);
             }
         }
-        if (count > 32 && GROUPS > 1) {
+        if (a.count > 32 && GROUPS > 1) {
             acc_s[grp][c] = acc;
             if (c == 0) { top_s[grp] = top; l_s[grp] = l; }
             __syncthreads();
@@ -813,10 +875,7 @@ __global__ void __launch_bounds__(GROUPS * HD) attn_q4_merge_kernel(const AqPara
             }
             __syncthreads();
         }
-        if (grp == 0) {
-            const int b = bh / p.c.Hkv, h = bh - b * p.c.Hkv, tok = row / p.G;
-            p.out[((long long)b * p.c.tokens + tok) * p.out_stride + (long long)(h * p.G + row - tok * p.G) * HD + c] = l == 0.0f ? 0.0f : acc / l;
-        }
+        if (grp == 0) a.out[c] = l == 0.0f ? 0.0f : acc / l;
     }
 }
 
@@ -839,12 +898,12 @@ static int aq_launch(AqParams p, void *ws, cudaStream_t st)
     }
     const int rc = launch_pdl("attention_q4cache", attn_q4_kernel<HD, BLOCKS>, dim3(N), dim3(AQ_THREADS), (size_t)S::SMEM, st, p);
     if (rc || p.c.stride * p.c.page_tokens <= S::UNIT) return rc;      // no stretch has two units
-    // Few stretches are in many parts each, and their CTAs few (64 of 32 parts: 6 us, 18 us with a load at a time); many are in two or three (2048 of them: 4 us, 32 us
-    // with the CTAs of the other kind).
+    // 128 channels, the whole call by CTAs and by warps: 8 stretches of 55 parts 10.6 and 12.1 us, 16 of 27 13.8 and 15.0, 24 of 18 17.7 and 16.4, 32 of 14 18.4 and 16.6,
+    // 264 with 16 rows in two or three 46 and 42
     const long long stretches = (long long)p.c.batch * p.c.Hkv * p.RC;
-    const dim3 grid((unsigned)(stretches < N ? stretches : N), S::ROWS < p.R ? S::ROWS : p.R);
-    if (stretches * 8 < N) return launch_pdl("attention_q4cache", attn_q4_merge_kernel<HD, 512 / HD, 16>, grid, dim3(512 / HD * HD), 0, st, p, S::ROWS);
-    return launch_pdl("attention_q4cache", attn_q4_merge_kernel<HD, 1, 4>, grid, dim3(HD), 0, st, p, S::ROWS);
+    const int rows = S::ROWS < p.R ? S::ROWS : p.R;
+    if (stretches * 22 < N) return launch_pdl("attention_q4cache", attn_q4_merge_kernel<HD>, dim3((unsigned)stretches, rows), dim3(512 / HD * HD), 0, st, p, S::ROWS);
+    return launch_pdl("attention_q4cache", attn_q4_merge_rows_kernel<HD>, dim3((unsigned)(stretches < N ? stretches : N), (rows + 3) / 4), dim3(128), 0, st, p, S::ROWS, rows);
 }
 
 template <int HD, int BLOCKS>
