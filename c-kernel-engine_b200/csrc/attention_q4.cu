@@ -55,9 +55,10 @@ struct AqShape {
     static constexpr int STAGE = 2 * CHUNK * ROW;                              // K rows, then V rows
     static constexpr int CTAS = NB > 1 && HD > 192 ? 1 : (NB > 1 || HD > 128 ? 2 : 3);                       // resident on an SM, for which registers and shared memory are kept
     static constexpr int STAGES = HD <= 64 ? 4 : (HD <= 128 && NB < 3 ? 3 : 2);
-    static constexpr int OREG = NB * G4 * 8, DUMP = (OREG + 2 * NB) * 32 * 4;      // a warp's accumulators, maxima and sums, register by register
+    static constexpr int MINE = NB * G4 * 2;                                  // each warp joins a quarter of the four warps' accumulators; it gives away the others
+    static constexpr int GIVEN = AQ_WARPS * (3 * MINE + 2 * NB) * 32 * 4;
     static constexpr int RING = AQ_WARPS * STAGES * STAGE, QF = NB * KS * 32 * 16, QS = NB * 32 * 8, EX = AQ_WARPS * NB * 8 * SP * 4, TAB = AQ_WARPS * 3 * G4 * 2 * CHUNK;
-    static constexpr int SMEM = RING + (QF + QS + EX + TAB > 2 * DUMP ? QF + QS + EX + TAB : 2 * DUMP);      // the exchange between warps lies over the queries
+    static constexpr int SMEM = RING + (QF + QS + EX + TAB > GIVEN ? QF + QS + EX + TAB : GIVEN);      // the exchange between warps lies over the queries
     static_assert(CTAS * (SMEM + 2048) <= 227 * 1024, "shared memory");
 };
 
@@ -187,7 +188,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
     const uint2 *qf2 = reinterpret_cast<const uint2 *>(qf);
     uint2 *qsum = reinterpret_cast<uint2 *>(aq_smem + S::RING + S::QF);           // [NB][lane] {hi, lo} sums of the scaled query over blocks 2t and 2t + 1, times 2^-6: both in fp16's normal range
     __shared__ float q_factor[ROWS];
-    float *dump = reinterpret_cast<float *>(aq_smem + S::RING);
+    float *given = reinterpret_cast<float *>(aq_smem + S::RING), *given_ref = given + AQ_WARPS * 3 * S::MINE * 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, g_row = PACK ? g & 3 : g;
     float *ex = reinterpret_cast<float *>(aq_smem + S::RING + S::QF + S::QS) + warp * NB * 8 * S::SP;
     // for each key of the warp's chunk: d times 2^b, and the middle m + 8 d of the values that a block can say, as two pieces; [G4][keys] halves each
@@ -319,22 +320,25 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
         if (lane == 0) entry = look(f_pos, f_slot);
         for (int i = 0; i < STAGES - 1; ++i) fetch();
 
+        float qx[ROWS / AQ_WARPS][G4];                         // rows of a stretch's queries, on their way while the stretch before is joined
+        auto load_q = [&]() {
+#pragma unroll
+            for (int i = 0; i < ROWS / AQ_WARPS; ++i) {
+                const int row = w.rc * ROWS + warp + i * AQ_WARPS, tok = p.by_group(row);
+                const float *src = p.q + ((long long)w.b * p.c.tokens + tok) * p.q_stride + (long long)(w.h * p.G + row - tok * p.G) * HD;
+#pragma unroll
+                for (int j = 0; j < G4; ++j) qx[i][j] = row < p.R ? __ldcg(src + 32 * j + lane) : 0.0f;
+            }
+        };
+        load_q();
         int stage = 0;
         uint32_t phase = 0;
         for (int left = (int)(last - first); left;) {
             // ---- a stretch: query fragments of its rows
             const int r0 = w.rc * ROWS, u_first = w.u;
             __syncthreads();                                   // the stretch before is done with them
-            float qx[(ROWS + AQ_WARPS - 1) / AQ_WARPS][G4];    // all on their way before the first is used
 #pragma unroll
-            for (int i = 0; i < (ROWS + AQ_WARPS - 1) / AQ_WARPS; ++i) {
-                const int row = r0 + warp + i * AQ_WARPS, tok = p.by_group(row);
-                const float *src = p.q + ((long long)w.b * p.c.tokens + tok) * p.q_stride + (long long)(w.h * p.G + row - tok * p.G) * HD;
-#pragma unroll
-                for (int j = 0; j < G4; ++j) qx[i][j] = row < p.R ? __ldcg(src + 32 * j + lane) : 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < (ROWS + AQ_WARPS - 1) / AQ_WARPS; ++i) {      // a warp per row, a lane the channels 4 (lane % 4 ..) of its blocks
+            for (int i = 0; i < ROWS / AQ_WARPS; ++i) {      // a warp per row, a lane the channels 4 (lane % 4 ..) of its blocks
                 const int r = warp + i * AQ_WARPS;
                 const float (&x)[G4] = qx[i];
                 float top = 0.0f;
@@ -650,11 +654,17 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
             }
 
             // ---- the stretch ends here: the four warps' results, relative to 2^ref, become one
+            const bool whole = u_first == 0 && w.u >= w.n;
+            if (u_first == 0 && tid == 0)                      // its last unit is n - u units behind the end of this CTA's part
+                p.desc[((size_t)w.b * p.c.Hkv + w.h) * p.RC + w.rc] = make_int2(me, whole ? -1 : (int)(((last + w.n - w.u) * parts - 1) / total));
+            float *part = whole ? nullptr : p.part + (size_t)(2 * me + (u_first == 0)) * ROWS * (HD + 2), *out = p.out + (long long)w.b * p.c.tokens * p.out_stride + (long long)w.h * p.G * HD;
+            if (left) {
+                aq_next_stretch(p, ROWS, S::UNIT, w);
+                load_q();
+            }
             const float unscale = __uint_as_float((uint32_t)(127 - b_run) << 23);
-            float ref[NB];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                ref[nb] = m_run[nb];
                 l_run[nb] += __shfl_xor_sync(0xffffffffu, l_run[nb], 1);
                 l_run[nb] += __shfl_xor_sync(0xffffffffu, l_run[nb], 2);
 #pragma unroll
@@ -668,71 +678,72 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                     }
                 }
             }
-            auto put = [&](float *to) {
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-                    for (int e = 0; e < G4 * 8; ++e) to[(nb * G4 * 8 + e) * 32 + lane] = o[nb][e >> 3][e >> 2 & 1][e & 3];
-                    to[(S::OREG + 2 * nb) * 32 + lane] = ref[nb];
-                    to[(S::OREG + 2 * nb + 1) * 32 + lane] = l_run[nb];
-                }
-            };
-            auto join = [&](const float *from) {
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    const float ref2 = from[(S::OREG + 2 * nb) * 32 + lane], l2 = from[(S::OREG + 2 * nb + 1) * 32 + lane], both = fmaxf(ref[nb], ref2);
-                    const float f = ref[nb] == -INFINITY ? 0.0f : aq_exp2(ref[nb] - both), f2 = ref2 == -INFINITY ? 0.0f : aq_exp2(ref2 - both);
-                    l_run[nb] = l_run[nb] * f + l2 * f2;
-                    ref[nb] = both;
-                    const float fa = __shfl_sync(0xffffffffu, f, 8 * t), fb = __shfl_sync(0xffffffffu, f, 8 * t + 4);
-                    const float f2a = __shfl_sync(0xffffffffu, f2, 8 * t), f2b = __shfl_sync(0xffffffffu, f2, 8 * t + 4);
-#pragma unroll
-                    for (int e = 0; e < G4 * 8; ++e) {
-                        float &x = o[nb][e >> 3][e >> 2 & 1][e & 3];
-                        x = x * (e & 1 ? fb : fa) + from[(nb * G4 * 8 + e) * 32 + lane] * (e & 1 ? f2b : f2a);
-                    }
-                }
-            };
-            float *half = dump + (warp & 1) * (S::DUMP / 4);
+            // quarter d of a block's registers goes to warp d: pairs d G4 .. of (channel block, x, y)
+            auto given_by = [&](int from, int to) { return given + (from * 3 + ((to - from - 1) & 3)) * S::MINE * 32 + lane; };
             __syncthreads();                                   // the queries are no longer needed
-            if (warp >= 2) put(half);
-            __syncthreads();
-            if (warp < 2) join(half);
-            __syncthreads();
-            if (warp == 1) put(dump);
-            __syncthreads();
-            if (warp == 0) {
-                join(dump);
-                const bool whole = u_first == 0 && w.u >= w.n;
-                float *part = whole ? nullptr : p.part + (size_t)(2 * me + (u_first == 0)) * ROWS * (HD + 2);
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    if (part && t == 0 && 8 * nb + g < ROWS) {
-                        part[(8 * nb + g) * (HD + 2) + HD] = ref[nb];
-                        part[(8 * nb + g) * (HD + 2) + HD + 1] = l_run[nb];
+            for (int d = 0; d < AQ_WARPS; ++d) {
+                if (d == warp) continue;
+                float *to = given_by(warp, d);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int e = 0; e < G4 * 2; ++e) {
+                        const int at = d * G4 * 2 + e;
+                        to[(nb * G4 * 2 + e) * 32] = o[nb][at >> 3][at >> 2 & 1][at & 3];
                     }
+            }
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int r = 8 * nb + 2 * t + e, row = r0 + r, tok = p.by_group(row);
-                        const float l = __shfl_sync(0xffffffffu, l_run[nb], 8 * t + 4 * e);
-                        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                        if (r >= ROWS || row >= p.R) continue;
-                        float *to = part ? part + r * (HD + 2) : p.out + ((long long)w.b * p.c.tokens + tok) * p.out_stride + (long long)(w.h * p.G + row - tok * p.G) * HD;
+            for (int nb = 0; nb < NB; ++nb) {
+                given_ref[(warp * NB + nb) * 64 + lane] = m_run[nb];
+                given_ref[(warp * NB + nb) * 64 + 32 + lane] = l_run[nb];
+            }
+            __syncthreads();
 #pragma unroll
-                        for (int j = 0; j < G4; ++j)
+            for (int nb = 0; nb < NB; ++nb) {
+                float ref[AQ_WARPS], f[AQ_WARPS], both = -INFINITY, l = 0.0f, sum[G4 * 2];
 #pragma unroll
-                            for (int x = 0; x < 2; ++x)
+                for (int s = 0; s < AQ_WARPS; ++s) {
+                    ref[s] = given_ref[(s * NB + nb) * 64 + lane];
+                    both = fmaxf(both, ref[s]);
+                }
 #pragma unroll
-                                for (int y = 0; y < 2; ++y) {
-                                    const float v = o[nb][j][x][2 * y + e];
-                                    to[32 * j + 2 * g + x + 16 * y] = part ? v : v * inv;
-                                }
+                for (int s = 0; s < AQ_WARPS; ++s) {
+                    f[s] = ref[s] == -INFINITY ? 0.0f : aq_exp2(ref[s] - both);
+                    l = fmaf(f[s], given_ref[(s * NB + nb) * 64 + 32 + lane], l);
+                }
+#pragma unroll
+                for (int e = 0; e < G4 * 2; ++e) sum[e] = 0.0f;
+#pragma unroll
+                for (int s = 0; s < AQ_WARPS; ++s) {           // in the same order whichever warp joins
+                    const float fa = __shfl_sync(0xffffffffu, f[s], 8 * t), fb = __shfl_sync(0xffffffffu, f[s], 8 * t + 4);
+                    const float *from = given_by(s, warp) + nb * G4 * 2 * 32;
+#pragma unroll
+                    for (int e = 0; e < G4 * 2; ++e) {
+                        float x;
+                        if (s == warp) x = o[nb][(s * G4 * 2 + e) >> 3][(s * G4 * 2 + e) >> 2 & 1][(s * G4 * 2 + e) & 3];
+                        else x = from[e * 32];
+                        sum[e] = fmaf(e & 1 ? fb : fa, x, sum[e]);
                     }
                 }
-                if (u_first == 0 && lane == 0)                  // its last unit is n - u units behind the end of this CTA's part
-                    p.desc[((size_t)w.b * p.c.Hkv + w.h) * p.RC + w.rc] = make_int2(me, whole ? -1 : (int)(((last + w.n - w.u) * parts - 1) / total));
+                if (part && warp == 0 && t == 0 && 8 * nb + g < ROWS) {
+                    part[(8 * nb + g) * (HD + 2) + HD] = both;
+                    part[(8 * nb + g) * (HD + 2) + HD + 1] = l;
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int r = 8 * nb + 2 * t + e, row = r0 + r, tok = p.by_group(row);
+                    const float row_l = __shfl_sync(0xffffffffu, l, 8 * t + 4 * e);
+                    const float inv = row_l == 0.0f ? 0.0f : 1.0f / row_l;
+                    if (r >= ROWS || row >= p.R) continue;
+                    float *to = part ? part + r * (HD + 2) : out + tok * p.out_stride + (long long)(row - tok * p.G) * HD;
+#pragma unroll
+                    for (int k = 0; k < G4; ++k) {
+                        const int at = warp * G4 + k;
+                        to[32 * (at >> 2) + 2 * g + (at >> 1 & 1) + 16 * (at & 1)] = part ? sum[2 * k + e] : sum[2 * k + e] * inv;
+                    }
+                }
             }
-            if (left) aq_next_stretch(p, ROWS, S::UNIT, w);
         }
         // a wait ran out: the copies still on their way, of the last STAGES units, end before the CTA does
         if (!ok)
