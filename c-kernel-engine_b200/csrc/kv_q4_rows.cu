@@ -18,19 +18,31 @@ namespace ckb {
 
 constexpr int KR_THREADS = 256;
 
+__device__ __forceinline__ float kr_min3(float a, float b, float c)
+{
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float kr_max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // the word of codes of lane l of the four, and the block's (d, m)
 __device__ __forceinline__ uint32_t kr_quantise(const float4 &x, const float4 &y, uint32_t &dm)
 {
     const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-    float lo = v[0], hi = v[0];
-    bool fine = true;
+    float lo = fminf(v[0], v[1]), hi = fmaxf(v[0], v[1]), zero = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        lo = fminf(lo, v[i]);
-        hi = fmaxf(hi, v[i]);
-        fine &= fabsf(v[i]) <= FLT_MAX;                        // minimum and maximum pass over NaN: it is looked for by itself
+    for (int i = 2; i < 8; i += 2) {
+        lo = kr_min3(lo, v[i], v[i + 1]);
+        hi = kr_max3(hi, v[i], v[i + 1]);
     }
-    if (!fine) hi = INFINITY;                                  // no code can say the block: d becomes infinite, below
+#pragma unroll
+    for (int i = 0; i < 8; ++i) zero = __fmaf_rn(v[i], 0.0f, zero);      // minimum and maximum pass over NaN: it is looked for by itself, with infinities
+    if (zero != 0.0f) hi = INFINITY;                           // no code can say the block: d becomes infinite, below
 #pragma unroll
     for (int o = 2; o; o >>= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
@@ -39,12 +51,17 @@ __device__ __forceinline__ uint32_t kr_quantise(const float4 &x, const float4 &y
     // the two roundings to fp16 that the format asks for; codes are then taken against the rounded pair, so that each is the nearest that the block can say
     const __half mh = __float2half_rn(lo), dh = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f));
     const float m = __half2float(mh), d = __half2float(dh), inv = d > 0.0f ? __frcp_rn(d) : 0.0f;
-    uint32_t codes = 0;
+    // The floor of a number of [0, 16) is in the last bits of its sixteenth's sum with 2^19, rounded down; what the sums' other bits add up to is taken off at the end.
+    // (Comparisons and shifts are what bounds the store: here a value costs two of them, and floor, clamp, convert and shift six.)
+    uint32_t codes = 0, others = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float t = floorf(__fadd_rn(__fmul_rn(__fsub_rn(v[i], m), inv), 0.5f));
-        codes |= (uint32_t)fminf(fmaxf(t, 0.0f), 15.0f) << (8 * (i & 3) + 4 * (i >> 2));
+        const float t = __saturatef(fminf(__fadd_rn(__fmul_rn(__fsub_rn(v[i], m), inv), 0.5f), 15.5f) * 0.0625f);
+        const int at = 8 * (i & 3) + 4 * (i >> 2);
+        codes += __float_as_uint(__fadd_rd(t, 524288.0f)) << at;
+        others += 0x49000000u << at;
     }
+    codes -= others;
     const bool good = fabsf(m) <= 65504.0f && d <= 65504.0f;
     dm = good ? (uint32_t)__half_as_ushort(mh) << 16 | __half_as_ushort(dh) : 0x7fff7fffu;
     return good ? codes : 0;
@@ -100,13 +117,13 @@ __global__ void __launch_bounds__(KR_THREADS) kv_store_q4_kernel(uint8_t *__rest
     a[0] = a[1] = b[0] = b[1] = make_float4(0.f, 0.f, 0.f, 0.f);
     long long at = -1;
     if (grp < p.groups) {
-        int row, block;
-        kr_where<false>(p, grp, row, block, at);
+        int row = p.by_items(grp), block = (int)(grp - (uint32_t)row * p.by_items.d);
         const float *x = k + row * p.k_stride + block * 32 + 4 * l, *y = v + row * p.v_stride + block * 32 + 4 * l;
-        a[0] = kr_load4<VEC>(x);
+        a[0] = kr_load4<VEC>(x);                               // on their way while the length and the table's entry are looked up
         a[1] = kr_load4<VEC>(x + 16);
         b[0] = kr_load4<VEC>(y);
         b[1] = kr_load4<VEC>(y + 16);
+        kr_where<false>(p, grp, row, block, at);
     }
     uint32_t dmk, dmv;
     const uint32_t wk = kr_quantise(a[0], a[1], dmk), wv = kr_quantise(b[0], b[1], dmv);
@@ -118,11 +135,12 @@ __global__ void __launch_bounds__(KR_THREADS) kv_store_q4_kernel(uint8_t *__rest
     if (l == 1) y[0] = dmv;
 }
 
-__device__ __forceinline__ float4 kr_values(uint32_t dm, uint32_t w)       // of the low nibbles of w
+// the code of byte `byte`, low nibble, as a number: in the last bits of 2^23, which is taken off again
+__device__ __forceinline__ float kr_code(uint32_t w, int byte) { return __fsub_rn(__uint_as_float((w >> 8 * byte & 15u) | 0x4b000000u), 8388608.0f); }
+__device__ __forceinline__ float4 kr_values(uint32_t dm, uint32_t w)       // of the low nibbles of w; d times a code is exact
 {
     const float d = half_bits_to_float(dm & 0xffffu), m = half_bits_to_float(dm >> 16);
-    return make_float4(__fadd_rn(__fmul_rn(d, (float)(w & 15u)), m), __fadd_rn(__fmul_rn(d, (float)(w >> 8 & 15u)), m), __fadd_rn(__fmul_rn(d, (float)(w >> 16 & 15u)), m),
-                       __fadd_rn(__fmul_rn(d, (float)(w >> 24 & 15u)), m));
+    return make_float4(__fmaf_rn(d, kr_code(w, 0), m), __fmaf_rn(d, kr_code(w, 1), m), __fmaf_rn(d, kr_code(w, 2), m), __fmaf_rn(d, kr_code(w, 3), m));
 }
 
 template <bool VEC>
