@@ -4,6 +4,7 @@
 // host.  What a call decides is the same in every run: free pages are handed out by number, the order of the atomics on the counts cannot
 // be seen in their sums.  Each call is one kernel that decides, by one CTA where an order over all pages or sequences is needed (latency: a few
 // dependent trips to L2), and one that moves the bytes of the pages chosen, at copy bandwidth, reading the list that the first one left.
+// Kernels start while the one before is still running and wait for it: tables are read through L2.
 #include "../../include/ckb200_cache.h"
 #include "device_common.cuh"
 #include "kv_q4.cuh"
@@ -147,9 +148,9 @@ __global__ void __launch_bounds__(KC_THREADS) kv_pages_copy_kernel(KvPool pool, 
         const int live = __ldcg(count_dev + 1);
         for (int b = blockIdx.x; b < t.batch; b += gridDim.x) {
             int *row = t.table + (size_t)b * t.stride;
-            const int n = kv_columns(kv_len(t.lens[b], t.stride, t.page_tokens), t.page_tokens);
+            const int n = kv_columns(kv_len(__ldcg(t.lens + b), t.stride, t.page_tokens), t.page_tokens);
             for (int i = threadIdx.x; i < n; i += KC_THREADS) {
-                const int e = row[i];
+                const int e = __ldcg(row + i);
                 if (e < live || e >= t.pages) continue;
                 const int to = __ldcg(place + e);
                 if (to >= 0) row[i] = to;
@@ -189,11 +190,12 @@ __global__ void __launch_bounds__(KP_THREADS) kv_pages_resize_kernel(KvTables t,
     int *len_s = kp_sm, *new_s = len_s + B, *part_s = new_s + B, *want_s = part_s + B, *first_s = want_s + B, *cow_s = first_s + B;
     int *src = ws + 4, *dst = src + B;
     pdl_trigger();
+    pdl_wait();
     if (threadIdx.x == 0) s_slow = 0;
     int shrinks = 0;
     for (int b = threadIdx.x; b < B; b += KP_THREADS) {
-        const int len = kv_len(t.lens[b], t.stride, pt);
-        int nl = new_lens[b], bad = 0;
+        const int len = kv_len(__ldcg(t.lens + b), t.stride, pt);
+        int nl = __ldcg(new_lens + b), bad = 0;
         if (nl > t.stride * pt) { nl = -1; bad = 1; }
         len_s[b] = len;
         new_s[b] = nl = nl < 0 ? len : nl;
@@ -206,7 +208,7 @@ __global__ void __launch_bounds__(KP_THREADS) kv_pages_resize_kernel(KvTables t,
         const int have = kv_columns(len_s[b], pt), need = kv_columns(new_s[b], pt);
         int *row = t.table + (size_t)b * t.stride;
         for (int i = need + lane; i < have; i += 32) {
-            const int e = kv_entry(row[i], t.pages);
+            const int e = kv_entry(__ldcg(row + i), t.pages);
             if (e >= 0) atomicSub(t.refs + e, 1);
             row[i] = -1;
         }
@@ -220,7 +222,7 @@ __global__ void __launch_bounds__(KP_THREADS) kv_pages_resize_kernel(KvTables t,
     for (int b = threadIdx.x; b < B; b += KP_THREADS) {
         int page = -1;
         if (new_s[b] > len_s[b] && len_s[b] % pt) {
-            page = kv_entry(t.table[(size_t)b * t.stride + len_s[b] / pt], t.pages);
+            page = kv_entry(__ldcg(t.table + (size_t)b * t.stride + len_s[b] / pt), t.pages);
             if (page >= 0 && __ldcg(t.refs + page) <= 1) page = -1;
         }
         part_s[b] = page;
@@ -273,7 +275,7 @@ __global__ void __launch_bounds__(KP_THREADS) kv_pages_resize_kernel(KvTables t,
                 int used = 0, nc = 0;
                 for (int b = 0; b < B; ++b) {
                     if (want_s[b] < 0) continue;
-                    int page = len_s[b] % pt ? kv_entry(t.table[(size_t)b * t.stride + len_s[b] / pt], t.pages) : -1, cow = 0;
+                    int page = len_s[b] % pt ? kv_entry(__ldcg(t.table + (size_t)b * t.stride + len_s[b] / pt), t.pages) : -1, cow = 0;
                     if (page >= 0) cow = __ldcg(t.refs + page) > 1;
                     const int want = cow + kv_columns(new_s[b], pt) - kv_columns(len_s[b], pt);
                     cow_s[b] = 0;
@@ -329,17 +331,18 @@ __global__ void __launch_bounds__(KP_THREADS) kv_pages_resize_kernel(KvTables t,
 // ws: [batch] lengths to come (-1: stays as it is), [batch][stride] rows to come
 __global__ void __launch_bounds__(128) kv_pages_fork_read_kernel(KvTables t, const int *__restrict__ parent, int *__restrict__ ws)
 {
-    const int b = blockIdx.x, from = parent[b];
     pdl_trigger();
+    pdl_wait();
+    const int b = blockIdx.x, from = __ldcg(parent + b);
     if (from < 0 || from >= t.batch || from == b) {
         if (threadIdx.x == 0) ws[b] = -1;
         return;
     }
-    const int len = kv_len(t.lens[from], t.stride, t.page_tokens), n = kv_columns(len, t.page_tokens);
+    const int len = kv_len(__ldcg(t.lens + from), t.stride, t.page_tokens), n = kv_columns(len, t.page_tokens);
     const int *row = t.table + (size_t)from * t.stride;
     int *to = ws + t.batch + (size_t)b * t.stride;
     for (int i = threadIdx.x; i < n; i += 128) {
-        const int e = kv_entry(row[i], t.pages);
+        const int e = kv_entry(__ldcg(row + i), t.pages);
         to[i] = e;
         if (e >= 0) atomicAdd(t.refs + e, 1);
     }
@@ -347,14 +350,15 @@ __global__ void __launch_bounds__(128) kv_pages_fork_read_kernel(KvTables t, con
 }
 __global__ void __launch_bounds__(128) kv_pages_fork_write_kernel(KvTables t, const int *__restrict__ ws)
 {
+    pdl_trigger();
     pdl_wait();
     const int b = blockIdx.x, len = __ldcg(ws + b);
     if (len < 0) return;
-    const int n = kv_columns(len, t.page_tokens), had = kv_columns(kv_len(t.lens[b], t.stride, t.page_tokens), t.page_tokens);
+    const int n = kv_columns(len, t.page_tokens), had = kv_columns(kv_len(__ldcg(t.lens + b), t.stride, t.page_tokens), t.page_tokens);
     const int *from = ws + t.batch + (size_t)b * t.stride;
     int *row = t.table + (size_t)b * t.stride;
     for (int i = threadIdx.x; i < max(n, had); i += 128) {
-        const int e = i < had ? kv_entry(row[i], t.pages) : -1;
+        const int e = i < had ? kv_entry(__ldcg(row + i), t.pages) : -1;
         if (e >= 0) atomicSub(t.refs + e, 1);
         row[i] = i < n ? __ldcg(from + i) : -1;
     }
@@ -366,10 +370,12 @@ __global__ void __launch_bounds__(128) kv_pages_fork_write_kernel(KvTables t, co
 __global__ void __launch_bounds__(KP_THREADS) kv_pages_fork_kernel(KvTables t, const int *__restrict__ parent)
 {
     extern __shared__ int kp_sm[];
+    pdl_trigger();
+    pdl_wait();
     int *len_s = kp_sm, *parent_s = len_s + t.batch;            // a parent: -1 for none
     for (int b = threadIdx.x; b < t.batch; b += KP_THREADS) {
-        const int from = parent[b];
-        len_s[b] = kv_len(t.lens[b], t.stride, t.page_tokens);
+        const int from = __ldcg(parent + b);
+        len_s[b] = kv_len(__ldcg(t.lens + b), t.stride, t.page_tokens);
         parent_s[b] = from < 0 || from >= t.batch || from == b ? -1 : from;
     }
     __syncthreads();
@@ -381,8 +387,8 @@ __global__ void __launch_bounds__(KP_THREADS) kv_pages_fork_kernel(KvTables t, c
         next[u] = -2;
         if (b >= t.batch || parent_s[b] < 0) continue;
         const int had = kv_columns(len_s[b], t.page_tokens), n = kv_columns(len_s[parent_s[b]], t.page_tokens);
-        if (i < had) now[u] = t.table[x];
-        if (i < n) next[u] = t.table[parent_s[b] * t.stride + i];
+        if (i < had) now[u] = __ldcg(t.table + x);
+        if (i < n) next[u] = __ldcg(t.table + parent_s[b] * t.stride + i);
         else if (i < had) next[u] = -1;
         if (i < n) next[u] = max(-1, next[u]);
     }
@@ -408,6 +414,7 @@ __global__ void __launch_bounds__(KP_THREADS) kv_pages_plan_kernel(KvTables t, i
     const int lane = threadIdx.x & 31;
     int *src = ws + 4, *dst = src + t.pages, *place = dst + t.pages;
     pdl_trigger();
+    pdl_wait();
     KpStretch pages = kp_stretch(t.pages);
     const int lo = pages.lo, hi = pages.hi, n = kp_count_free(t.refs, pages);
     const int free_here[1] = {lane == 0 ? n : 0};
@@ -432,7 +439,7 @@ __global__ void __launch_bounds__(KP_THREADS) kv_pages_plan_kernel(KvTables t, i
             dst[i] = d;
         }
         place[s] = d;
-        t.refs[d] = t.refs[s];
+        t.refs[d] = __ldcg(t.refs + s);
         t.refs[s] = 0;
     }
     if (threadIdx.x == 0) {
@@ -512,12 +519,11 @@ extern "C" int ckb200_dev_kv_pages_resize(int *page_table, int table_stride, int
     if ((rc = ckb_check_device(what))) return rc;
     const KvTables t = {page_table, kv_lens, page_refs, table_stride, batch, num_pages, page_tokens};
     const size_t smem = 6 * sizeof(int) * (size_t)batch;
-    if (smem > 40 * 1024 && ckb_check_cuda((int)cudaFuncSetAttribute(kv_pages_resize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 6 * (int)sizeof(int) * KP_MAX_BATCH), what))
+    if (smem > 32 * 1024 && ckb_check_cuda((int)cudaFuncSetAttribute(kv_pages_resize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 6 * (int)sizeof(int) * KP_MAX_BATCH), what))
         return CKB_ERR_CUDA;
     cudaStream_t st = ckb_stream(stream);
     int *ws = (int *)workspace;
-    kv_pages_resize_kernel<<<1, KP_THREADS, smem, st>>>(t, new_lens, status, ws);
-    if ((rc = ckb_check_launch(what)) || !planes) return rc;
+    if ((rc = launch_pdl(what, kv_pages_resize_kernel, dim3(1), dim3(KP_THREADS), smem, st, t, new_lens, status, ws)) || !planes) return rc;
     const KvPool pool = {(uint8_t *)pages, plane_stride, page_bytes, planes, num_pages};
     return launch_pdl(what, kv_pages_copy_kernel, dim3(copy_grid(batch, planes, page_bytes)), dim3(KC_THREADS), 0, st, pool, (const int *)(ws + 4), (const int *)(ws + 4 + batch), (const int *)ws, 0, KvTables{},
                       (const int *)NULL);
@@ -536,12 +542,9 @@ extern "C" int ckb200_dev_kv_pages_fork(int *page_table, int table_stride, int *
     if ((rc = ckb_check_device(what))) return rc;
     const KvTables t = {page_table, kv_lens, page_refs, table_stride, batch, num_pages, page_tokens};
     cudaStream_t st = ckb_stream(stream);
-    if ((long long)batch * table_stride <= KP_THREADS * KP_FORK) {
-        kv_pages_fork_kernel<<<1, KP_THREADS, 2 * sizeof(int) * (size_t)batch, st>>>(t, parent);
-        return ckb_check_launch(what);
-    }
-    kv_pages_fork_read_kernel<<<batch, 128, 0, st>>>(t, parent, (int *)workspace);
-    if ((rc = ckb_check_launch(what))) return rc;
+    if ((long long)batch * table_stride <= KP_THREADS * KP_FORK)
+        return launch_pdl(what, kv_pages_fork_kernel, dim3(1), dim3(KP_THREADS), 2 * sizeof(int) * (size_t)batch, st, t, parent);
+    if ((rc = launch_pdl(what, kv_pages_fork_read_kernel, dim3(batch), dim3(128), 0, st, t, parent, (int *)workspace))) return rc;
     return launch_pdl(what, kv_pages_fork_write_kernel, dim3(batch), dim3(128), 0, st, t, (const int *)workspace);
 }
 
@@ -558,8 +561,7 @@ extern "C" int ckb200_dev_kv_pages_compact(int *page_table, int table_stride, co
     const KvTables t = {page_table, const_cast<int *>(kv_lens), page_refs, table_stride, batch, num_pages, page_tokens};
     cudaStream_t st = ckb_stream(stream);
     int *ws = (int *)workspace;
-    kv_pages_plan_kernel<<<1, KP_THREADS, 0, st>>>(t, live, ws);
-    if ((rc = ckb_check_launch(what))) return rc;
+    if ((rc = launch_pdl(what, kv_pages_plan_kernel, dim3(1), dim3(KP_THREADS), 0, st, t, live, ws))) return rc;
     const KvPool pool = {(uint8_t *)pages, plane_stride, page_bytes, planes, num_pages};
     const unsigned pieces = copy_grid(num_pages / 2, planes, page_bytes), grid = pieces > (unsigned)batch ? pieces : (unsigned)batch;      // each also takes rows of the table
     return launch_pdl(what, kv_pages_copy_kernel, dim3(grid), dim3(KC_THREADS), 0, st, pool, (const int *)(ws + 4), (const int *)(ws + 4 + num_pages), (const int *)ws, 0, t,

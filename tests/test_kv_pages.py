@@ -95,7 +95,7 @@ def make(lib, rng, batch, stride, pages, page_tokens, planes=3, page_bytes=160, 
 @pytest.mark.gpu
 @pytest.mark.parametrize("batch,stride,pages,page_tokens,planes,page_bytes", [(1, 1, 1, 16, 1, 16), (3, 4, 9, 16, 2, 320), (8, 6, 40, 16, 3, 5120), (33, 5, 90, 48, 1, 4112), (70, 9, 500, 16, 2, 160),
                                                                              (5, 300, 12, 16, 1, 32), (1100, 3, 2100, 16, 1, 16), (6, 5, 31, 64, 160, 2560), (4, 3, 12, 16, 0, 0),
-                                                                             (310, 28, 9000, 16, 1, 16), (128, 64, 700, 16, 1, 16), (4096, 2, 4500, 16, 1, 16)])
+                                                                             (310, 28, 9000, 16, 1, 16), (128, 64, 700, 16, 1, 16), (1700, 2, 1900, 16, 1, 16), (4096, 2, 4500, 16, 1, 16)])
 def test_any_order_of_calls(gpu, batch, stride, pages, page_tokens, planes, page_bytes):  # noqa: F811
     """Grown, shrunk, freed, forked onto one another, compacted, with too little room now and then: after each call everything is what the host's walk gives."""
     rng = np.random.default_rng(batch * 7 + pages)
