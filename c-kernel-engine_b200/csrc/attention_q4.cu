@@ -18,19 +18,19 @@
 //   output  O^T = V^T P^T 16 channels x 8 query rows; A words are the same two bytes (four channels) of two keys, joined by one byte permute
 //
 // A query row is a (token, head) of the kv head's group: up to 8 NB rows share every code that is unpacked (NB = 1 for decoding, more for
-// drafts and portions of prompts).
+// drafts and portions of prompts).  Up to four rows take one product instead of two: its eight columns are their hi and their lo pieces.
 //
-// Work.  A unit is 128 keys of one (sequence, kv head, 8 NB rows); the units of all sequences form one line that is cut evenly among the CTAs that
+// Work.  A unit is 128 keys of one (sequence, block of 8 NB rows, kv head); the units of all sequences form one line that is cut evenly among the CTAs that
 // the GPU holds at once, so long and short sequences load it alike and nothing but the lengths on the device decides.  Each of the four warps takes
 // a quarter of a unit through a ring of its own (untiled bulk copies: 32 rows of K and of V, or 16 where pages may end between), without meeting the
-// others until a sequence's stretch ends.  Stretches that lie within one CTA are written out at once, the others as partial results that
-// a second kernel joins (log-sum-exp).
+// others until a sequence's stretch ends; then each warp joins a quarter of the accumulators while the next queries load.  Stretches that lie within one CTA are
+// written out at once, the others as partial results that a second kernel joins (log-sum-exp).
 //
 // What bounds it.  Not HBM: the ring alone, without the arithmetic, takes 113 us for four sequences of 131072 tokens (64 heads over 8 of 128 channels,
-// 667 MB, 102 us at the measured copy rate), the whole kernel 221 us, 3.0 TB/s.  A chunk of 32 keys is 1009 warp instructions, 74 of them products, issued at 2.1 an
-// SM and cycle: half-rate logic (codes, 300 of them), half-precision and conversion instructions and the products, each alone at 15 to 30 % of its pipe, hinder one another.
-// Two, three or four CTAs an SM (8 to 16 warps, 255 to 128 registers): 239 / 221 / 223 us; chunks of 64 keys 213 us, but 10.2 us instead of 9.2 for 77 keys; a warp that
-// fetches for four others, which takes the registers of four: 217 us.
+// 667 MB, 102 us at the measured copy rate), the whole kernel 218 us, 3.1 TB/s (32 heads: 190 us, 3.5 TB/s).  A chunk of 32 keys is 1005 warp instructions, 74 of them
+// products (38 with four rows), issued at 2.2 an SM and cycle: products, half-precision instructions and integer multiplications share one pipe, half-rate logic (codes, 300
+// instructions) has another, each is busy for 20 to 40 % of the time, and a warp waits 1.75 cycles an instruction for the one before it.
+// Two, three or four CTAs an SM (8 to 16 warps, 255 to 128 registers): 239 / 218 / 223 us.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -925,9 +925,8 @@ static size_t aq_bytes(int batch, int Hkv, int R)
 }
 
 // Blocks of 8 query rows that share the codes a CTA unpacks; 0: up to four, with both pieces of a row in one product (32 heads over 8, four sequences of 131072
-// tokens 188 us, 218 us in a block of 8; 32 of up to 4096 51 and 57).  A unit costs 1 : 1.45 : 2.3 with one, two and three blocks (128 channels), so three are worth
-// it only where they hold all the rows: 20 rows of 16 sequences (five drafts, up to 8190 tokens) 119 us with three, 152 us with two and two; 516 rows 55 us in blocks
-// of two, 61 us in blocks of three.
+// tokens 190 us, 217 us in a block of 8; 32 of up to 4096 48 and 53).  Three blocks leave no register free and are worth it only where they hold all the rows: 20 rows of
+// 16 sequences (five drafts, up to 8190 tokens) 99 us with three, 109 us one by one, 130 us with two and two; 516 rows 38 us in blocks of two, 42 us one by one, 41 us in threes.
 static int aq_blocks(long long rows, int hd) { return rows <= 4 ? 0 : rows <= 8 ? 1 : (rows > 16 && rows <= 24 && hd <= 128 ? 3 : 2); }
 
 }  // namespace ckb

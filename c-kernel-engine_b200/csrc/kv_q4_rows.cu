@@ -2,7 +2,8 @@
 //
 // A block of 32 values is the work of four lanes, for K and for V: lane l has values 4l .. 4l + 3 and 16 + 4l .. 16 + 4l + 3, which are the nibbles of code bytes
 // 4l .. 4l + 3, so that only the block's least and largest value cross lanes (two shuffles each).  A warp's loads and stores are of whole 32-byte sectors.
-// Bound by HBM, 4.625 bytes a value either way: reading 4 bytes when storing, writing them when loading.
+// Bound by HBM, 4.625 bytes a value either way: reading 4 bytes when storing, writing them when loading.  8192 rows of K and V of 1024 values: 14.4 us loaded
+// (5.4 TB/s), 16.4 us stored (4.7 TB/s: comparisons and shifts of the quantiser keep their pipe busy for more than half the time).
 #include <cuda_fp16.h>
 #include <float.h>
 #include <math.h>
