@@ -852,7 +852,12 @@ __global__ void __launch_bounds__(512 / HD * HD) attn_q4_merge_kernel(const AqPa
             const int n = min(32, a.count - i0);
             const float *mine = i0 + lane == 0 ? a.first : a.base + (i0 + min(lane, n - 1)) * a.step;
             const float ref = lane < n ? __ldcg(mine + HD) : -INFINITY, part_l = __ldcg(mine + HD + 1);
-            float now = ref;
+            float v[LOADS], now = ref;
+            auto load = [&](int k0) {
+#pragma unroll
+                for (int u = 0; u < LOADS; ++u) v[u] = k0 + u < n ? __ldcg((i0 + k0 + u ? a.base + (i0 + k0 + u) * a.step : a.first) + c) : 0.0f;
+            };
+            load(0);                                            // on their way while the weights are found
 #pragma unroll
             for (int o = 16; o; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
             now = fmaxf(now, top);
@@ -863,12 +868,11 @@ __global__ void __launch_bounds__(512 / HD * HD) attn_q4_merge_kernel(const AqPa
             for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             l = l * keep + sum;
             acc *= keep;
-            for (int k0 = 0; k0 < n; k0 += LOADS) {
-                float v[LOADS];
-#pragma unroll
-                for (int u = 0; u < LOADS; ++u) v[u] = k0 + u < n ? __ldcg((i0 + k0 + u ? a.base + (i0 + k0 + u) * a.step : a.first) + c) : 0.0f;
+            for (int k0 = 0;;) {
 #pragma unroll
                 for (int u = 0; u < LOADS; ++u) acc = fmaf(__shfl_sync(0xffffffffu, f, k0 + u), v[u], acc);
+                if ((k0 += LOADS) >= n) break;
+                load(k0);
             }
         }
         if (a.count > 32 && GROUPS > 1) {

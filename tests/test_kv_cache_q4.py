@@ -281,6 +281,8 @@ ATTENTION_CASES = [
     # more parts of one sequence than a warp has lanes, sequences by the dozen, more of them than threads in a block
     (3, 1, 64, 16, [9000], 1, 0), (2, 1, 128, 32, [5000, 17], 2, 0), (4, 2, 64, 16, [(37 * i) % 411 for i in range(90)], 1, 0), (1, 1, 64, 16, [i % 19 for i in range(700)], 1, 0),
     (5, 1, 256, 16, [4500], 1, 2 ** 31 - 1),
+    # the same with several blocks of query rows and kv heads, and a stretch in a dozen parts
+    (16, 4, 64, 16, [(29 * i) % 61 for i in range(150)], 9, 20), (3, 3, 96, 16, [(31 * i) % 50 for i in range(200)], 3, 0), (24, 24, 64, 16, [2400], 1, 0), (24, 12, 128, 32, [1300, 5, 1299], 4, 0),
     (16, 2, 64, 16, [300, 90], 17, 40), (2, 2, 128, 16, [130], 130, 16), (4, 1, 128, 16, [3000, 5, 2049], 1, 0), (8, 8, 64, 256, [2500], 3, 2048), (4, 1, 128, 64, [50], 100, 0),
 ]
 
