@@ -902,8 +902,10 @@ static int aq_launch(AqParams p, void *ws, cudaStream_t st)
 {
     using S = AqShape<HD, BLOCKS>;
     static_assert(S::SMEM <= 227 * 1024, "shared memory");
-    const int N = ckb_sm_count() * S::CTAS;
     p.RC = (p.R + S::ROWS - 1) / S::ROWS;
+    // as many CTAs as can be resident, no more than units that the table has room for
+    const long long stretches = (long long)p.c.batch * p.c.Hkv * p.RC, units = stretches * ((p.c.stride * p.c.page_tokens + S::UNIT - 1) / S::UNIT);
+    const int most = ckb_sm_count() * S::CTAS, N = units < most ? (int)units : most;
     p.desc = (int2 *)ws;
     p.part = (float *)((uint8_t *)ws + aq_desc_bytes<HD, BLOCKS>(p.c.batch, p.c.Hkv, p.R));
     static bool attr_set = false;
@@ -913,9 +915,8 @@ static int aq_launch(AqParams p, void *ws, cudaStream_t st)
     }
     const int rc = launch_pdl("attention_q4cache", attn_q4_kernel<HD, BLOCKS>, dim3(N), dim3(AQ_THREADS), (size_t)S::SMEM, st, p);
     if (rc || p.c.stride * p.c.page_tokens <= S::UNIT) return rc;      // no stretch has two units
-    // 128 channels, the whole call by CTAs and by warps: 8 stretches of 55 parts 10.6 and 12.1 us, 16 of 27 13.8 and 15.0, 24 of 18 17.7 and 16.4, 32 of 14 18.4 and 16.6,
-    // 264 with 16 rows in two or three 46 and 42
-    const long long stretches = (long long)p.c.batch * p.c.Hkv * p.RC;
+    // 128 channels, the whole call by CTAs and by warps: 8 stretches of 32 parts 10.0 and 12.1 us, 16 of 27 13.0 and 14.8, 24 of 18 16.0 and 15.5, 32 of 14 16.8 and 16.0,
+    // 40 with 16 rows of 7 21.6 and 17.6
     const int rows = S::ROWS < p.R ? S::ROWS : p.R;
     if (stretches * 22 < N) return launch_pdl("attention_q4cache", attn_q4_merge_kernel<HD>, dim3((unsigned)stretches, rows), dim3(512 / HD * HD), 0, st, p, S::ROWS);
     return launch_pdl("attention_q4cache", attn_q4_merge_rows_kernel<HD>, dim3((unsigned)(stretches < N ? stretches : N), (rows + 3) / 4), dim3(128), 0, st, p, S::ROWS, rows);
