@@ -27,7 +27,7 @@
 // written out at once, the others as partial results that a second kernel joins (log-sum-exp).
 //
 // What bounds it.  Not HBM: the ring alone, without the arithmetic, takes 113 us for four sequences of 131072 tokens (64 heads over 8 of 128 channels,
-// 667 MB, 102 us at the measured copy rate), the whole kernel 218 us, 3.1 TB/s (32 heads: 190 us, 3.5 TB/s).  A chunk of 32 keys is 1005 warp instructions, 74 of them
+// 667 MB, 102 us at the measured copy rate), the whole kernel 218 us, 3.1 TB/s (32 heads: 188 us, 3.5 TB/s).  A chunk of 32 keys is 1005 warp instructions, 74 of them
 // products (38 with four rows), issued at 2.2 an SM and cycle: products, half-precision instructions and integer multiplications share one pipe, half-rate logic (codes, 300
 // instructions) has another, each is busy for 20 to 40 % of the time, and a warp waits 1.75 cycles an instruction for the one before it.
 // Two, three or four CTAs an SM (8 to 16 warps, 255 to 128 registers): 239 / 218 / 223 us.
@@ -55,6 +55,8 @@ struct AqShape {
     static constexpr int STAGE = 2 * CHUNK * ROW;                              // K rows, then V rows
     static constexpr int CTAS = NB > 1 && HD > 192 ? 1 : (NB > 1 || HD > 128 ? 2 : 3);                       // resident on an SM, for which registers and shared memory are kept
     static constexpr int STAGES = HD <= 64 ? 4 : (HD <= 128 && NB < 3 ? 3 : 2);
+    // the next stretch's queries load while one is joined, where there are registers: three blocks 96.7 us with it and 93.9 us without (20 rows of 16 sequences), four rows 190 and 188 us
+    static constexpr bool EARLY = !PACK && NB < 3;
     static constexpr int MINE = NB * G4 * 2;                                  // each warp joins a quarter of the four warps' accumulators; it gives away the others
     static constexpr int GIVEN = AQ_WARPS * (3 * MINE + 2 * NB) * 32 * 4;
     static constexpr int RING = AQ_WARPS * STAGES * STAGE, QF = NB * KS * 32 * 16, QS = NB * 32 * 8, EX = AQ_WARPS * NB * 8 * SP * 4, TAB = AQ_WARPS * 3 * G4 * 2 * CHUNK;
@@ -320,7 +322,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
         if (lane == 0) entry = look(f_pos, f_slot);
         for (int i = 0; i < STAGES - 1; ++i) fetch();
 
-        float qx[ROWS / AQ_WARPS][G4];                         // rows of a stretch's queries, on their way while the stretch before is joined
+        float qx[ROWS / AQ_WARPS][G4];                         // rows of a stretch's queries
         auto load_q = [&]() {
 #pragma unroll
             for (int i = 0; i < ROWS / AQ_WARPS; ++i) {
@@ -330,12 +332,13 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                 for (int j = 0; j < G4; ++j) qx[i][j] = row < p.R ? __ldcg(src + 32 * j + lane) : 0.0f;
             }
         };
-        load_q();
+        if (S::EARLY) load_q();
         int stage = 0;
         uint32_t phase = 0;
         for (int left = (int)(last - first); left;) {
             // ---- a stretch: query fragments of its rows
             const int r0 = w.rc * ROWS, u_first = w.u;
+            if (!S::EARLY) load_q();
             __syncthreads();                                   // the stretch before is done with them
 #pragma unroll
             for (int i = 0; i < ROWS / AQ_WARPS; ++i) {      // a warp per row, a lane the channels 4 (lane % 4 ..) of its blocks
@@ -660,7 +663,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
             float *part = whole ? nullptr : p.part + (size_t)(2 * me + (u_first == 0)) * ROWS * (HD + 2), *out = p.out + (long long)w.b * p.c.tokens * p.out_stride + (long long)w.h * p.G * HD;
             if (left) {
                 aq_next_stretch(p, ROWS, S::UNIT, w);
-                load_q();
+                if (S::EARLY) load_q();
             }
             const float unscale = __uint_as_float((uint32_t)(127 - b_run) << 23);
 #pragma unroll
@@ -930,8 +933,8 @@ static size_t aq_bytes(int batch, int Hkv, int R)
 }
 
 // Blocks of 8 query rows that share the codes a CTA unpacks; 0: up to four, with both pieces of a row in one product (32 heads over 8, four sequences of 131072
-// tokens 190 us, 217 us in a block of 8; 32 of up to 4096 48 and 53).  Three blocks leave no register free and are worth it only where they hold all the rows: 20 rows of
-// 16 sequences (five drafts, up to 8190 tokens) 99 us with three, 109 us one by one, 130 us with two and two; 516 rows 38 us in blocks of two, 42 us one by one, 41 us in threes.
+// tokens 188 us, 217 us in a block of 8; 32 of up to 4096 48 and 53).  Three blocks leave no register free and are worth it only where they hold all the rows: 20 rows of
+// 16 sequences (five drafts, up to 8190 tokens) 94 us with three, 109 us one by one, 130 us with two and two; 516 rows 38 us in blocks of two, 42 us one by one, 41 us in threes.
 static int aq_blocks(long long rows, int hd) { return rows <= 4 ? 0 : rows <= 8 ? 1 : (rows > 16 && rows <= 24 && hd <= 128 ? 3 : 2); }
 
 }  // namespace ckb
