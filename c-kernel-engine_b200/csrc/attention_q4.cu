@@ -15,6 +15,8 @@
 //
 //   scores  S^T = K Q^T   mma.m16n8k16: 16 keys x 8 query rows; a thread's A words are 4 bytes of codes of keys g and g + 8 (lane = 4 g + t), which
 //                         settles which channel sits at which k: the query's fragments are laid out to match
+//           from S^T to the operand P^T: a thread's weights of one key and two rows are a word of each piece, and a transpose of 8 x 8 halves between lanes makes
+//                         them those of one row and two keys
 //   output  O^T = V^T P^T 16 channels x 8 query rows; A words are the same two bytes (four channels) of two keys, joined by one byte permute
 //
 // A query row is a (token, head) of the kv head's group: up to 8 NB rows share every code that is unpacked (NB = 1 for decoding, more for
@@ -51,16 +53,15 @@ struct AqShape {
     static constexpr bool PACK = BLOCKS == 0;
     static constexpr int NB = PACK ? 1 : BLOCKS, G4 = HD / 32, KS = HD / 16, ROW = G4 * KQ4_BLOCK, ROWS = PACK ? 4 : 8 * NB;
     static constexpr int XT = 2, CHUNK = 16 * XT, UNIT = AQ_WARPS * CHUNK;      // a warp takes XT tiles of 16 keys at a time
-    static constexpr int SP = CHUNK + 8;                                          // floats between rows of the score exchange: 8 lanes' float2 loads touch every bank once
     static constexpr int STAGE = 2 * CHUNK * ROW;                              // K rows, then V rows
     static constexpr int CTAS = NB > 1 && HD > 192 ? 1 : (NB > 1 || HD > 128 ? 2 : 3);                       // resident on an SM, for which registers and shared memory are kept
     static constexpr int STAGES = HD <= 64 ? 4 : (HD <= 128 && NB < 3 ? 3 : 2);
     // the next stretch's queries load while one is joined, where there are registers: three blocks 96.7 us with it and 93.9 us without (20 rows of 16 sequences), four rows 190 and 188 us
     static constexpr bool EARLY = !PACK && NB < 3;
     static constexpr int MINE = NB * G4 * 2;                                  // each warp joins a quarter of the four warps' accumulators; it gives away the others
-    static constexpr int GIVEN = AQ_WARPS * (3 * MINE + 2 * NB) * 32 * 4;
-    static constexpr int RING = AQ_WARPS * STAGES * STAGE, QF = NB * KS * 32 * 16, QS = NB * 32 * 8, EX = AQ_WARPS * NB * 8 * SP * 4, TAB = AQ_WARPS * 3 * G4 * 2 * CHUNK;
-    static constexpr int SMEM = RING + (QF + QS + EX + TAB > GIVEN ? QF + QS + EX + TAB : GIVEN);      // the exchange between warps lies over the queries
+    static constexpr int GIVEN = AQ_WARPS * (3 * MINE * 32 + NB * 16) * 4;
+    static constexpr int RING = AQ_WARPS * STAGES * STAGE, QF = NB * KS * 32 * 16, QS = NB * 32 * 8, TAB = AQ_WARPS * 3 * G4 * 2 * CHUNK;
+    static constexpr int SMEM = RING + (QF + QS + TAB > GIVEN ? QF + QS + TAB : GIVEN);      // the exchange between warps lies over the queries
     static_assert(CTAS * (SMEM + 2048) <= 227 * 1024, "shared memory");
 };
 
@@ -146,6 +147,13 @@ __device__ __forceinline__ float aq_exp2(float x)
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));       // two units in the last place
     return y;
 }
+// of a matrix of 8 x 8 halves, thread 4 g + t: (row g, columns 2t, 2t + 1) in, (column g, rows 2t, 2t + 1) out
+__device__ __forceinline__ uint32_t aq_transpose(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 __device__ __forceinline__ uint32_t aq_u32(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
 __device__ __forceinline__ uint32_t aq_u16(const uint8_t *p) { return *reinterpret_cast<const uint16_t *>(p); }
 // nibble P of each half of the word, as 16 c * 2^-24
@@ -191,10 +199,9 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
     uint2 *qsum = reinterpret_cast<uint2 *>(aq_smem + S::RING + S::QF);           // [NB][lane] {hi, lo} sums of the scaled query over blocks 2t and 2t + 1, times 2^-6: both in fp16's normal range
     __shared__ float q_factor[ROWS];
     float *given = reinterpret_cast<float *>(aq_smem + S::RING), *given_ref = given + AQ_WARPS * 3 * S::MINE * 32;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, g_row = PACK ? g & 3 : g;
-    float *ex = reinterpret_cast<float *>(aq_smem + S::RING + S::QF + S::QS) + warp * NB * 8 * S::SP;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, col = PACK ? 2 * t & 3 : 2 * t;      // a thread has query rows col and col + 1 of each block
     // for each key of the warp's chunk: d times 2^b, and the middle m + 8 d of the values that a block can say, as two pieces; [G4][keys] halves each
-    __half *tab = reinterpret_cast<__half *>(aq_smem + S::RING + S::QF + S::QS + S::EX) + warp * 3 * G4 * S::CHUNK;
+    __half *tab = reinterpret_cast<__half *>(aq_smem + S::RING + S::QF + S::QS) + warp * 3 * G4 * S::CHUNK;
     const int tab_at = (lane & 16) | (lane & 6) << 1 | (lane & 8) >> 2 | (lane & 1);      // keys 2t, 2t + 1, 2t + 8 and 2t + 9 of a tile side by side: one load for a thread
     const int N = gridDim.x, me = blockIdx.x;
 
@@ -378,16 +385,18 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
             }
             __syncthreads();
             float om[NB][2];                                   // row g: block g's sum of weight times middle
-            float o[NB][G4][2][4], m_run[NB], l_run[NB], fac[NB];      // m_run: the reference of the weights, in powers of two
-            int pos_row[NB], b_run = 14;                       // pos_row: the position of row g of each block, -1 where there is none
+            float o[NB][G4][2][4], m_run[NB][2], l_run[NB][2], fac[NB][2];      // m_run: the reference of the weights, in powers of two; l_run: of this thread's keys
+            int pos_row[NB][2], b_run = 14;                    // pos_row: the position of a row, -1 where there is none
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                const int row = r0 + 8 * nb + g_row;
-                pos_row[nb] = row < p.R ? w.len - p.c.tokens + p.by_group(row) : -1;
-                fac[nb] = q_factor[8 * nb + g_row];
-                m_run[nb] = -INFINITY;
-                l_run[nb] = 0.0f;
-                om[nb][0] = om[nb][1] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = r0 + 8 * nb + col + e;
+                    pos_row[nb][e] = row < p.R ? w.len - p.c.tokens + p.by_group(row) : -1;
+                    fac[nb][e] = q_factor[8 * nb + col + e];
+                    m_run[nb][e] = -INFINITY;
+                    l_run[nb][e] = om[nb][e] = 0.0f;
+                }
 #pragma unroll
                 for (int e = 0; e < G4 * 8; ++e) o[nb][e >> 3][e >> 2 & 1][e & 3] = 0.0f;
             }
@@ -428,7 +437,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                                     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                                         for (int e = 0; e < 2; ++e) {
-                                            const int pos = __shfl_sync(0xffffffffu, pos_row[nb], 4 * (2 * t + e));
+                                            const int pos = pos_row[nb][e];
                                             if (at_key <= pos && (p.window == 0 || at_key > pos - p.window))
 #pragma unroll
                                                 for (int x = 0; x < 2; ++x) o[nb][j][x][e] = o[nb][j][x][e + 2] = __int_as_float(0x7fffffff);
@@ -455,8 +464,8 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                             tab[(2 * G4 + j) * S::CHUNK + 32 * y + tab_at] = lo;
                         }
                     // ---- scores of tiles of 16 keys.  A product waits long for the one before it in its sum: those of several tiles and blocks take turns.
+                    float s[S::XT][NB][4];                     // keys 16 x + g and 8 further on, rows col and col + 1
                     {
-                        float s[S::XT][NB][4];
                         const uint8_t *key_row = kb + g * ROW;
 #pragma unroll
                         for (int x = 0; x < S::XT; ++x) {
@@ -513,70 +522,78 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                                     for (int e = 0; e < 4; ++e) s[x][nb][e] = fmaf(d[x][e >> 1], acc[x][e], s[x][nb][e]);
                             }
                         }
-#pragma unroll
-                        for (int x = 0; x < S::XT; ++x)
-#pragma unroll
-                            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) ex[(nb * 8 + 2 * t + (e & 1)) * S::SP + 16 * x + 8 * (e >> 1) + g] = s[x][nb][e];
                     }
-                    __syncwarp();
-
-                    // ---- from (keys g, rows 2t) to (row g, keys 2t): weights times 2^10, as two pieces
-                    uint32_t ph[NB][2 * S::XT], pl[NB][2 * S::XT];             // keys 8y + 2t and 8y + 2t + 1
-                    float alpha[NB];
+                    // ---- weights times 2^10, as two pieces.  The reference follows the maximum when that is more than 2^3 ahead: each time costs every accumulator a product,
+                    // and only then the maximum over the keys is found.
                     bool moved = b_new != b_run;
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
-                        float2 v[2 * S::XT];
-                        float top = -INFINITY;
+                        if constexpr (PACK) {                  // what hi and lo pieces gave, columns c and c + 4
 #pragma unroll
-                        for (int y = 0; y < 2 * S::XT; ++y) {
-                            v[y] = *reinterpret_cast<const float2 *>(ex + (nb * 8 + g_row) * S::SP + 8 * y + 2 * t);
-                            if constexpr (PACK) {
-                                const float2 rest = *reinterpret_cast<const float2 *>(ex + (g_row + 4) * S::SP + 8 * y + 2 * t);
-                                v[y].x += rest.x;
-                                v[y].y += rest.y;
-                            }
-                            if (mixed) {
-                                const int key = key0 + 8 * y + 2 * t, from = p.window > 0 ? pos_row[nb] - p.window : -1;
-                                const bool page = there >> (y >> 1) & 1u;
-                                if (!page || key > pos_row[nb] || key <= from) v[y].x = -INFINITY;
-                                if (!page || key + 1 > pos_row[nb] || key + 1 <= from) v[y].y = -INFINITY;
-                            }
-                            top = fmaxf(top, fmaxf(v[y].x, v[y].y));
-                        }
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                        // the reference follows the maximum when it is more than 2^3 behind: each time costs every accumulator a product
-                        top *= fac[nb];
-                        const bool far = top > m_run[nb] + 3.0f;
-                        const float m_new = far ? top : m_run[nb];
-                        moved |= far;
-                        const float ref = m_new == -INFINITY ? 0.0f : m_new;
-                        alpha[nb] = m_run[nb] == -INFINITY ? 0.0f : aq_exp2(m_run[nb] - ref);
-                        m_run[nb] = m_new;
-                        float sum = 0.0f;
+                            for (int x = 0; x < S::XT; ++x)
 #pragma unroll
-                        for (int y = 0; y < 2 * S::XT; ++y) {
-                            const float2 e = make_float2(aq_exp2(fmaf(v[y].x, fac[nb], 10.0f - ref)), aq_exp2(fmaf(v[y].y, fac[nb], 10.0f - ref)));
-                            sum += e.x + e.y;
-                            aq_split(e, ph[nb][y], pl[nb][y]);
+                                for (int e = 0; e < 4; ++e) s[x][nb][e] += __shfl_xor_sync(0xffffffffu, s[x][nb][e], 2);
                         }
-                        l_run[nb] = fmaf(l_run[nb], alpha[nb], sum);
+                        if (mixed) {
+#pragma unroll
+                            for (int x = 0; x < S::XT; ++x)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const int key = key0 + 16 * x + 8 * (e >> 1) + g, pos = pos_row[nb][e & 1];
+                                    if (!(there >> x & 1u) || key > pos || (p.window > 0 && key <= pos - p.window)) s[x][nb][e] = -INFINITY;
+                                }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float top = -INFINITY;
+#pragma unroll
+                            for (int x = 0; x < S::XT; ++x) top = fmaxf(top, fmaxf(s[x][nb][e], s[x][nb][e + 2]));
+                            moved |= top * fac[nb][e] > m_run[nb][e] + 3.0f;
+                        }
                     }
                     if (__any_sync(0xffffffffu, moved)) {      // rare once the first keys have been seen
                         const float shift = __uint_as_float((uint32_t)(127 + b_new - b_run) << 23);
+                        b_run = b_new;
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
-                            const float f0 = __shfl_sync(0xffffffffu, alpha[nb], 8 * t), f1 = __shfl_sync(0xffffffffu, alpha[nb], 8 * t + 4);
-                            om[nb][0] *= f0;
-                            om[nb][1] *= f1;
+                            float alpha[2];
 #pragma unroll
-                            for (int e = 0; e < G4 * 8; ++e) o[nb][e >> 3][e >> 2 & 1][e & 3] *= (e & 1 ? f1 : f0) * shift;
+                            for (int e = 0; e < 2; ++e) {
+                                float top = -INFINITY;
+#pragma unroll
+                                for (int x = 0; x < S::XT; ++x) top = fmaxf(top, fmaxf(s[x][nb][e], s[x][nb][e + 2]));
+#pragma unroll
+                                for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                                top *= fac[nb][e];
+                                const float m_new = top > m_run[nb][e] + 3.0f ? top : m_run[nb][e];
+                                alpha[e] = m_run[nb][e] == -INFINITY ? 0.0f : aq_exp2(m_run[nb][e] - m_new);
+                                m_run[nb][e] = m_new;
+                                l_run[nb][e] *= alpha[e];
+                                om[nb][e] *= alpha[e];
+                                alpha[e] *= shift;
+                            }
+#pragma unroll
+                            for (int e = 0; e < G4 * 8; ++e) o[nb][e >> 3][e >> 2 & 1][e & 3] *= alpha[e & 1];
                         }
-                        b_run = b_new;
                     }
+                    uint32_t ph[NB][2 * S::XT], pl[NB][2 * S::XT];             // of row g: keys 8y + 2t and 8y + 2t + 1
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const float c0 = 10.0f - (m_run[nb][0] == -INFINITY ? 0.0f : m_run[nb][0]), c1 = 10.0f - (m_run[nb][1] == -INFINITY ? 0.0f : m_run[nb][1]);
+                        float sum0 = 0.0f, sum1 = 0.0f;        // of the chunk: a long sequence's sum rounds once a chunk
+#pragma unroll
+                        for (int y = 0; y < 2 * S::XT; ++y) {
+                            const float2 e = make_float2(aq_exp2(fmaf(s[y >> 1][nb][2 * (y & 1)], fac[nb][0], c0)), aq_exp2(fmaf(s[y >> 1][nb][2 * (y & 1) + 1], fac[nb][1], c1)));
+                            sum0 += e.x;
+                            sum1 += e.y;
+                            aq_split(e, ph[nb][y], pl[nb][y]);
+                            ph[nb][y] = aq_transpose(ph[nb][y]);
+                            pl[nb][y] = aq_transpose(pl[nb][y]);
+                        }
+                        l_run[nb][0] += sum0;
+                        l_run[nb][1] += sum1;
+                    }
+                    __syncwarp();                              // the table below is complete
                     // ---- values.  The tensor cores cut what they add to an accumulator instead of rounding it: a chunk's sums start from zero and are
                     // added up by the rounding adder, and codes are taken from their middle, so that the terms do not all have one sign.
                     const uint8_t *at_t = reinterpret_cast<const uint8_t *>(tab) + 8 * t;
@@ -650,7 +667,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                             for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] += acc[nb][e >> 2][e & 3];
                     }
                 }
-                __syncwarp();                                  // the stage and its word, the exchange and the table are free again
+                __syncwarp();                                  // the stage and its word and the table are free again
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 --left;
                 if (++w.u >= w.n || left == 0) break;
@@ -668,8 +685,11 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
             const float unscale = __uint_as_float((uint32_t)(127 - b_run) << 23);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                l_run[nb] += __shfl_xor_sync(0xffffffffu, l_run[nb], 1);
-                l_run[nb] += __shfl_xor_sync(0xffffffffu, l_run[nb], 2);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) {
+                    l_run[nb][0] += __shfl_xor_sync(0xffffffffu, l_run[nb][0], d);
+                    l_run[nb][1] += __shfl_xor_sync(0xffffffffu, l_run[nb][1], d);
+                }
 #pragma unroll
                 for (int j = 0; j < G4; ++j) {
                     const float a0 = __shfl_sync(0xffffffffu, om[nb][0], 4 * j + t), a1 = __shfl_sync(0xffffffffu, om[nb][1], 4 * j + t);
@@ -697,47 +717,47 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                     }
             }
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                given_ref[(warp * NB + nb) * 64 + lane] = m_run[nb];
-                given_ref[(warp * NB + nb) * 64 + 32 + lane] = l_run[nb];
-            }
+            for (int nb = 0; nb < NB; ++nb)
+                if (g == 0) *reinterpret_cast<float4 *>(given_ref + (warp * NB + nb) * 16 + 4 * t) = make_float4(m_run[nb][0], l_run[nb][0], m_run[nb][1], l_run[nb][1]);
             __syncthreads();
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                float ref[AQ_WARPS], f[AQ_WARPS], both = -INFINITY, l = 0.0f, sum[G4 * 2];
+                float4 ref[AQ_WARPS];                          // reference and sum of the two rows
+                float both[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, f[AQ_WARPS][2], sum[G4 * 2];
 #pragma unroll
                 for (int s = 0; s < AQ_WARPS; ++s) {
-                    ref[s] = given_ref[(s * NB + nb) * 64 + lane];
-                    both = fmaxf(both, ref[s]);
+                    ref[s] = *reinterpret_cast<const float4 *>(given_ref + (s * NB + nb) * 16 + 4 * t);
+                    both[0] = fmaxf(both[0], ref[s].x);
+                    both[1] = fmaxf(both[1], ref[s].z);
                 }
 #pragma unroll
                 for (int s = 0; s < AQ_WARPS; ++s) {
-                    f[s] = ref[s] == -INFINITY ? 0.0f : aq_exp2(ref[s] - both);
-                    l = fmaf(f[s], given_ref[(s * NB + nb) * 64 + 32 + lane], l);
+                    f[s][0] = ref[s].x == -INFINITY ? 0.0f : aq_exp2(ref[s].x - both[0]);
+                    f[s][1] = ref[s].z == -INFINITY ? 0.0f : aq_exp2(ref[s].z - both[1]);
+                    l[0] = fmaf(f[s][0], ref[s].y, l[0]);
+                    l[1] = fmaf(f[s][1], ref[s].w, l[1]);
                 }
 #pragma unroll
                 for (int e = 0; e < G4 * 2; ++e) sum[e] = 0.0f;
 #pragma unroll
                 for (int s = 0; s < AQ_WARPS; ++s) {           // in the same order whichever warp joins
-                    const float fa = __shfl_sync(0xffffffffu, f[s], 8 * t), fb = __shfl_sync(0xffffffffu, f[s], 8 * t + 4);
                     const float *from = given_by(s, warp) + nb * G4 * 2 * 32;
 #pragma unroll
                     for (int e = 0; e < G4 * 2; ++e) {
                         float x;
                         if (s == warp) x = o[nb][(s * G4 * 2 + e) >> 3][(s * G4 * 2 + e) >> 2 & 1][(s * G4 * 2 + e) & 3];
                         else x = from[e * 32];
-                        sum[e] = fmaf(e & 1 ? fb : fa, x, sum[e]);
+                        sum[e] = fmaf(f[s][e & 1], x, sum[e]);
                     }
-                }
-                if (part && warp == 0 && t == 0 && 8 * nb + g < ROWS) {
-                    part[(8 * nb + g) * (HD + 2) + HD] = both;
-                    part[(8 * nb + g) * (HD + 2) + HD + 1] = l;
                 }
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int r = 8 * nb + 2 * t + e, row = r0 + r, tok = p.by_group(row);
-                    const float row_l = __shfl_sync(0xffffffffu, l, 8 * t + 4 * e);
-                    const float inv = row_l == 0.0f ? 0.0f : 1.0f / row_l;
+                    const float inv = l[e] == 0.0f ? 0.0f : 1.0f / l[e];
+                    if (part && warp == 0 && g == 0 && r < ROWS) {
+                        part[r * (HD + 2) + HD] = both[e];
+                        part[r * (HD + 2) + HD + 1] = l[e];
+                    }
                     if (r >= ROWS || row >= p.R) continue;
                     float *to = part ? part + r * (HD + 2) : out + tok * p.out_stride + (long long)(row - tok * p.G) * HD;
 #pragma unroll
