@@ -29,9 +29,9 @@
 // written out at once, the others as partial results that a second kernel joins (log-sum-exp).
 //
 // What bounds it.  Not HBM: the ring alone, without the arithmetic, takes 113 us for four sequences of 131072 tokens (64 heads over 8 of 128 channels,
-// 667 MB, 102 us at the measured copy rate), the whole kernel 218 us, 3.1 TB/s (32 heads: 188 us, 3.5 TB/s).  A chunk of 32 keys is 1005 warp instructions, 74 of them
+// 667 MB, 102 us at the measured copy rate), the whole kernel 218 us, 3.1 TB/s (32 heads: 180 us, 3.7 TB/s).  A chunk of 32 keys is 1004 warp instructions, 74 of them
 // products (38 with four rows), issued at 2.2 an SM and cycle: products, half-precision instructions and integer multiplications share one pipe, half-rate logic (codes, 300
-// instructions) has another, each is busy for 20 to 40 % of the time, and a warp waits 1.75 cycles an instruction for the one before it.
+// instructions) has another, each is busy for 20 to 40 % of the time, and a warp waits 1.8 cycles an instruction for the one before it.
 // Two, three or four CTAs an SM (8 to 16 warps, 255 to 128 registers): 239 / 218 / 223 us.
 #include <cuda_fp16.h>
 #include <math.h>
@@ -953,7 +953,7 @@ static size_t aq_bytes(int batch, int Hkv, int R)
 }
 
 // Blocks of 8 query rows that share the codes a CTA unpacks; 0: up to four, with both pieces of a row in one product (32 heads over 8, four sequences of 131072
-// tokens 188 us, 217 us in a block of 8; 32 of up to 4096 48 and 53).  Three blocks leave no register free and are worth it only where they hold all the rows: 20 rows of
+// tokens 180 us, 217 us in a block of 8; 32 of up to 4096 46 and 53).  Three blocks leave no register free and are worth it only where they hold all the rows: 20 rows of
 // 16 sequences (five drafts, up to 8190 tokens) 94 us with three, 109 us one by one, 130 us with two and two; 516 rows 38 us in blocks of two, 42 us one by one, 41 us in threes.
 static int aq_blocks(long long rows, int hd) { return rows <= 4 ? 0 : rows <= 8 ? 1 : (rows > 16 && rows <= 24 && hd <= 128 ? 3 : 2); }
 
