@@ -29,10 +29,10 @@
 // written out at once, the others as partial results that a second kernel joins (log-sum-exp).
 //
 // What bounds it.  Not HBM: the ring alone, without the arithmetic, takes 113 us for four sequences of 131072 tokens (64 heads over 8 of 128 channels,
-// 667 MB, 102 us at the measured copy rate), the whole kernel 218 us, 3.1 TB/s (32 heads: 180 us, 3.7 TB/s).  A chunk of 32 keys is 1004 warp instructions, 74 of them
+// 667 MB, 102 us at the measured copy rate), the whole kernel 210 us, 3.2 TB/s (32 heads: 180 us, 3.7 TB/s).  A chunk of 32 keys is 1004 warp instructions, 74 of them
 // products (38 with four rows), issued at 2.2 an SM and cycle: products, half-precision instructions and integer multiplications share one pipe, half-rate logic (codes, 300
 // instructions) has another, each is busy for 20 to 40 % of the time, and a warp waits 1.8 cycles an instruction for the one before it.
-// Two, three or four CTAs an SM (8 to 16 warps, 255 to 128 registers): 239 / 218 / 223 us.
+// Two, three or four CTAs an SM (8 to 16 warps, 255 to 128 registers): 239 / 218 / 210 us.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -47,15 +47,15 @@ namespace ckb {
 
 constexpr int AQ_WARPS = 4, AQ_THREADS = 32 * AQ_WARPS;
 
-// BLOCKS 0: up to four query rows, whose hi pieces are columns 0 .. 3 of a product and whose lo pieces are columns 4 .. 7
+// BLOCKS 4: one block and four CTAs an SM, for long caches; 0: up to four query rows, whose hi pieces are columns 0 .. 3 of a product and whose lo pieces are columns 4 .. 7
 template <int HD, int BLOCKS>
 struct AqShape {
-    static constexpr bool PACK = BLOCKS == 0;
-    static constexpr int NB = PACK ? 1 : BLOCKS, G4 = HD / 32, KS = HD / 16, ROW = G4 * KQ4_BLOCK, ROWS = PACK ? 4 : 8 * NB;
+    static constexpr bool PACK = BLOCKS == 0, FOUR = BLOCKS == 4;
+    static constexpr int NB = PACK || FOUR ? 1 : BLOCKS, G4 = HD / 32, KS = HD / 16, ROW = G4 * KQ4_BLOCK, ROWS = PACK ? 4 : 8 * NB;
     static constexpr int XT = 2, CHUNK = 16 * XT, UNIT = AQ_WARPS * CHUNK;      // a warp takes XT tiles of 16 keys at a time
     static constexpr int STAGE = 2 * CHUNK * ROW;                              // K rows, then V rows
-    static constexpr int CTAS = NB > 1 && HD > 192 ? 1 : (NB > 1 || HD > 128 ? 2 : 3);                       // resident on an SM, for which registers and shared memory are kept
-    static constexpr int STAGES = HD <= 64 ? 4 : (HD <= 128 && NB < 3 ? 3 : 2);
+    static constexpr int CTAS = NB > 1 && HD > 192 ? 1 : (NB > 1 || HD > 128 ? 2 : (FOUR ? 4 : 3));                       // resident on an SM, for which registers and shared memory are kept
+    static constexpr int STAGES = HD <= 64 ? 4 : (HD <= 128 && NB < 3 && !FOUR ? 3 : 2);
     // the next stretch's queries load while one is joined, where there are registers: three blocks 96.7 us with it and 93.9 us without (20 rows of 16 sequences), four rows 190 and 188 us
     static constexpr bool EARLY = !PACK && NB < 3;
     static constexpr int MINE = NB * G4 * 2;                                  // each warp joins a quarter of the four warps' accumulators; it gives away the others
@@ -957,6 +957,11 @@ static size_t aq_bytes(int batch, int Hkv, int R)
 // 16 sequences (five drafts, up to 8190 tokens) 94 us with three, 109 us one by one, 130 us with two and two; 516 rows 38 us in blocks of two, 42 us one by one, 41 us in threes.
 static int aq_blocks(long long rows, int hd) { return rows <= 4 ? 0 : rows <= 8 ? 1 : (rows > 16 && rows <= 24 && hd <= 128 ? 3 : 2); }
 
+// Eight rows of 128 channels: four CTAs an SM, with 128 registers a thread, hide more of the waiting than three with 168, but take longer for a chunk: 210 and 218 us for four sequences
+// of 131072 tokens, 53 and 54 us for 32 of up to 4096, 40 and 44 us for 48 of up to 2047, but 35 and 35 us for 16 of up to 4096, 24 and 23 us for 8, 19 and 16 us for 4, 76 and 72 us for 256 of up to
+// 600.  So they are taken where the table has room for eight units a CTA and sixteen a stretch.
+static bool aq_four(long long stretches, int units, int hd) { return hd == 128 && units >= 16 && stretches * units >= 8LL * 4 * ckb_sm_count(); }
+
 }  // namespace ckb
 
 using namespace ckb;
@@ -964,14 +969,15 @@ using namespace ckb;
 #define AQ_EACH(hd, nb, F)                                                                                              \
     (hd == 64 ? (nb == 0 ? F<64, 0> : nb == 1 ? F<64, 1> : nb == 2 ? F<64, 2> : F<64, 3>)                               \
      : hd == 96 ? (nb == 0 ? F<96, 0> : nb == 1 ? F<96, 1> : nb == 2 ? F<96, 2> : F<96, 3>)                             \
-     : hd == 128 ? (nb == 0 ? F<128, 0> : nb == 1 ? F<128, 1> : nb == 2 ? F<128, 2> : F<128, 3>)                        \
+     : hd == 128 ? (nb == 0 ? F<128, 0> : nb == 1 ? F<128, 1> : nb == 2 ? F<128, 2> : nb == 3 ? F<128, 3> : F<128, 4>)                        \
      : hd == 192 ? (nb == 0 ? F<192, 0> : nb == 1 ? F<192, 1> : F<192, 2>)                                              \
                  : (nb == 0 ? F<256, 0> : nb == 1 ? F<256, 1> : F<256, 2>))
 
 extern "C" size_t ckb200_attention_q4cache_workspace_bytes(int batch, int num_tokens, int num_heads, int num_kv_heads, int head_dim)
 {
     if (batch <= 0 || num_tokens <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads || (long long)batch * num_tokens * num_heads > 1 << 30 || !ckb200_kv_q4_page_bytes(1, 16, head_dim)) return 0;
-    const int nb = aq_blocks((long long)num_tokens * (num_heads / num_kv_heads), head_dim);
+    int nb = aq_blocks((long long)num_tokens * (num_heads / num_kv_heads), head_dim);
+    if (nb == 1 && head_dim == 128) nb = 4;                    // whichever the call takes: four CTAs an SM need more
     return AQ_EACH(head_dim, nb, aq_bytes)(batch, num_kv_heads, num_tokens * (num_heads / num_kv_heads));
 }
 
@@ -1011,6 +1017,7 @@ extern "C" int ckb200_dev_attention_q4cache(const float *q, long long q_stride, 
     p.err = ckb_device_error_word();
     p.by_page = kv_divide((uint32_t)page_tokens);
     p.by_group = kv_divide((uint32_t)p.G);
-    const int nb = aq_blocks(p.R, head_dim);
+    int nb = aq_blocks(p.R, head_dim);
+    if (nb == 1 && aq_four((long long)batch * num_kv_heads, (table_stride * page_tokens + 127) / 128, head_dim)) nb = 4;
     return AQ_EACH(head_dim, nb, aq_launch)(p, workspace, ckb_stream(stream));
 }

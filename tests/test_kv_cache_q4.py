@@ -283,6 +283,8 @@ ATTENTION_CASES = [
     (5, 1, 256, 16, [4500], 1, 2 ** 31 - 1),
     # the same with several blocks of query rows and kv heads, and a stretch in a dozen parts
     (16, 4, 64, 16, [(29 * i) % 61 for i in range(150)], 9, 20), (3, 3, 96, 16, [(31 * i) % 50 for i in range(200)], 3, 0), (24, 24, 64, 16, [2400], 1, 0), (24, 12, 128, 32, [1300, 5, 1299], 4, 0),
+    # tables with room for so much that four CTAs an SM are taken
+    (40, 8, 128, 16, [2100] + [(13 * i) % 90 for i in range(40)], 1, 0), (16, 8, 128, 64, [9, 4200, 0] + [(17 * i) % 70 for i in range(25)], 3, 700),
     (16, 2, 64, 16, [300, 90], 17, 40), (2, 2, 128, 16, [130], 130, 16), (4, 1, 128, 16, [3000, 5, 2049], 1, 0), (8, 8, 64, 256, [2500], 3, 2048), (4, 1, 128, 64, [50], 100, 0),
 ]
 
