@@ -29,9 +29,9 @@
 // written out at once, the others as partial results that a second kernel joins (log-sum-exp).
 //
 // What bounds it.  Not HBM: the ring alone, without the arithmetic, takes 113 us for four sequences of 131072 tokens (64 heads over 8 of 128 channels,
-// 667 MB, 102 us at the measured copy rate), the whole kernel 210 us, 3.2 TB/s (32 heads: 180 us, 3.7 TB/s).  A chunk of 32 keys is 1004 warp instructions, 74 of them
-// products (38 with four rows), issued at 2.2 an SM and cycle: products, half-precision instructions and integer multiplications share one pipe, half-rate logic (codes, 300
-// instructions) has another, each is busy for 20 to 40 % of the time, and a warp waits 1.8 cycles an instruction for the one before it.
+// 667 MB, 102 us at the measured copy rate), the whole kernel 210 us, 3.2 TB/s (32 heads: 180 us, 3.7 TB/s).  A chunk of 32 keys is 1060 warp instructions, 74 of them
+// products (38 with four rows), issued at 2.5 an SM and cycle: products, half-precision instructions and integer multiplications share one pipe, half-rate logic (codes, 300
+// instructions) has another, each is busy for 20 to 40 % of the time, and a warp waits 1.7 cycles an instruction for the one before it.
 // Two, three or four CTAs an SM (8 to 16 warps, 255 to 128 registers): 239 / 218 / 210 us.
 #include <cuda_fp16.h>
 #include <math.h>
