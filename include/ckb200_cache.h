@@ -93,7 +93,7 @@ int ckb200_dev_kv_pages_resize(int *page_table, int table_stride, int *kv_lens, 
 int ckb200_dev_kv_pages_fork(int *page_table, int table_stride, int *kv_lens, int *page_refs, const int *parent, int batch, int num_pages, int page_tokens,
                              void *workspace, size_t workspace_bytes, void *stream);
 /* With L pages in use, the pages numbered L and above that are in use move, in their order, to the free ones below L; tables and references follow.
- * *live (may be NULL) becomes L: the pool's pages from L on hold nothing. */
+ * *live (may be NULL) becomes L: the pool's pages from L on hold nothing.  With batch 0 nothing is done, as in every call here: *live stays as it is. */
 int ckb200_dev_kv_pages_compact(int *page_table, int table_stride, const int *kv_lens, int *page_refs, int batch, int num_pages, int page_tokens, void *pages,
                                 int planes, long long plane_stride, long long page_bytes, int *live, void *workspace, size_t workspace_bytes, void *stream);
 

@@ -316,3 +316,14 @@ def test_a_conversation(gpu):  # noqa: F811
         call.compact()
     told[1] = [r[:0] for r in told[1]]
     step([45, 1, 44, 24], 1)                                    # the freed one begins anew
+
+
+@pytest.mark.gpu
+def test_compacting_no_sequences_leaves_live_alone(gpu):  # noqa: F811
+    m, d = make(gpu, np.random.default_rng(3), 2, 3, 9, 16)
+    for call in (m, d):
+        call.resize([20, 40])
+        call.resize([0, 40])
+    assert gpu.ckb200_dev_kv_pages_compact(*d.tables(), 0, d.pages, m.pt, *d.whole(), d.live.data_ptr(), *d.space(None)) == 0
+    d.same()
+    assert int(d.live) == 77
