@@ -319,6 +319,39 @@ def test_a_conversation(gpu):  # noqa: F811
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch,stride,pages,page_tokens,free", [(3, 4, 30, 16, None), (40, 6, 200, 48, None), (1700, 3, 5000, 16, None), (4096, 2, 8192, 16, None), (4096, 2, 8193, 16, None),
+                                                                 (700, 9, 9000, 16, None), (40, 180, 200, 48, 30), (60, 9000, 9000, 16, 40), (1700, 3, 1500, 16, None), (4096, 2, 3900, 16, None)])
+def test_shared_pages_are_copied(gpu, batch, stride, pages, page_tokens, free):  # noqa: F811
+    """A few prompts in all sequences, each continued: every one but the last that names a prompt's partial page gets a copy of it, counted here.  With little room (a small pool, or
+    one sequence that holds all but `free` pages) some are refused and the others copied one by one."""
+    rng = np.random.default_rng(batch + pages)
+    prompts = max(1, batch // 50)
+    m, d = make(gpu, rng, batch, stride, pages, page_tokens, planes=1, page_bytes=32)
+    first = np.where(np.arange(batch) < prompts, rng.integers(1, page_tokens, batch) + page_tokens * rng.integers(0, min(stride, 4) - 1, batch), 0)
+    parent = np.where(np.arange(batch) < prompts, -1, rng.integers(0, prompts, batch))
+    if free:
+        parent[-1] = -1
+    for call, arg in (("resize", first), ("fork", parent)):
+        getattr(m, call)(arg)
+        getattr(d, call)(arg)
+    new = np.full(batch, -1)
+    if free:
+        new[-1] = (int((m.refs == 0).sum()) - free) * page_tokens
+        assert not m.resize(new)[-1]
+        d.resize(new)
+    d.same()
+    before, lens = m.table.copy(), m.lens.copy()
+    new = np.minimum(lens + 1 + page_tokens * (np.arange(batch) % 3 == 0), stride * page_tokens)
+    want = m.resize(new)
+    d.resize(new)
+    d.same()
+    assert np.array_equal(d.status.cpu().numpy(), want)
+    last = np.maximum(lens - 1, 0) // page_tokens
+    copies = int((m.table[np.arange(batch), last] != before[np.arange(batch), last]).sum())
+    assert copies >= (20 if batch > 3 else 2) and want.any() == (free is not None or pages < batch)
+
+
+@pytest.mark.gpu
 def test_compacting_no_sequences_leaves_live_alone(gpu):  # noqa: F811
     m, d = make(gpu, np.random.default_rng(3), 2, 3, 9, 16)
     for call in (m, d):
