@@ -11,7 +11,7 @@
 //   * Value codes are taken from their middle.  With c in place of c - 8 all terms of the sum have one sign, the tensor cores cut what they add to an accumulator
 //     instead of rounding it, and the error adds up: 2.3e-5 of the result at 131072 keys, 7e-7 as it is here.
 //   * Ranges: queries are scaled so that the largest of a row is in [2^14, 2^15), weights, relative to a reference that may lag 2^3 behind the largest, by 2^10, steps d by
-//     2^b with the largest of them so far in [1, 2): no piece falls out of fp16's range whatever the cache's magnitude.  A weight times a step is a rounded half-precision product and its exact remainder.
+//     2^b with the largest of them so far in [1, 2), middles, which reach 9 * 65504, so that the chunk's largest |m| + 8 |d| is in [2^14, 2^15): no piece passes fp16's range.  A weight times a step is a rounded half-precision product and its exact remainder.
 //
 //   scores  S^T = K Q^T   mma.m16n8k16: 16 keys x 8 query rows; a thread's A words are 4 bytes of codes of keys g and g + 8 (lane = 4 g + t), which
 //                         settles which channel sits at which k: the query's fragments are laid out to match
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
     __shared__ float q_factor[ROWS];
     float *given = reinterpret_cast<float *>(aq_smem + S::RING), *given_ref = given + AQ_WARPS * 3 * S::MINE * 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, col = PACK ? 2 * t & 3 : 2 * t;      // a thread has query rows col and col + 1 of each block
-    // for each key of the warp's chunk: d times 2^b, and the middle m + 8 d of the values that a block can say, as two pieces; [G4][keys] halves each
+    // for each key of the warp's chunk: d times 2^b, and the middle m + 8 d of the values that a block can say, scaled too, as two pieces; [G4][keys] halves each
     __half *tab = reinterpret_cast<__half *>(aq_smem + S::RING + S::QF + S::QS) + warp * 3 * G4 * S::CHUNK;
     const int tab_at = (lane & 16) | (lane & 6) << 1 | (lane & 8) >> 2 | (lane & 1);      // keys 2t, 2t + 1, 2t + 8 and 2t + 9 of a tile side by side: one load for a thread
     const int N = gridDim.x, me = blockIdx.x;
@@ -453,11 +453,19 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                     // the largest d so far times 2^b is in [1, 2): its products with weights of up to 2^13 stay in fp16's range, their remainders above its least step
                     const int b_new = min(b_run, 15 - (int)min(29u, max(1u, __reduce_max_sync(0xffffffffu, dtop) >> 10)));
                     const __half2 d_scale = aq_h2((uint32_t)(15 + b_new) << 10);
+                    // Middles reach nine times the largest half: the chunk's largest |m| + 8 |d|, below 2^20, is brought into [2^14, 2^15), their products back again.
+                    float size = 0.0f;
+#pragma unroll
+                    for (int y = 0; y < KL; ++y)
+#pragma unroll
+                        for (int j = 0; j < G4; ++j) size = fmaxf(size, fabsf(aq_hi(dm[y][j])) + 8.0f * fabsf(aq_lo(dm[y][j])));
+                    const int size_ex = max(127 - 24, min(127 + 19, (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(size)) >> 23)));
+                    const float mid_up = __uint_as_float((uint32_t)(127 + 14 + 127 - size_ex) << 23), mid_down = __uint_as_float((uint32_t)(size_ex - 14) << 23);
 #pragma unroll
                     for (int y = 0; y < KL; ++y)
 #pragma unroll
                         for (int j = 0; j < G4; ++j) {
-                            const float mid = fmaf(8.0f, aq_lo(dm[y][j]), aq_hi(dm[y][j]));
+                            const float mid = fmaf(8.0f, aq_lo(dm[y][j]), aq_hi(dm[y][j])) * mid_up;
                             const __half hi = __float2half_rn(mid), lo = __float2half_rn(mid - __half2float(hi));
                             tab[j * S::CHUNK + 32 * y + tab_at] = __low2half(__hmul2_rn(aq_h2(dm[y][j]), d_scale));
                             tab[(G4 + j) * S::CHUNK + 32 * y + tab_at] = hi;
@@ -615,8 +623,8 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                         }
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
-                            om[nb][0] += acc[nb][0];
-                            om[nb][1] += acc[nb][1];
+                            om[nb][0] = fmaf(acc[nb][0], mid_down, om[nb][0]);
+                            om[nb][1] = fmaf(acc[nb][1], mid_down, om[nb][1]);
                         }
                     }
                     const uint8_t *key_row = vb + 2 * t * ROW + 4 + 2 * g;

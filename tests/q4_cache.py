@@ -102,6 +102,37 @@ class Cache:
                 off[b * tokens + t] = (2 * (e + len(keys) * 2.0 ** -24) + 2.0 ** -20).repeat(hd, -1).reshape(heads, hd) * va.max(1)[:, None].repeat(group, 1).reshape(heads, hd)
         return out.reshape(len(q), -1), off.reshape(len(q), -1)
 
+    def attention_weighed(self, q, tokens, heads, window=0):
+        """As attention, with a bound in which every key counts by its weight and each channel by its own block.
+
+        With z = |m| + 16 |d| for a block (the two terms d (code - 8) and m + 8 d that a value is made of are smaller together), w the weights relative to the largest and l
+        their sum: a score that is off by e (the bound above) changes the result by w e (z + Z) / l, Z the mean of z; so do n roundings of the sums, and 2^-20 for the exponential,
+        the scaling and the two fp16 pieces of weights, steps and middles, 22 bits each.  What is lost whatever the weight: a weight's pieces end at 2^-25 where the largest is 2^10 or
+        more, 2^-35 z; the product of weight and step, rounded to two pieces that end at 2^-25 each, where the step is 2^-10 or more: 8 * 2^-24 / 2^10 * 2^10 |d| = 2^-21 |d|, or less than
+        2^-32 z where the step is smaller than that, but z among the largest."""
+        hd, group = self.head_dim, heads // self.kv_heads
+        out, off = np.zeros((len(q), heads, hd)), np.zeros((len(q), heads, hd))
+        for b in range(len(self.lens)):
+            for t in range(tokens):
+                pos = self.length(b) - tokens + t
+                keys = [p for p in range(max(0, pos - window + 1) if window else 0, pos + 1) if self.place(b, p)]
+                if not keys:
+                    continue
+                rk, rv = self.rows(b, keys, self.k), self.rows(b, keys, self.v)
+                k, v, ka = values(rk), values(rv), magnitudes(rk)
+                dm = np.abs(np.ascontiguousarray(rv.reshape(*rv.shape[:-1], -1, BLOCK)[..., :4]).view(np.float16).astype(np.float64)).repeat(32, -2)
+                d, z = dm[..., 0], dm[..., 1] + 16 * dm[..., 0]
+                x = q[b * tokens + t].astype(np.float64).reshape(self.kv_heads, group, hd)
+                s = np.einsum("hgd,hnd->hgn", x, k) / np.sqrt(hd)
+                w = np.exp(s - s.max(-1, keepdims=True))
+                total = w.sum(-1, keepdims=True)
+                e = np.einsum("hgd,hnd->hgn", np.abs(x), ka) / np.sqrt(hd) * (hd * 2.0 ** -24 + 2.0 ** -21)
+                rel = w * (2 * e + 2 * len(keys) * 2.0 ** -24 + 2.0 ** -20)
+                mean = np.einsum("hgn,hnd->hgd", w, z) / total
+                out[b * tokens + t] = (np.einsum("hgn,hnd->hgd", w, v) / total).reshape(heads, hd)
+                off[b * tokens + t] = ((np.einsum("hgn,hnd->hgd", rel, z) + rel.sum(-1, keepdims=True) * mean + (2.0 ** -21 * d + 2.0 ** -32 * z).sum(1)[:, None]) / total).reshape(heads, hd)
+        return out.reshape(len(q), -1), off.reshape(len(q), -1)
+
 
 class Tables:
     """Page tables, lengths and reference counts under the calls of the header; `pool` [planes][pages] is any array of page contents."""

@@ -484,3 +484,38 @@ def test_results_do_not_change_from_run_to_run(gpu):
     dev = Device(gpu, c)
     first = dev.attention(q, 1, 16)
     assert all(np.array_equal(first, dev.attention(q, 1, 16)) for _ in range(5))
+
+
+def within(got, want, off):
+    """Blocks that the store holds to be beyond fp16 read as NaN, in the channels that they are in; everything else is within its bound."""
+    spoilt = np.isnan(want)
+    assert np.array_equal(np.isnan(got), spoilt)
+    far = np.where(spoilt, 0, np.abs(got - want) / np.where(spoilt, 1, np.maximum(off, 1e-300)))
+    assert far.max() <= 1, f"{(far > 1).sum()} of {far.size}, the worst {far.max():.3g} times what is allowed"
+
+
+def set_values(c, b, pos, block, x):
+    """Block `block` of the value row at a position, of every kv head, holds x."""
+    page, slot = c.place(b, pos)
+    c.v[page, :, slot, block * BLOCK:(block + 1) * BLOCK] = host.quantize(np.asarray(x, dtype=np.float32))
+
+
+WIDE = {"from zero": np.linspace(0, 150000, 32), "high": np.linspace(60000, 72000, 32), "both": np.linspace(-60000, 390000, 32),
+        "largest": np.linspace(65000, 1040000, 32)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", WIDE)
+@pytest.mark.parametrize("heads,head_dim,tokens", [(4, 64, 1), (8, 128, 1), (4, 128, 5), (2, 64, 6), (12, 256, 1)])
+def test_value_blocks_beyond_half_precision(gpu, kind, heads, head_dim, tokens):
+    """A value block whose step and least value are fp16 numbers, but whose middle is not, is read as what it says by the tokens that see it, and does not reach the
+    others: those before it, and those whose window has passed it although it lies in the same 32 keys as some that they see."""
+    rng = np.random.default_rng(head_dim + tokens)
+    for at, window in ((70, 0), (89, 0), (64, 24), (2, 0)):
+        c = random_cache(rng, 2, head_dim, 16, [90])
+        set_values(c, 0, at, 1, WIDE[kind])
+        assert np.isfinite(host.values(c.v[c.place(0, at)[0], :, at % 16])).all()
+        q = rng.standard_normal((tokens, heads * head_dim)).astype(np.float32)
+        got = Device(gpu, c).attention(q, tokens, heads, window)
+        assert np.isfinite(got).all()
+        within(got, *c.attention_weighed(q, tokens, heads, window))
