@@ -10,8 +10,10 @@
 //     subnormal has in leading zeros is lost below: 2e-5 of the result at 500 keys.)
 //   * Value codes are taken from their middle.  With c in place of c - 8 all terms of the sum have one sign, the tensor cores cut what they add to an accumulator
 //     instead of rounding it, and the error adds up: 2.3e-5 of the result at 131072 keys, 7e-7 as it is here.
-//   * Ranges: queries are scaled so that the largest of a row is in [2^14, 2^15), weights, relative to a reference that may lag 2^3 behind the largest, by 2^10, steps d by
-//     2^b with the largest of them so far in [1, 2), middles, which reach 9 * 65504, so that the chunk's largest |m| + 8 |d| is in [2^14, 2^15): no piece passes fp16's range.  A weight times a step is a rounded half-precision product and its exact remainder.
+//   * Ranges: queries are scaled so that the largest of a row is in [2^14, 2^15), weights, relative to a reference that may lag 2^3 behind the largest, by 2^10.  Steps and middles (which
+//     reach 9 * 65504) are scaled chunk by chunk, so that the largest step is below 4 and the largest middle below 2^15: no piece passes fp16's range.  Blocks whose step is about 2^10 below the
+//     chunk's largest would lose bits with that scale.  They are left out of the products and weighed in fp32, key by key, and every block is as exact as it would be alone (32 sequences of up
+//     to 4096 tokens: 51 us without such blocks, 60 us with one key of 64, 262 us with 31 keys of 32).  A weight times a step is a rounded half-precision product and its exact remainder.
 //
 //   scores  S^T = K Q^T   mma.m16n8k16: 16 keys x 8 query rows; a thread's A words are 4 bytes of codes of keys g and g + 8 (lane = 4 g + t), which
 //                         settles which channel sits at which k: the query's fragments are laid out to match
@@ -181,6 +183,31 @@ __device__ __forceinline__ void aq_weigh(uint32_t hi, uint32_t lo, uint32_t d, u
 constexpr float AQ_UNSCALE = 1048576.0f;       // 2^20
 __device__ __forceinline__ float aq_lo(uint32_t dm) { return __low2float(*reinterpret_cast<const __half2 *>(&dm)); }
 __device__ __forceinline__ float aq_hi(uint32_t dm) { return __high2float(*reinterpret_cast<const __half2 *>(&dm)); }
+// For scales (d, m) of the blocks of a lane's key: the biased exponent of the chunk's largest |m| plus eight of its largest |d|, below 2^20 for what the store makes, and
+// the lane's smallest |d|.  Numbers that are none do not count.
+template <int G4>
+__device__ __forceinline__ int aq_size(const uint32_t (&dm)[G4], float &least)
+{
+    __half2 top = __habs2(aq_h2(dm[0])), low = top;
+#pragma unroll
+    for (int j = 1; j < G4; ++j) {
+        top = __hmax2(top, __habs2(aq_h2(dm[j])));
+        low = __hmin2(low, __habs2(aq_h2(dm[j])));
+    }
+    least = __low2float(low);
+    const float size = fmaxf(0.0f, fmaf(8.0f, __low2float(top), __high2float(top)));
+    return max(127 - 24, min(127 + 19, (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(size)) >> 23)));
+}
+// what brings that into [16, 32), and back
+__device__ __forceinline__ float aq_up(int size) { return __uint_as_float((uint32_t)(258 - size) << 23); }
+__device__ __forceinline__ float aq_down(int size) { return __uint_as_float((uint32_t)(size - 4) << 23); }
+// A block that is so much smaller that products with its step (or, where that is zero, with its one value) would lose bits.
+constexpr float AQ_LEAST = 0x1p-10f;
+__device__ __forceinline__ bool aq_late(uint32_t dm, float up)
+{
+    const float d = fabsf(aq_lo(dm)) * up, m = fabsf(aq_hi(dm)) * up;
+    return fmaf(8.0f, d, m) < 2.0f && (d > 0.0f ? d < AQ_LEAST : m > 0.0f && m < 0x1p-13f);
+}
 __device__ __forceinline__ bool aq_no_number(uint32_t dm) { return (dm & 0x7c00u) == 0x7c00u || (dm & 0x7c000000u) == 0x7c000000u; }
 
 template <int HD, int BLOCKS>
@@ -386,7 +413,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
             __syncthreads();
             float om[NB][2];                                   // row g: block g's sum of weight times middle
             float o[NB][G4][2][4], m_run[NB][2], l_run[NB][2], fac[NB][2];      // m_run: the reference of the weights, in powers of two; l_run: of this thread's keys
-            int pos_row[NB][2], b_run = 14;                    // pos_row: the position of a row, -1 where there is none
+            int pos_row[NB][2];                                 // pos_row: the position of a row, -1 where there is none
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -415,62 +442,47 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                     const uint8_t *kb = aq_smem + (warp * STAGES + stage) * S::STAGE, *vb = kb + S::CHUNK * ROW;
                     const bool mixed = there != (1u << S::XT) - 1u || key0 < all_from || key0 + S::CHUNK > all_to;
                     // ---- the values' scales, a lane a key
-                    constexpr int KL = S::CHUNK / 32;
-                    uint32_t dm[KL][G4], dtop = 0;
+                    static_assert(S::CHUNK == 32, "a lane a key");
+                    uint32_t dm[G4];
 #pragma unroll
-                    for (int y = 0; y < KL; ++y)
-#pragma unroll
-                        for (int j = 0; j < G4; ++j) dm[y][j] = aq_u32(vb + (32 * y + lane) * ROW + j * KQ4_BLOCK);
-                    if (mixed) {
+                    for (int j = 0; j < G4; ++j) dm[j] = aq_u32(vb + lane * ROW + j * KQ4_BLOCK);
+                    auto keep_seen = [&](bool mark) {          // in a chunk that not every row sees whole
                         // What no row sees must not reach the products even with weight zero (0 x NaN), what some rows see only those: scales that are no
                         // numbers are taken out, and the rows that see them marked.
-#pragma unroll
-                        for (int y = 0; y < KL; ++y) {
-                            const bool in = (there >> (2 * y + (lane >> 4)) & 1u) && key0 + 32 * y + lane < w.end;
-#pragma unroll
-                            for (int j = 0; j < G4; ++j) {
-                                const bool nan = in && aq_no_number(dm[y][j]);
-                                if (!in || nan) dm[y][j] = 0;
-                                for (uint32_t bad = __ballot_sync(0xffffffffu, nan); bad; bad &= bad - 1) {
-                                    const int at_key = key0 + 32 * y + __ffs(bad) - 1;
-#pragma unroll
-                                    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                                        for (int e = 0; e < 2; ++e) {
-                                            const int pos = pos_row[nb][e];
-                                            if (at_key <= pos && (p.window == 0 || at_key > pos - p.window))
-#pragma unroll
-                                                for (int x = 0; x < 2; ++x) o[nb][j][x][e] = o[nb][j][x][e + 2] = __int_as_float(0x7fffffff);
-                                        }
-                                }
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int y = 0; y < KL; ++y)
-#pragma unroll
-                        for (int j = 0; j < G4; ++j) dtop = max(dtop, (dm[y][j] & 0x7c00u) == 0x7c00u ? 0u : dm[y][j] & 0x7fffu);
-                    // the largest d so far times 2^b is in [1, 2): its products with weights of up to 2^13 stay in fp16's range, their remainders above its least step
-                    const int b_new = min(b_run, 15 - (int)min(29u, max(1u, __reduce_max_sync(0xffffffffu, dtop) >> 10)));
-                    const __half2 d_scale = aq_h2((uint32_t)(15 + b_new) << 10);
-                    // Middles reach nine times the largest half: the chunk's largest |m| + 8 |d|, below 2^20, is brought into [2^14, 2^15), their products back again.
-                    float size = 0.0f;
-#pragma unroll
-                    for (int y = 0; y < KL; ++y)
-#pragma unroll
-                        for (int j = 0; j < G4; ++j) size = fmaxf(size, fabsf(aq_hi(dm[y][j])) + 8.0f * fabsf(aq_lo(dm[y][j])));
-                    const int size_ex = max(127 - 24, min(127 + 19, (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(size)) >> 23)));
-                    const float mid_up = __uint_as_float((uint32_t)(127 + 14 + 127 - size_ex) << 23), mid_down = __uint_as_float((uint32_t)(size_ex - 14) << 23);
-#pragma unroll
-                    for (int y = 0; y < KL; ++y)
+                        const bool in = (there >> (lane >> 4) & 1u) && key0 + lane < w.end;
 #pragma unroll
                         for (int j = 0; j < G4; ++j) {
-                            const float mid = fmaf(8.0f, aq_lo(dm[y][j]), aq_hi(dm[y][j])) * mid_up;
-                            const __half hi = __float2half_rn(mid), lo = __float2half_rn(mid - __half2float(hi));
-                            tab[j * S::CHUNK + 32 * y + tab_at] = __low2half(__hmul2_rn(aq_h2(dm[y][j]), d_scale));
-                            tab[(G4 + j) * S::CHUNK + 32 * y + tab_at] = hi;
-                            tab[(2 * G4 + j) * S::CHUNK + 32 * y + tab_at] = lo;
+                            const bool nan = in && aq_no_number(dm[j]);
+                            if (!in || nan) dm[j] = 0;
+                            if (!mark) continue;
+                            for (uint32_t bad = __ballot_sync(0xffffffffu, nan); bad; bad &= bad - 1) {
+                                const int at_key = key0 + __ffs(bad) - 1;
+#pragma unroll
+                                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) {
+                                        const int pos = pos_row[nb][e];
+                                        if (at_key <= pos && (p.window == 0 || at_key > pos - p.window))
+#pragma unroll
+                                            for (int x = 0; x < 2; ++x) o[nb][j][x][e] = o[nb][j][x][e + 2] = __int_as_float(0x7fffffff);
+                                    }
+                            }
                         }
+                    };
+                    if (mixed) keep_seen(true);
+                    // The chunk's size times `up` is in [16, 32): steps are below 4, so that their products with weights of up to 2^13 stay in fp16's range, middles times 2^10 below 2^15.
+                    float least;
+                    const int size = aq_size(dm, least);
+                    const float up = aq_up(size);
+                    const bool small = least * up < AQ_LEAST;      // there may be blocks that do not go with this scale
+#pragma unroll
+                    for (int j = 0; j < G4; ++j) {
+                        const float d = aq_lo(dm[j]) * up, mid = fmaf(8192.0f, d, aq_hi(dm[j]) * (1024.0f * up));
+                        const __half hi = __float2half_rn(mid);
+                        tab[j * S::CHUNK + tab_at] = __float2half_rn(d);
+                        tab[(G4 + j) * S::CHUNK + tab_at] = hi;
+                        tab[(2 * G4 + j) * S::CHUNK + tab_at] = __float2half_rn(mid - __half2float(hi));
+                    }
                     // ---- scores of tiles of 16 keys.  A product waits long for the one before it in its sum: those of several tiles and blocks take turns.
                     float s[S::XT][NB][4];                     // keys 16 x + g and 8 further on, rows col and col + 1
                     {
@@ -533,7 +545,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                     }
                     // ---- weights times 2^10, as two pieces.  The reference follows the maximum when that is more than 2^3 ahead: each time costs every accumulator a product,
                     // and only then the maximum over the keys is found.
-                    bool moved = b_new != b_run;
+                    bool moved = false;
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
                         if constexpr (PACK) {                  // what hi and lo pieces gave, columns c and c + 4
@@ -560,8 +572,6 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                         }
                     }
                     if (__any_sync(0xffffffffu, moved)) {      // rare once the first keys have been seen
-                        const float shift = __uint_as_float((uint32_t)(127 + b_new - b_run) << 23);
-                        b_run = b_new;
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
                             float alpha[2];
@@ -578,7 +588,6 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                                 m_run[nb][e] = m_new;
                                 l_run[nb][e] *= alpha[e];
                                 om[nb][e] *= alpha[e];
-                                alpha[e] *= shift;
                             }
 #pragma unroll
                             for (int e = 0; e < G4 * 8; ++e) o[nb][e >> 3][e >> 2 & 1][e & 3] *= alpha[e & 1];
@@ -605,6 +614,58 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                     // ---- values.  The tensor cores cut what they add to an accumulator instead of rounding it: a chunk's sums start from zero and are
                     // added up by the rounding adder, and codes are taken from their middle, so that the terms do not all have one sign.
                     const uint8_t *at_t = reinterpret_cast<const uint8_t *>(tab) + 8 * t;
+                    if (__any_sync(0xffffffffu, small)) {
+                        // Blocks that would lose bits beside the chunk's largest leave the table; their values are weighed in fp32, key by key.
+#pragma unroll
+                        for (int j = 0; j < G4; ++j) dm[j] = aq_u32(vb + lane * ROW + j * KQ4_BLOCK);
+                        if (mixed) keep_seen(false);
+                        uint32_t mine = 0;
+#pragma unroll
+                        for (int j = 0; j < G4; ++j) {
+                            if (!aq_late(dm[j], aq_up(size))) continue;
+                            mine |= 1u << j;
+#pragma unroll
+                            for (int i = 0; i < 3; ++i) tab[(i * G4 + j) * S::CHUNK + tab_at] = __float2half_rn(0.0f);
+                        }
+#pragma unroll 1
+                        for (uint32_t keys = __ballot_sync(0xffffffffu, mine != 0); keys; keys &= keys - 1) {
+                            const int key = __ffs(keys) - 1;
+                            const uint32_t of_key = __shfl_sync(0xffffffffu, mine, key);
+                            float weight[NB][2];               // of rows col and col + 1
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) {
+                                uint32_t hi = 0, lo = 0;
+#pragma unroll
+                                for (int y = 0; y < 2 * S::XT; ++y) {      // by masks: an array that is indexed would lie in memory
+                                    const uint32_t is = key >> 3 == y ? 0xffffffffu : 0u;
+                                    hi |= ph[nb][y] & is;
+                                    lo |= pl[nb][y] & is;
+                                }
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const int from = 4 * (col + e) + (key >> 1 & 3);
+                                    const uint32_t h = __shfl_sync(0xffffffffu, hi, from), l = __shfl_sync(0xffffffffu, lo, from);
+                                    weight[nb][e] = PACK && t >= 2 ? 0.0f : (key & 1 ? aq_hi(h) + aq_hi(l) : aq_lo(h) + aq_lo(l));
+                                }
+                            }
+#pragma unroll
+                            for (int j = 0; j < G4; ++j) {
+                                if (!(of_key >> j & 1u)) continue;
+                                const uint8_t *at = vb + key * ROW + j * KQ4_BLOCK;
+                                const uint32_t scales = aq_u32(at), codes = aq_u16(at + 4 + 2 * g);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {  // byte e / 2, nibble e % 2
+                                    const float v = fmaf(aq_lo(scales), (float)(codes >> 4 * e & 15u), aq_hi(scales));
+#pragma unroll
+                                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                                        for (int r = 0; r < 2; ++r) o[nb][j][e >> 1][2 * (e & 1) + r] = fmaf(weight[nb][r], v, o[nb][j][e >> 1][2 * (e & 1) + r]);
+                                }
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    const float down = aq_down(size);
                     {
                         float acc[NB][4];
 #pragma unroll
@@ -623,8 +684,8 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                         }
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) {
-                            om[nb][0] = fmaf(acc[nb][0], mid_down, om[nb][0]);
-                            om[nb][1] = fmaf(acc[nb][1], mid_down, om[nb][1]);
+                            om[nb][0] = fmaf(acc[nb][0], down, om[nb][0]);
+                            om[nb][1] = fmaf(acc[nb][1], down, om[nb][1]);
                         }
                     }
                     const uint8_t *key_row = vb + 2 * t * ROW + 4 + 2 * g;
@@ -672,7 +733,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] += acc[nb][e >> 2][e & 3];
+                            for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] = fmaf(acc[nb][e >> 2][e & 3], down, o[nb][j][e >> 2][e & 3]);
                     }
                 }
                 __syncwarp();                                  // the stage and its word and the table are free again
@@ -690,7 +751,6 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                 aq_next_stretch(p, ROWS, S::UNIT, w);
                 if (S::EARLY) load_q();
             }
-            const float unscale = __uint_as_float((uint32_t)(127 - b_run) << 23);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -702,7 +762,7 @@ __global__ void __launch_bounds__(AQ_THREADS, AqShape<HD, BLOCKS>::CTAS) attn_q4
                 for (int j = 0; j < G4; ++j) {
                     const float a0 = __shfl_sync(0xffffffffu, om[nb][0], 4 * j + t), a1 = __shfl_sync(0xffffffffu, om[nb][1], 4 * j + t);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] = fmaf(o[nb][j][e >> 2][e & 3], unscale, e & 1 ? a1 : a0);
+                    for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] += (e & 1 ? a1 : a0) * 0x1p-10f;
                     if constexpr (PACK) {                      // what hi and lo pieces gave, column c and c + 4
 #pragma unroll
                         for (int e = 0; e < 8; ++e) o[nb][j][e >> 2][e & 3] += __shfl_xor_sync(0xffffffffu, o[nb][j][e >> 2][e & 3], 2);

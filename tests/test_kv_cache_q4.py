@@ -522,6 +522,52 @@ def test_value_blocks_beyond_half_precision(gpu, kind, heads, head_dim, tokens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("ratio", [13, 18, 26])
+@pytest.mark.parametrize("heads,head_dim,tokens", [(4, 64, 1), (8, 128, 1), (4, 128, 5), (2, 96, 6), (12, 256, 1)])
+def test_value_blocks_of_very_different_steps(gpu, heads, head_dim, tokens, ratio):
+    """Steps of one channel block, of one key that has next to no weight, and of one key that only the last token sees, are 2^ratio times those of the rest: what is made of the rest
+    is as exact as without them."""
+    rng = np.random.default_rng(head_dim + ratio)
+    low = np.float32(2.0 ** -12)
+    for kind in ("block", "key", "last"):
+        c = random_cache(rng, 2, head_dim, 16, [100])
+        for pos in range(100):
+            page, slot = c.place(0, pos)
+            c.v[page, :, slot] = host.quantize(rng.standard_normal((2, head_dim)).astype(np.float32) * low)
+            if kind == "block":
+                set_values(c, 0, pos, 0, rng.standard_normal(32) * low * 2.0 ** ratio)
+        q = (rng.standard_normal((tokens, heads * head_dim)) * 0.05).astype(np.float32)
+        large = host.quantize(rng.standard_normal((2, head_dim)).astype(np.float32) * low * np.float32(2.0 ** ratio))
+        if kind == "key":                                       # its scores are -60 and less: all queries have a part along it
+            q.reshape(tokens, heads, head_dim)[..., 0] = 2.0
+            page, slot = c.place(0, 9)
+            k = np.zeros((2, head_dim), dtype=np.float32)
+            k[:, 0] = -30 * np.sqrt(head_dim)
+            c.k[page, :, slot], c.v[page, :, slot] = host.quantize(k), large
+        elif kind == "last":
+            page, slot = c.place(0, 99)
+            c.v[page, :, slot] = large
+        within(Device(gpu, c).attention(q, tokens, heads), *c.attention_weighed(q, tokens, heads))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,head_dim,tokens,window", [(4, 64, 1, 0), (8, 128, 1, 0), (16, 128, 3, 0), (8, 256, 2, 40)])
+def test_value_blocks_of_all_magnitudes(gpu, heads, head_dim, tokens, window):
+    """Each block of each key has a magnitude of its own between 2^-20 and 2^15, some are all one number, some all zero."""
+    rng = np.random.default_rng(heads + head_dim)
+    c = random_cache(rng, 2, head_dim, 16, [150, 31])
+    for b, n in enumerate(c.lens):
+        for pos in range(int(n)):
+            x = rng.standard_normal((2, head_dim // 32, 32)) * 2.0 ** rng.integers(-20, 16, (2, head_dim // 32, 1))
+            x = np.where(rng.random((2, head_dim // 32, 1)) < 0.1, x[..., :1], x)
+            x = np.where(rng.random((2, head_dim // 32, 1)) < 0.1, 0, x)
+            page, slot = c.place(b, pos)
+            c.v[page, :, slot] = host.quantize(x.reshape(2, head_dim).astype(np.float32))
+    q = (rng.standard_normal((2 * tokens, heads * head_dim)) * 0.5).astype(np.float32)
+    within(Device(gpu, c).attention(q, tokens, heads, window), *c.attention_weighed(q, tokens, heads, window))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("heads,head_dim,tokens", [(4, 64, 1), (8, 128, 1), (4, 128, 5), (16, 64, 1)])
 def test_long_sequences_of_distinct_rows(gpu, heads, head_dim, tokens):
     """70001 rows, no two alike, against torch in 64 bits: 3e-6 of the result's norm, a dozen roundings to the 22 bits of two fp16 pieces."""
