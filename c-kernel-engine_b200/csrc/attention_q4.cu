@@ -56,7 +56,7 @@ struct AqShape {
     static constexpr int NB = PACK || FOUR ? 1 : BLOCKS, G4 = HD / 32, KS = HD / 16, ROW = G4 * KQ4_BLOCK, ROWS = PACK ? 4 : 8 * NB;
     static constexpr int XT = 2, CHUNK = 16 * XT, UNIT = AQ_WARPS * CHUNK;      // a warp takes XT tiles of 16 keys at a time
     static constexpr int STAGE = 2 * CHUNK * ROW;                              // K rows, then V rows
-    static constexpr int CTAS = NB > 1 && HD > 192 ? 1 : (NB > 1 || HD > 128 ? 2 : (FOUR ? 4 : 3));                       // resident on an SM, for which registers and shared memory are kept
+    static constexpr int CTAS = NB > 1 || HD > 128 ? 2 : (FOUR ? 4 : 3);                       // resident on an SM, for which registers and shared memory are kept
     static constexpr int STAGES = HD <= 64 ? 4 : (HD <= 128 && NB < 3 && !FOUR ? 3 : 2);
     // the next stretch's queries load while one is joined, where there are registers: three blocks 96.7 us with it and 93.9 us without (20 rows of 16 sequences), four rows 190 and 188 us
     static constexpr bool EARLY = !PACK && NB < 3;
@@ -1021,9 +1021,10 @@ static size_t aq_bytes(int batch, int Hkv, int R)
 }
 
 // Blocks of 8 query rows that share the codes a CTA unpacks; 0: up to four, with both pieces of a row in one product (32 heads over 8, four sequences of 131072
-// tokens 180 us, 217 us in a block of 8; 32 of up to 4096 46 and 53).  Three blocks leave no register free and are worth it only where they hold all the rows: 20 rows of
-// 16 sequences (five drafts, up to 8190 tokens) 94 us with three, 109 us one by one, 130 us with two and two; 516 rows 38 us in blocks of two, 42 us one by one, 41 us in threes.
-static int aq_blocks(long long rows, int hd) { return rows <= 4 ? 0 : rows <= 8 ? 1 : (rows > 16 && rows <= 24 && hd <= 128 ? 3 : 2); }
+// tokens 186 us, 213 us in a block of 8; 32 of up to 4096 47 and 52).  Three blocks leave no register free and are worth it only where they hold all the rows: 20 rows of
+// 16 sequences (five drafts, up to 8190 tokens) 96 us with three, 108 us one by one, 128 us with two and two; 516 rows 39 us in blocks of two, 42 us one by one, 41 us in threes.
+// Above 128 channels two blocks leave one CTA an SM (256) or spill (192): 16 rows of 8 sequences of 4096 tokens 24 us one by one and 30 us in twos (192: 19 and 21), 516 rows behind 1024 42 and 58 (32 and 38).
+static int aq_blocks(long long rows, int hd) { return rows <= 4 ? 0 : rows <= 8 || hd > 128 ? 1 : (rows > 16 && rows <= 24 ? 3 : 2); }
 
 // Eight rows of 128 channels: four CTAs an SM, with 128 registers a thread, hide more of the waiting than three with 168, but take longer for a chunk: 210 and 218 us for four sequences
 // of 131072 tokens, 53 and 54 us for 32 of up to 4096, 40 and 44 us for 48 of up to 2047, but 35 and 35 us for 16 of up to 4096, 24 and 23 us for 8, 19 and 16 us for 4, 76 and 72 us for 256 of up to
@@ -1038,8 +1039,8 @@ using namespace ckb;
     (hd == 64 ? (nb == 0 ? F<64, 0> : nb == 1 ? F<64, 1> : nb == 2 ? F<64, 2> : F<64, 3>)                               \
      : hd == 96 ? (nb == 0 ? F<96, 0> : nb == 1 ? F<96, 1> : nb == 2 ? F<96, 2> : F<96, 3>)                             \
      : hd == 128 ? (nb == 0 ? F<128, 0> : nb == 1 ? F<128, 1> : nb == 2 ? F<128, 2> : nb == 3 ? F<128, 3> : F<128, 4>)                        \
-     : hd == 192 ? (nb == 0 ? F<192, 0> : nb == 1 ? F<192, 1> : F<192, 2>)                                              \
-                 : (nb == 0 ? F<256, 0> : nb == 1 ? F<256, 1> : F<256, 2>))
+     : hd == 192 ? (nb == 0 ? F<192, 0> : F<192, 1>)                                                                    \
+                 : (nb == 0 ? F<256, 0> : F<256, 1>))
 
 extern "C" size_t ckb200_attention_q4cache_workspace_bytes(int batch, int num_tokens, int num_heads, int num_kv_heads, int head_dim)
 {
