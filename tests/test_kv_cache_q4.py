@@ -568,6 +568,28 @@ def test_value_blocks_of_all_magnitudes(gpu, heads, head_dim, tokens, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,head_dim,page_tokens,lens,tokens,window,columns", [
+    (16, 2, 128, 16, [150, 33, 0, 700] + [(29 * i) % 90 for i in range(16)], 1, 0, 960),      # four CTAs an SM
+    (7, 1, 128, 64, [300, 64], 1, 50, 1), (24, 3, 64, 48, [200, 5], 3, 0, 1), (9, 1, 96, 16, [70], 2, 33, 1), (4, 2, 192, 16, [90, 200], 4, 0, 1), (3, 3, 192, 32, [130], 1, 0, 1),
+    (20, 2, 256, 16, [60, 40], 2, 0, 1), (4, 1, 128, 32, [2500], 1, 0, 1), (6, 1, 64, 16, [40], 40, 7, 1)])
+def test_magnitudes_in_every_form(gpu, heads, kv_heads, head_dim, page_tokens, lens, tokens, window, columns):
+    """The same for every number of rows and channels, with pages missing, a page that does not exist and windows; steps of neighbours 2^-24 to 2^15 apart, some blocks no numbers."""
+    rng = np.random.default_rng(heads + 7 * head_dim)
+    c = random_cache(rng, kv_heads, head_dim, page_tokens, lens, extra_columns=columns, hole=True)
+    for b, n in enumerate(lens):
+        for pos in range(n):
+            at = c.place(b, pos)
+            if not at:
+                continue
+            x = rng.standard_normal((kv_heads, head_dim // 32, 32)) * 2.0 ** rng.choice([-20, -13, -12, 0, 1, 2, 2, 2, 13], (kv_heads, head_dim // 32, 1))
+            c.v[at[0], :, at[1]] = host.quantize((x + 10.0 * rng.standard_normal(x.shape[:2] + (1,)) * (rng.random(x.shape[:2] + (1,)) < 0.1)).reshape(kv_heads, head_dim).astype(np.float32))
+            if rng.random() < 0.004:
+                c.v[at[0], :, at[1], :4] = 255
+    q = (rng.standard_normal((len(lens) * tokens, heads * head_dim)) * 0.3).astype(np.float32)
+    within(Device(gpu, c).attention(q, tokens, heads, window), *c.attention_weighed(q, tokens, heads, window))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("heads,head_dim,tokens", [(4, 64, 1), (8, 128, 1), (4, 128, 5), (16, 64, 1)])
 def test_long_sequences_of_distinct_rows(gpu, heads, head_dim, tokens):
     """70001 rows, no two alike, against torch in 64 bits: 3e-6 of the result's norm, a dozen roundings to the 22 bits of two fp16 pieces."""
