@@ -31,10 +31,10 @@
 // written out at once, the others as partial results that a second kernel joins (log-sum-exp).
 //
 // What bounds it.  Not HBM: the ring alone, without the arithmetic, takes 113 us for four sequences of 131072 tokens (64 heads over 8 of 128 channels,
-// 667 MB, 102 us at the measured copy rate), the whole kernel 210 us, 3.2 TB/s (32 heads: 180 us, 3.7 TB/s).  A chunk of 32 keys is 1060 warp instructions, 74 of them
+// 667 MB, 102 us at the measured copy rate), the whole call 215 us, 3.1 TB/s (32 heads: 187 us, 3.6 TB/s).  A chunk of 32 keys is 1045 warp instructions, 74 of them
 // products (38 with four rows), issued at 2.5 an SM and cycle: products, half-precision instructions and integer multiplications share one pipe, half-rate logic (codes, 300
-// instructions) has another, each is busy for 20 to 40 % of the time, and a warp waits 1.7 cycles an instruction for the one before it.
-// Two, three or four CTAs an SM (8 to 16 warps, 255 to 128 registers): 239 / 218 / 210 us.
+// instructions) has another, each is busy for 20 to 40 % of the time, and a warp waits 1.8 cycles an instruction for the one before it.
+// Two, three or four CTAs an SM (8 to 16 warps, 255 to 128 registers): 235 / 215 / 207 us inside a graph.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -58,7 +58,7 @@ struct AqShape {
     static constexpr int STAGE = 2 * CHUNK * ROW;                              // K rows, then V rows
     static constexpr int CTAS = NB > 1 || HD > 128 ? 2 : (FOUR ? 4 : 3);                       // resident on an SM, for which registers and shared memory are kept
     static constexpr int STAGES = HD <= 64 ? 4 : (HD <= 128 && NB < 3 && !FOUR ? 3 : 2);
-    // the next stretch's queries load while one is joined, where there are registers: three blocks 96.7 us with it and 93.9 us without (20 rows of 16 sequences), four rows 190 and 188 us
+    // the next stretch's queries load while one is joined, where there are registers: three blocks 97 us with it and 96 us without (20 rows of 16 sequences), four rows 187 and 186 us
     static constexpr bool EARLY = !PACK && NB < 3;
     static constexpr int MINE = NB * G4 * 2;                                  // each warp joins a quarter of the four warps' accumulators; it gives away the others
     static constexpr int GIVEN = AQ_WARPS * (3 * MINE * 32 + NB * 16) * 4;
@@ -1026,9 +1026,11 @@ static size_t aq_bytes(int batch, int Hkv, int R)
 // Above 128 channels two blocks leave one CTA an SM (256) or spill (192): 16 rows of 8 sequences of 4096 tokens 24 us one by one and 30 us in twos (192: 19 and 21), 516 rows behind 1024 42 and 58 (32 and 38).
 static int aq_blocks(long long rows, int hd) { return rows <= 4 ? 0 : rows <= 8 || hd > 128 ? 1 : (rows > 16 && rows <= 24 ? 3 : 2); }
 
-// Eight rows of 128 channels: four CTAs an SM, with 128 registers a thread, hide more of the waiting than three with 168, but take longer for a chunk: 210 and 218 us for four sequences
-// of 131072 tokens, 53 and 54 us for 32 of up to 4096, 40 and 44 us for 48 of up to 2047, but 35 and 35 us for 16 of up to 4096, 24 and 23 us for 8, 19 and 16 us for 4, 76 and 72 us for 256 of up to
-// 600.  So they are taken where the table has room for eight units a CTA and sixteen a stretch.
+// Eight rows of 128 channels: four CTAs an SM, with 128 registers a thread, hide more of the waiting than three with 168, but take longer for a chunk.  They are taken where the table has
+// room for eight units a CTA and sixteen a stretch.  Of lengths the host sees the table's columns alone.  With tables that just fit (four and three CTAs, inside a graph, 64 heads over 8): four
+// sequences of 131072 tokens 207 and 215 us, 128 of up to 3000 113 and 117, 32 of up to 4096 52 and 53, 48 of up to 2047 37 and 38; the rule leaves 16 of up to 4096 (26.4 and 26.2), 8 (21.7 and 19.0),
+// 4 (17.6 and 16.6) and 256 of up to 600 (74 and 73) to three.  With tables that have room for 131072 tokens it takes four for these too: 26.5 and 26.2 us, 22.1 and 18.8, 17.7 and 16.6, 74 and 73; one of 20000 20.6
+// and 18.4, two of up to 8000 13.8 and 15.3.
 static bool aq_four(long long stretches, int units, int hd) { return hd == 128 && units >= 16 && stretches * units >= 8LL * 4 * ckb_sm_count(); }
 
 }  // namespace ckb
