@@ -62,7 +62,8 @@ int ckb200_dev_rope_kv_store_q4(float *q, const float *k, const float *v, void *
  * tokens' own rows among it: attention_forward_decode_head_major_gqa_flash_f16cache (src/kernels/attention_kernels.c:3450-3557) over Q4_1 rows.
  * q, out: rows of [num_heads][head_dim] floats, q_stride and out_stride floats apart; scale 1 / sqrt(head_dim).  The token at position p sees keys
  * max(0, p - sliding_window + 1) .. p (sliding_window 0: 0 .. p); one that sees none gets zeros.  num_heads is a multiple of num_kv_heads.
- * Queries, weights, steps and middles (m + 8 d) enter products as two fp16 pieces, 22 bits, sums are fp32; a weight is held to 2^-35 of its row's largest.
+ * Queries, weights, steps and middles (m + 8 d) enter products as two fp16 pieces, 22 bits, sums are fp32.  Pieces end at 2^-35 of its row's largest for a weight, at 2^-39 of it for a query's
+ * channel and at 2^-33 of it for the sum of 32 channels that goes with m.
  * `workspace`: ckb200_attention_q4cache_workspace_bytes() bytes of any content, aligned to 16; not shared by calls that may run at once. */
 size_t ckb200_attention_q4cache_workspace_bytes(int batch, int num_tokens, int num_heads, int num_kv_heads, int head_dim);
 int ckb200_dev_attention_q4cache(const float *q, long long q_stride, const void *k_pages, const void *v_pages, float *out, long long out_stride, const int *page_table,
